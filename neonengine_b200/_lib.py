@@ -52,6 +52,17 @@ class NeonPtConfig(ctypes.Structure):
     _fields_ = [("width", c_int), ("height", c_int), ("n_lights", c_int), ("device", c_int)]
 
 
+class NeonKv4Config(ctypes.Structure):
+    """Mirror of ``neon_kv4_config`` (include/neon_kv4.h)."""
+    _fields_ = [("n_q_heads", c_int), ("n_kv_heads", c_int), ("head_dim", c_int), ("page_size", c_int), ("device", c_int)]
+
+
+class NeonKv4Batch(ctypes.Structure):
+    """Mirror of ``neon_kv4_batch``."""
+    _fields_ = [("seq_lens", c_void_p), ("cu_q", c_void_p), ("page_table", c_void_p), ("table_stride", ctypes.c_int64),
+                ("table_width", c_int), ("batch", c_int), ("n_pages", ctypes.c_int64)]
+
+
 # name -> (restype, argtypes); must list every symbol include/neon_pt.h declares
 PT_SIGNATURES = {
     "neon_pt_create": (c_int, [ctypes.POINTER(NeonPtConfig), c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, ctypes.POINTER(c_void_p)]),
@@ -113,6 +124,22 @@ DECODER_SIGNATURES = {
     "neon_decoder_step_bytes": (c_int, [c_void_p, c_void_p, c_int, ctypes.POINTER(ctypes.c_double)]),
 }
 
+# name -> (restype, argtypes); must list every symbol include/neon_kv4.h declares
+KV4_SIGNATURES = {
+    "neon_kv4_create": (c_int, [ctypes.POINTER(NeonKv4Config), ctypes.POINTER(c_void_p)]),
+    "neon_kv4_destroy": (c_int, [c_void_p]),
+    "neon_kv4_last_error": (ctypes.c_char_p, [c_void_p]),
+    "neon_kv4_record_bytes": (ctypes.c_int64, [c_void_p]),
+    "neon_kv4_append": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int] + [c_void_p, ctypes.c_int64] * 3
+                        + [c_void_p, ctypes.c_float, c_void_p, c_int, c_void_p]),
+    "neon_kv4_read": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_void_p]),
+    "neon_kv4_attend_workspace": (ctypes.c_uint64, [c_void_p, c_void_p, c_int, c_int]),
+    "neon_kv4_attend": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, ctypes.c_int64, c_void_p, c_int, ctypes.c_float, c_int,
+                                c_void_p, c_void_p, ctypes.c_uint64, c_void_p]),
+    "neon_kv4_status": (c_int, [c_void_p, ctypes.POINTER(c_int)]),
+    "neon_kv4_launch_count": (ctypes.c_int64, [c_void_p]),
+}
+
 # name -> (restype, argtypes); must list every symbol include/neon_moe.h declares
 SIGNATURES = {
     "neon_moe_create": (c_int, [ctypes.POINTER(NeonMoeConfig), ctypes.POINTER(c_void_p)]),
@@ -162,7 +189,8 @@ def load() -> ctypes.CDLL:
         raise ImportError(f"{SO_PATH} is missing: build it with `python -m neonengine_b200.build` "
                           "(there is no CPU fallback)")
     lib = ctypes.CDLL(SO_PATH)
-    for name, (res, args) in {**SIGNATURES, **DECODER_SIGNATURES, **WATER_SIGNATURES, **SVGF_SIGNATURES, **PT_SIGNATURES}.items():
+    for name, (res, args) in {**SIGNATURES, **DECODER_SIGNATURES, **WATER_SIGNATURES, **SVGF_SIGNATURES, **PT_SIGNATURES,
+                              **KV4_SIGNATURES}.items():
         fn = getattr(lib, name)  # AttributeError if a declared symbol is not exported
         fn.restype = res
         fn.argtypes = args

@@ -1,0 +1,20 @@
+// What other parts of the library call of the 4-bit paged cache (neon_kv4.cu).
+#pragma once
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace neon {
+namespace kv4 {
+struct Shape;
+struct Batch;
+struct AppendParams;
+
+// Opts the attention kernels into their shared memory on the current device.
+cudaError_t configure_attend();
+// Each enqueues on `st` and returns the number of kernels launched.  Arguments as in neon_kv4.h, checked by the caller.
+int launch_append(const AppendParams& p, int dtype, int out_dtype, cudaStream_t st);
+uint64_t attend_workspace(const Shape& s, const Batch& b, int max_rows);
+int launch_attend(const Shape& s, const Batch& b, const uint8_t* cache, int dtype, const void* q, long long q_stride, const uint16_t* sinks,
+                  int window, float scale, int max_rows, void* out, float* workspace, cudaStream_t st);
+}  // namespace kv4
+}  // namespace neon

@@ -1,0 +1,302 @@
+// Host side of the 4-bit paged cache declared in include/neon_kv4.h: checks arguments, picks the kernel variant and
+// enqueues it.  No CPU fallback exists: a call launches CUDA kernels or fails with an error code.
+#include "../../include/neon_kv4.h"
+
+#include <algorithm>
+#include <atomic>
+#include <cmath>
+#include <cstdarg>
+#include <cstdio>
+#include <new>
+#include <string>
+
+#include "kv4_append.cuh"
+#include "kv4_attend.cuh"
+#include "kv4_launch.h"
+
+using namespace neon;
+using namespace neon::kv4;
+
+struct neon_kv4_handle {
+    neon_kv4_config cfg{};
+    Shape shape{};
+    std::string err;
+    int* status = nullptr;
+    std::atomic<int64_t> launches{0};
+};
+
+namespace {
+thread_local std::string g_create_error;
+
+int fail(neon_kv4_handle* h, int code, const char* fmt, ...) {
+    char buf[512];
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(buf, sizeof buf, fmt, ap);
+    va_end(ap);
+    if (h) h->err = buf; else g_create_error = buf;
+    return code;
+}
+
+// Makes the handle's device current for a scope and the caller's again after it.
+struct OnDevice {
+    int before = -1;
+    bool ok;
+    explicit OnDevice(int device) {
+        ok = cudaGetDevice(&before) == cudaSuccess && (before == device || cudaSetDevice(device) == cudaSuccess);
+        if (before == device) before = -1;
+    }
+    ~OnDevice() { if (before >= 0) cudaSetDevice(before); }
+};
+
+#define ON_DEVICE(h)                    \
+    OnDevice on_device_((h)->cfg.device); \
+    if (!on_device_.ok) return fail((h), NEON_MOE_ECUDA, "cudaSetDevice(%d) failed", (h)->cfg.device)
+
+int launched(neon_kv4_handle* h, int n) {
+    const cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return fail(h, NEON_MOE_ECUDA, "launch failed: %s", cudaGetErrorString(e));
+    h->launches += n;
+    return NEON_MOE_OK;
+}
+
+bool aligned(const void* p, int64_t stride, int dtype) {
+    const int size = dtype == NEON_KV4_F32 ? 4 : 2;
+    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride * size % 16 == 0;
+}
+
+int check_batch(neon_kv4_handle* h, const neon_kv4_batch* b, const void* cache, int rows) {
+    if (!b || !b->seq_lens || !b->page_table || !cache) return fail(h, NEON_MOE_EINVAL, "null batch, seq_lens, page_table or cache");
+    if (b->batch < 1 || b->batch > NEON_KV4_MAX_BATCH)
+        return fail(h, NEON_MOE_EINVAL, "batch %d outside 1..%d", b->batch, NEON_KV4_MAX_BATCH);
+    if (b->table_width < 1 || b->table_stride < b->table_width || (int64_t)b->table_width * h->cfg.page_size > (1 << 30))
+        return fail(h, NEON_MOE_EINVAL, "page table of %d columns, rows %lld apart", b->table_width, (long long)b->table_stride);
+    if (b->n_pages < 1) return fail(h, NEON_MOE_EINVAL, "a cache of %lld pages", (long long)b->n_pages);
+    if (rows < 0 || (!b->cu_q && rows < b->batch))
+        return fail(h, NEON_MOE_EINVAL, "%d rows for %d sequences of one row each", rows, b->batch);
+    if (reinterpret_cast<uintptr_t>(cache) % 16) return fail(h, NEON_MOE_EINVAL, "the cache is not 16-byte aligned");
+    return NEON_MOE_OK;
+}
+}  // namespace
+
+namespace neon {
+namespace kv4 {
+
+cudaError_t configure_attend() {
+    static std::atomic<bool> done[64];
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess || done[dev & 63]) return e;
+    auto set = [&](const void* k) {
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+    };
+#define SET(D, NT)                                           \
+    set((const void*)attend_kernel<D, NT, __nv_bfloat16>); \
+    set((const void*)attend_kernel<D, NT, __half>);
+    SET(64, 1) SET(64, 2) SET(64, 4) SET(128, 1) SET(128, 2)
+#undef SET
+    if (e == cudaSuccess) done[dev & 63] = true;
+    return e;
+}
+
+namespace {
+constexpr int kSms = 148, kSharedPerSm = 227 * 1024;
+
+// Columns of an item's products: as many query rows as there are, up to 32 (16 at 128 columns, whose outputs take twice
+// the registers): every further group of eight saves reading, converting and scaling the cache once more.
+int column_groups(const Shape& s, int max_rows) {
+    const long long rows = (long long)std::max(max_rows, 1) * (s.nq / s.nkv);
+    if (rows <= 8) return 1;
+    if (rows <= 16 || s.D == 128) return 2;
+    return 4;
+}
+int ctas_per_sm(const Shape& s, int nt) { return s.D == 64 && nt <= 2 ? 2 : 1; }
+int attend_grid(const Shape& s, const Batch& b, int nt) {
+    const long long steps = ((long long)b.width * s.P + kStep - 1) / kStep;
+    const long long blocks = (long long)b.rows * (s.nq / s.nkv) / (8 * nt) + b.n;
+    const long long most = steps * blocks * s.nkv;  // units there can be
+    return (int)std::min<long long>(kSms * ctas_per_sm(s, nt), std::max<long long>(most, 1));
+}
+
+template <int D, int NT, class T>
+void launch_attend_t(AttendParams p, int grid, cudaStream_t st) {
+    using W = WarpSmem<D>;
+    const int before = (p.b.n + 2) / 2 * 16, budget = kSharedPerSm / ctas_per_sm(p.s, NT) - 1024 - before;
+    p.stages = std::min(W::kMaxStages, (budget / kAttendWarps - W::bytes(0)) / W::kRing);
+    attend_kernel<D, NT, T><<<grid, kAttendWarps * 32, before + kAttendWarps * W::bytes(p.stages), st>>>(p);
+    const long long tasks = (long long)p.b.rows * p.s.nq;
+    merge_kernel<D, T><<<(unsigned)((tasks + 7) / 8), 256, before, st>>>(p);
+}
+}  // namespace
+
+uint64_t attend_workspace(const Shape& s, const Batch& b, int max_rows) {
+    const int nt = column_groups(s, max_rows);
+    return (uint64_t)attend_grid(s, b, nt) * kAttendWarps * 2 * 8 * nt * (s.D + 2) * sizeof(float);
+}
+
+int launch_attend(const Shape& s, const Batch& b, const uint8_t* cache, int dtype, const void* q, long long q_stride, const uint16_t* sinks,
+                  int window, float scale, int max_rows, void* out, float* workspace, cudaStream_t st) {
+    AttendParams p{};
+    p.b = b; p.s = s; p.cache = cache; p.q = q; p.q_stride = q_stride; p.sinks = sinks;
+    p.window = window; p.G = s.nq / s.nkv; p.scale = scale; p.out = out; p.part = workspace;
+    const int nt = column_groups(s, max_rows), grid = attend_grid(s, b, nt);
+    p.row_blocks = 8 * nt;
+    p.workers = grid * kAttendWarps;
+#define RUN(DIM, NT)                                                            \
+    if (s.D == DIM && nt == NT) {                                               \
+        if (dtype == NEON_KV4_BF16) launch_attend_t<DIM, NT, __nv_bfloat16>(p, grid, st); \
+        else launch_attend_t<DIM, NT, __half>(p, grid, st);                     \
+    }
+    RUN(64, 1) RUN(64, 2) RUN(64, 4) RUN(128, 1) RUN(128, 2)
+#undef RUN
+    return 2;
+}
+
+int launch_append(const AppendParams& p, int dtype, int out_dtype, cudaStream_t st) {
+    const int units = (p.q ? p.s.nq : 0) * (p.s.D / 16) + 2 * p.s.nkv * (p.s.D / 16);
+    const int threads = std::min(512, std::max(64, (units + 31) / 32 * 32));
+#define RUN(DT)                                                                                  \
+    if (dtype == DT) {                                                                           \
+        if (out_dtype == NEON_KV4_F16) append_kernel<DT, __half><<<p.b.rows, threads, 0, st>>>(p);   \
+        else append_kernel<DT, __nv_bfloat16><<<p.b.rows, threads, 0, st>>>(p);                  \
+    }
+    RUN(NEON_KV4_F32) RUN(NEON_KV4_BF16) RUN(NEON_KV4_F16)
+#undef RUN
+    return 1;
+}
+
+}  // namespace kv4
+}  // namespace neon
+
+extern "C" {
+
+const char* neon_kv4_last_error(const neon_kv4_handle* h) { return h ? h->err.c_str() : g_create_error.c_str(); }
+int64_t neon_kv4_launch_count(const neon_kv4_handle* h) { return h ? h->launches.load() : 0; }
+int64_t neon_kv4_record_bytes(const neon_kv4_handle* h) { return h ? h->shape.record() : 0; }
+
+int neon_kv4_create(const neon_kv4_config* cfg, neon_kv4_handle** out) {
+    if (!cfg || !out) return fail(nullptr, NEON_MOE_EINVAL, "null argument");
+    *out = nullptr;
+    const auto& c = *cfg;
+    if (c.head_dim != 64 && c.head_dim != 128) return fail(nullptr, NEON_MOE_EINVAL, "head_dim must be 64 or 128");
+    if (c.page_size != 16 && c.page_size != 32 && c.page_size != 64) return fail(nullptr, NEON_MOE_EINVAL, "page_size must be 16, 32 or 64");
+    if (c.n_kv_heads < 1 || c.n_kv_heads > 128) return fail(nullptr, NEON_MOE_EINVAL, "n_kv_heads must be 1..128");
+    if (c.n_q_heads < c.n_kv_heads || c.n_q_heads % c.n_kv_heads || c.n_q_heads / c.n_kv_heads > 32)
+        return fail(nullptr, NEON_MOE_EINVAL, "n_q_heads must be 1 to 32 times n_kv_heads");
+    int count = 0;
+    if (cudaGetDeviceCount(&count) != cudaSuccess || c.device < 0 || c.device >= count) {
+        cudaGetLastError();
+        return fail(nullptr, NEON_MOE_ECUDA, "no CUDA device %d", c.device);
+    }
+    auto* h = new (std::nothrow) neon_kv4_handle;
+    if (!h) return fail(nullptr, NEON_MOE_ECUDA, "out of host memory");
+    h->cfg = c;
+    h->shape = {c.n_q_heads, c.n_kv_heads, c.head_dim, c.page_size};
+    OnDevice dev(c.device);
+    if (!dev.ok || cudaMalloc(&h->status, sizeof(int)) != cudaSuccess || cudaMemset(h->status, 0, sizeof(int)) != cudaSuccess ||
+        configure_attend() != cudaSuccess) {
+        const cudaError_t e = cudaGetLastError();
+        if (h->status) cudaFree(h->status);
+        delete h;
+        return fail(nullptr, NEON_MOE_ECUDA, "setting up device %d: %s", c.device, cudaGetErrorString(e));
+    }
+    *out = h;
+    return NEON_MOE_OK;
+}
+
+int neon_kv4_destroy(neon_kv4_handle* h) {
+    if (!h) return NEON_MOE_OK;
+    {
+        OnDevice dev(h->cfg.device);
+        if (dev.ok && h->status) cudaFree(h->status);  // waits for the device
+        cudaGetLastError();
+    }
+    delete h;
+    return NEON_MOE_OK;
+}
+
+static Batch device_batch(const neon_kv4_handle* h, const neon_kv4_batch* b, int rows) {
+    return {b->seq_lens, b->cu_q, b->page_table, b->table_stride, b->n_pages, b->table_width, b->batch, rows, h->status};
+}
+
+int neon_kv4_append(neon_kv4_handle* h, const neon_kv4_batch* batch, void* cache, int rows, int dtype, const void* q, int64_t q_stride,
+                    const void* k, int64_t k_stride, const void* v, int64_t v_stride, const float* inv_freq, float mscale, void* q_out,
+                    int out_dtype, void* cuda_stream) {
+    if (!h) return NEON_MOE_EINVAL;
+    if (int rc = check_batch(h, batch, cache, rows)) return rc;
+    if (!k || !v || !inv_freq || !q != !q_out) return fail(h, NEON_MOE_EINVAL, "null k, v or inv_freq, or one of q and q_out without the other");
+    if (dtype != NEON_KV4_F32 && dtype != NEON_KV4_BF16 && dtype != NEON_KV4_F16) return fail(h, NEON_MOE_EINVAL, "dtype %d", dtype);
+    if (q_out && out_dtype != NEON_KV4_BF16 && out_dtype != NEON_KV4_F16) return fail(h, NEON_MOE_EINVAL, "out_dtype %d", out_dtype);
+    const Shape& s = h->shape;
+    if (k_stride < s.nkv * s.D || v_stride < s.nkv * s.D || (q && q_stride < s.nq * s.D))
+        return fail(h, NEON_MOE_EINVAL, "a row stride is smaller than the row");
+    if (!aligned(k, k_stride, dtype) || !aligned(v, v_stride, dtype) || (q && !aligned(q, q_stride, dtype)) || reinterpret_cast<uintptr_t>(q_out) % 16)
+        return fail(h, NEON_MOE_EINVAL, "q, k, v and q_out rows have to start on 16-byte boundaries");
+    if (rows == 0) return NEON_MOE_OK;
+    ON_DEVICE(h);
+    AppendParams p{};
+    p.b = device_batch(h, batch, rows);
+    p.s = s;
+    p.q = q; p.k = k; p.v = v;
+    p.q_stride = q_stride; p.k_stride = k_stride; p.v_stride = v_stride;
+    p.n_parts = 1;
+    p.inv_freq = inv_freq; p.mscale = mscale; p.q_out = q_out;
+    p.cache = static_cast<uint8_t*>(cache);
+    return launched(h, launch_append(p, dtype, out_dtype, static_cast<cudaStream_t>(cuda_stream)));
+}
+
+int neon_kv4_read(neon_kv4_handle* h, const neon_kv4_batch* batch, const void* cache, int rows, void* k_out, void* v_out, int dtype,
+                  void* cuda_stream) {
+    if (!h) return NEON_MOE_EINVAL;
+    if (int rc = check_batch(h, batch, cache, rows)) return rc;
+    if (dtype != NEON_KV4_F32 && dtype != NEON_KV4_BF16) return fail(h, NEON_MOE_EINVAL, "dtype %d", dtype);
+    if (reinterpret_cast<uintptr_t>(k_out) % 16 || reinterpret_cast<uintptr_t>(v_out) % 16)
+        return fail(h, NEON_MOE_EINVAL, "k_out and v_out have to be 16-byte aligned");
+    if (rows == 0 || (!k_out && !v_out)) return NEON_MOE_OK;
+    ON_DEVICE(h);
+    const ReadParams p{device_batch(h, batch, rows), h->shape, static_cast<const uint8_t*>(cache), k_out, v_out};
+    const int threads = std::min(256, std::max(32, 2 * h->shape.nkv * h->shape.D / 8 / 32 * 32));
+    cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);
+    if (dtype == NEON_KV4_F32) read_kernel<float><<<rows, threads, 0, st>>>(p);
+    else read_kernel<__nv_bfloat16><<<rows, threads, 0, st>>>(p);
+    return launched(h, 1);
+}
+
+uint64_t neon_kv4_attend_workspace(neon_kv4_handle* h, const neon_kv4_batch* batch, int rows, int max_rows) {
+    if (!h || !batch || batch->batch < 1 || rows < 0) return 0;
+    return attend_workspace(h->shape, device_batch(h, batch, rows), max_rows);
+}
+
+int neon_kv4_attend(neon_kv4_handle* h, const neon_kv4_batch* batch, const void* cache, int rows, int dtype, const void* q, int64_t q_stride,
+                    const void* sinks, int window, float scale, int max_rows, void* out, void* workspace, uint64_t workspace_bytes,
+                    void* cuda_stream) {
+    if (!h) return NEON_MOE_EINVAL;
+    if (int rc = check_batch(h, batch, cache, rows)) return rc;
+    if (!q || !out || !workspace) return fail(h, NEON_MOE_EINVAL, "null q, out or workspace");
+    if (dtype != NEON_KV4_BF16 && dtype != NEON_KV4_F16) return fail(h, NEON_MOE_EINVAL, "dtype %d", dtype);
+    if (window < 0) return fail(h, NEON_MOE_EINVAL, "window %d", window);
+    if (!std::isfinite(scale)) return fail(h, NEON_MOE_EINVAL, "scale is not finite");
+    const Shape& s = h->shape;
+    if (q_stride < s.nq * s.D) return fail(h, NEON_MOE_EINVAL, "a row stride is smaller than the row");
+    if (!aligned(q, q_stride, dtype) || reinterpret_cast<uintptr_t>(out) % 16 || reinterpret_cast<uintptr_t>(workspace) % 16)
+        return fail(h, NEON_MOE_EINVAL, "q rows, out and workspace have to start on 16-byte boundaries");
+    const Batch b = device_batch(h, batch, rows);
+    if (workspace_bytes < attend_workspace(s, b, max_rows))
+        return fail(h, NEON_MOE_EINVAL, "workspace of %llu bytes, %llu wanted", (unsigned long long)workspace_bytes,
+                    (unsigned long long)attend_workspace(s, b, max_rows));
+    if (rows == 0) return NEON_MOE_OK;
+    ON_DEVICE(h);
+    return launched(h, launch_attend(s, b, static_cast<const uint8_t*>(cache), dtype, q, q_stride, static_cast<const uint16_t*>(sinks), window,
+                                     scale, max_rows, out, static_cast<float*>(workspace), static_cast<cudaStream_t>(cuda_stream)));
+}
+
+int neon_kv4_status(neon_kv4_handle* h, int* status) {
+    if (!h || !status) return NEON_MOE_EINVAL;
+    ON_DEVICE(h);
+    cudaError_t e = cudaDeviceSynchronize();
+    if (e == cudaSuccess) e = cudaMemcpy(status, h->status, sizeof(int), cudaMemcpyDeviceToHost);
+    if (e == cudaSuccess) e = cudaMemset(h->status, 0, sizeof(int));
+    return e == cudaSuccess ? NEON_MOE_OK : fail(h, NEON_MOE_ECUDA, "reading the status: %s", cudaGetErrorString(e));
+}
+
+}  // extern "C"
