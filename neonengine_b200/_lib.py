@@ -63,6 +63,11 @@ class NeonKv4Batch(ctypes.Structure):
                 ("table_width", c_int), ("batch", c_int), ("n_pages", ctypes.c_int64)]
 
 
+class NeonSamplerConfig(ctypes.Structure):
+    """Mirror of ``neon_sampler_config`` (include/neon_sampler.h)."""
+    _fields_ = [("vocab", c_int), ("device", c_int)]
+
+
 # name -> (restype, argtypes); must list every symbol include/neon_pt.h declares
 PT_SIGNATURES = {
     "neon_pt_create": (c_int, [ctypes.POINTER(NeonPtConfig), c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, ctypes.POINTER(c_void_p)]),
@@ -140,6 +145,16 @@ KV4_SIGNATURES = {
     "neon_kv4_launch_count": (ctypes.c_int64, [c_void_p]),
 }
 
+# name -> (restype, argtypes); must list every symbol include/neon_sampler.h declares
+SAMPLER_SIGNATURES = {
+    "neon_sampler_create": (c_int, [ctypes.POINTER(NeonSamplerConfig), ctypes.POINTER(c_void_p)]),
+    "neon_sampler_destroy": (c_int, [c_void_p]),
+    "neon_sampler_last_error": (ctypes.c_char_p, [c_void_p]),
+    "neon_sampler_workspace": (ctypes.c_uint64, [c_void_p, c_int]),
+    "neon_sampler_run": (c_int, [c_void_p, c_void_p, c_int, ctypes.c_int64, c_int] + [c_void_p] * 9 + [ctypes.c_uint64, c_void_p]),
+    "neon_sampler_launch_count": (ctypes.c_int64, [c_void_p]),
+}
+
 # name -> (restype, argtypes); must list every symbol include/neon_moe.h declares
 SIGNATURES = {
     "neon_moe_create": (c_int, [ctypes.POINTER(NeonMoeConfig), ctypes.POINTER(c_void_p)]),
@@ -190,7 +205,7 @@ def load() -> ctypes.CDLL:
                           "(there is no CPU fallback)")
     lib = ctypes.CDLL(SO_PATH)
     for name, (res, args) in {**SIGNATURES, **DECODER_SIGNATURES, **WATER_SIGNATURES, **SVGF_SIGNATURES, **PT_SIGNATURES,
-                              **KV4_SIGNATURES}.items():
+                              **KV4_SIGNATURES, **SAMPLER_SIGNATURES}.items():
         fn = getattr(lib, name)  # AttributeError if a declared symbol is not exported
         fn.restype = res
         fn.argtypes = args

@@ -224,6 +224,7 @@ int neon_kv4_append(neon_kv4_handle* h, const neon_kv4_batch* batch, void* cache
                     int out_dtype, void* cuda_stream) {
     if (!h) return NEON_MOE_EINVAL;
     if (int rc = check_batch(h, batch, cache, rows)) return rc;
+    if (rows == 0) return NEON_MOE_OK;
     if (!k || !v || !inv_freq || !q != !q_out) return fail(h, NEON_MOE_EINVAL, "null k, v or inv_freq, or one of q and q_out without the other");
     if (dtype != NEON_KV4_F32 && dtype != NEON_KV4_BF16 && dtype != NEON_KV4_F16) return fail(h, NEON_MOE_EINVAL, "dtype %d", dtype);
     if (q_out && out_dtype != NEON_KV4_BF16 && out_dtype != NEON_KV4_F16) return fail(h, NEON_MOE_EINVAL, "out_dtype %d", out_dtype);
@@ -232,7 +233,6 @@ int neon_kv4_append(neon_kv4_handle* h, const neon_kv4_batch* batch, void* cache
         return fail(h, NEON_MOE_EINVAL, "a row stride is smaller than the row");
     if (!aligned(k, k_stride, dtype) || !aligned(v, v_stride, dtype) || (q && !aligned(q, q_stride, dtype)) || reinterpret_cast<uintptr_t>(q_out) % 16)
         return fail(h, NEON_MOE_EINVAL, "q, k, v and q_out rows have to start on 16-byte boundaries");
-    if (rows == 0) return NEON_MOE_OK;
     ON_DEVICE(h);
     AppendParams p{};
     p.b = device_batch(h, batch, rows);
@@ -249,10 +249,11 @@ int neon_kv4_read(neon_kv4_handle* h, const neon_kv4_batch* batch, const void* c
                   void* cuda_stream) {
     if (!h) return NEON_MOE_EINVAL;
     if (int rc = check_batch(h, batch, cache, rows)) return rc;
+    if (rows == 0) return NEON_MOE_OK;
     if (dtype != NEON_KV4_F32 && dtype != NEON_KV4_BF16) return fail(h, NEON_MOE_EINVAL, "dtype %d", dtype);
     if (reinterpret_cast<uintptr_t>(k_out) % 16 || reinterpret_cast<uintptr_t>(v_out) % 16)
         return fail(h, NEON_MOE_EINVAL, "k_out and v_out have to be 16-byte aligned");
-    if (rows == 0 || (!k_out && !v_out)) return NEON_MOE_OK;
+    if (!k_out && !v_out) return NEON_MOE_OK;
     ON_DEVICE(h);
     const ReadParams p{device_batch(h, batch, rows), h->shape, static_cast<const uint8_t*>(cache), k_out, v_out};
     const int threads = std::min(256, std::max(32, 2 * h->shape.nkv * h->shape.D / 8 / 32 * 32));
@@ -272,6 +273,7 @@ int neon_kv4_attend(neon_kv4_handle* h, const neon_kv4_batch* batch, const void*
                     void* cuda_stream) {
     if (!h) return NEON_MOE_EINVAL;
     if (int rc = check_batch(h, batch, cache, rows)) return rc;
+    if (rows == 0) return NEON_MOE_OK;
     if (!q || !out || !workspace) return fail(h, NEON_MOE_EINVAL, "null q, out or workspace");
     if (dtype != NEON_KV4_BF16 && dtype != NEON_KV4_F16) return fail(h, NEON_MOE_EINVAL, "dtype %d", dtype);
     if (window < 0) return fail(h, NEON_MOE_EINVAL, "window %d", window);
@@ -284,7 +286,6 @@ int neon_kv4_attend(neon_kv4_handle* h, const neon_kv4_batch* batch, const void*
     if (workspace_bytes < attend_workspace(s, b, max_rows))
         return fail(h, NEON_MOE_EINVAL, "workspace of %llu bytes, %llu wanted", (unsigned long long)workspace_bytes,
                     (unsigned long long)attend_workspace(s, b, max_rows));
-    if (rows == 0) return NEON_MOE_OK;
     ON_DEVICE(h);
     return launched(h, launch_attend(s, b, static_cast<const uint8_t*>(cache), dtype, q, q_stride, static_cast<const uint16_t*>(sinks), window,
                                      scale, max_rows, out, static_cast<float*>(workspace), static_cast<cudaStream_t>(cuda_stream)));

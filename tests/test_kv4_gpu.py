@@ -474,4 +474,7 @@ def test_refusals(systems):
     assert lib.neon_kv4_append(kv._h, batch._ref, one, 2, 9, one, 512, one, 128, one, 128, one, 1.0, one, 1, None) == 1
     assert lib.neon_kv4_read(kv._h, batch._ref, one, 2, one, one, 2, None) == 1
     assert lib.neon_kv4_read(kv._h, None, one, 2, one, one, 1, None) == 1
+    none = kv.batch(torch.zeros(2, dtype=torch.int32, device=DEV), table, torch.zeros(3, dtype=torch.int32, device=DEV))
+    empty = kv.append(none, cache, q[:0], k[:0], v[:0], f)
+    assert kv.attend(none, cache, empty).shape == (0, 8, 64) and kv.read(none, cache, rows=0)[0].shape == (0, 2, 64)
     assert kv.status() == 0
