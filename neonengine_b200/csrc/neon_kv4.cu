@@ -82,23 +82,6 @@ int check_batch(neon_kv4_handle* h, const neon_kv4_batch* b, const void* cache, 
 namespace neon {
 namespace kv4 {
 
-cudaError_t configure_attend() {
-    static std::atomic<bool> done[64];
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess || done[dev & 63]) return e;
-    auto set = [&](const void* k) {
-        if (e == cudaSuccess) e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
-    };
-#define SET(D, NT)                                           \
-    set((const void*)attend_kernel<D, NT, __nv_bfloat16>); \
-    set((const void*)attend_kernel<D, NT, __half>);
-    SET(64, 1) SET(64, 2) SET(64, 4) SET(128, 1) SET(128, 2)
-#undef SET
-    if (e == cudaSuccess) done[dev & 63] = true;
-    return e;
-}
-
 namespace {
 constexpr int kSms = 148, kSharedPerSm = 227 * 1024;
 
@@ -114,41 +97,76 @@ int ctas_per_sm(const Shape& s, int nt) { return s.D == 64 && nt <= 2 ? 2 : 1; }
 int attend_grid(const Shape& s, const Batch& b, int nt) {
     const long long steps = ((long long)b.width * s.P + kStep - 1) / kStep;
     const long long blocks = (long long)b.rows * (s.nq / s.nkv) / (8 * nt) + b.n;
-    const long long most = steps * blocks * s.nkv;  // units there can be
+    const long long most = (steps * blocks * s.nkv + kAttendWarps - 1) / kAttendWarps;  // CTAs that there can be steps for
     return (int)std::min<long long>(kSms * ctas_per_sm(s, nt), std::max<long long>(most, 1));
 }
 
-template <int D, int NT, class T>
-void launch_attend_t(AttendParams p, int grid, cudaStream_t st) {
-    using W = WarpSmem<D>;
-    const int before = (p.b.n + 2) / 2 * 16, budget = kSharedPerSm / ctas_per_sm(p.s, NT) - 1024 - before;
+template <class F>
+void with_pdl(void (*kernel)(AttendParams), unsigned grid, int threads, size_t smem, cudaStream_t st, const F& p) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    cudaLaunchKernelEx(&cfg, kernel, p);
+}
+
+template <int DIM, int PAGE, int NT>
+cudaError_t attend_variant(const AttendParams* run, cudaStream_t st) {
+    using W = WarpSmem<DIM>;
+    if (!run) return cudaFuncSetAttribute(attend_kernel<DIM, PAGE, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, 226 * 1024);
+    AttendParams p = *run;
+    const int plan = plan_bytes(p.b.n), budget = kSharedPerSm / ctas_per_sm(p.s, NT) - 2048 - plan;
     p.stages = std::min(W::kMaxStages, (budget / kAttendWarps - W::bytes(0)) / W::kRing);
-    attend_kernel<D, NT, T><<<grid, kAttendWarps * 32, before + kAttendWarps * W::bytes(p.stages), st>>>(p);
+    attend_kernel<DIM, PAGE, NT><<<p.grid, kAttendWarps * 32, plan + kAttendWarps * W::bytes(p.stages), st>>>(p);
     const long long tasks = (long long)p.b.rows * p.s.nq;
-    merge_kernel<D, T><<<(unsigned)((tasks + 7) / 8), 256, before, st>>>(p);
+    with_pdl(merge_kernel<DIM>, (unsigned)((tasks + 7) / 8), 256, plan, st, p);
+    return cudaSuccess;
+}
+// Calls f with every variant that there is; the one of a shape and a number of column groups.
+template <class F>
+cudaError_t each_variant(const F& f) {
+    cudaError_t e = cudaSuccess;
+#define TRY(DIM, PAGE, NT) if (e == cudaSuccess) e = f(DIM, PAGE, NT, &attend_variant<DIM, PAGE, NT>);
+#define PAGES(DIM, NT) TRY(DIM, 16, NT) TRY(DIM, 32, NT) TRY(DIM, 64, NT)
+    PAGES(64, 1) PAGES(64, 2) PAGES(64, 4) PAGES(128, 1) PAGES(128, 2)
+#undef PAGES
+#undef TRY
+    return e;
 }
 }  // namespace
 
+cudaError_t configure_attend() {
+    static std::atomic<bool> done[64];
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess || done[dev & 63]) return e;
+    e = each_variant([](int, int, int, auto variant) { return variant(nullptr, nullptr); });
+    if (e == cudaSuccess) done[dev & 63] = true;
+    return e;
+}
+
 uint64_t attend_workspace(const Shape& s, const Batch& b, int max_rows) {
     const int nt = column_groups(s, max_rows);
-    return (uint64_t)attend_grid(s, b, nt) * kAttendWarps * 2 * 8 * nt * (s.D + 2) * sizeof(float);
+    return (uint64_t)attend_grid(s, b, nt) * (2 + kAttendWarps) * 8 * nt * (s.D + 2) * sizeof(float);
 }
 
 int launch_attend(const Shape& s, const Batch& b, const uint8_t* cache, int dtype, const void* q, long long q_stride, const uint16_t* sinks,
                   int window, float scale, int max_rows, void* out, float* workspace, cudaStream_t st) {
     AttendParams p{};
     p.b = b; p.s = s; p.cache = cache; p.q = q; p.q_stride = q_stride; p.sinks = sinks;
-    p.window = window; p.G = s.nq / s.nkv; p.scale = scale; p.out = out; p.part = workspace;
-    const int nt = column_groups(s, max_rows), grid = attend_grid(s, b, nt);
-    p.row_blocks = 8 * nt;
-    p.workers = grid * kAttendWarps;
-#define RUN(DIM, NT)                                                            \
-    if (s.D == DIM && nt == NT) {                                               \
-        if (dtype == NEON_KV4_BF16) launch_attend_t<DIM, NT, __nv_bfloat16>(p, grid, st); \
-        else launch_attend_t<DIM, NT, __half>(p, grid, st);                     \
-    }
-    RUN(64, 1) RUN(64, 2) RUN(64, 4) RUN(128, 1) RUN(128, 2)
-#undef RUN
+    p.window = window; p.G = s.nq / s.nkv; p.half = dtype == NEON_KV4_F16; p.scale = scale; p.out = out; p.part = workspace;
+    const int nt = column_groups(s, max_rows);
+    p.grid = attend_grid(s, b, nt);
+    p.R = 8 * nt;
+    each_variant([&](int dim, int page, int groups, auto variant) {
+        return dim == s.D && page == s.P && groups == nt ? variant(&p, st) : cudaSuccess;
+    });
     return 2;
 }
 
