@@ -13,7 +13,7 @@
 //   scale is exact.  Queries are f16, every row scaled by a power of two so that its largest value lies in [2^14, 2^15):
 //   exact for bf16 and f16 down to 2^-28 of the largest.
 //   Values: a pair of positions of one column is one f16x2 operand, multiplied by the two positions' scales relative to
-//   the largest scale met so far (outputs are rescaled when it grows).  Where scales lie further apart than 2^6, or grow
+//   the largest scale met so far (outputs are rescaled when it grows).  Where scales lie further apart than 2^7, or grow
 //   by more than 2^2, a probability that f16 rounds away could belong to a value that counts: such a step's values are
 //   added in f32, one position at a time (five times as long, and rare), so no spread of scales loses anything.
 //   Probabilities are rounded to f16 (2^-12), once; sums and statistics are f32, and the softmax sum is one more product, with
@@ -32,7 +32,7 @@ constexpr int kStep = 64;             // positions of a step
 constexpr float kNoMax = -1e30f;      // running maximum before the first score
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr uint32_t kRaise = 0x5c00;   // f16 2^8: what a probability relative to the running maximum may reach
-constexpr int kSpread = 6, kGrowth = 2;  // how far (log2) value scales may lie below the largest, and the largest may grow, for f16 operands
+constexpr int kSpread = 7, kGrowth = 2;  // how far (log2) value scales may lie below the largest, and the largest may grow, for f16 operands
 
 struct AttendParams {
     Batch b;
@@ -44,9 +44,12 @@ struct AttendParams {
     int window, G, half;  // half: q and out are f16, else bf16
     float scale;
     void* out;
-    float* part;  // [CTA][2][R][2 + D] partial results of the CTAs, then [CTA][warp][R][2 + D] of warps
+    float* part;  // partial results: [CTA][2] of CTAs, then [CTA][warp] of warps, each [R][D] outputs and [R][2] maxima and sums
     int grid, stages;
     int R;        // rows (tokens times G) of an item: 8 * NT
+    uint32_t G_inverse;  // ceil(2^32 / G)
+    // r / G for r < 2^26, exact as G <= 32
+    __device__ __forceinline__ int token(int r) const { return G == 1 ? r : (int)__umulhi((uint32_t)r, G_inverse); }
 };
 
 constexpr int kAttendWarps = 8;
@@ -69,42 +72,43 @@ __device__ __forceinline__ SeqPlan plan_of(const AttendParams& p, int s) {
     r.pos0 = full - r.n;
     const int lo = p.window > 0 ? max(r.pos0 - p.window + 1, 0) : 0;
     r.lo_step = lo / kStep;
-    r.blocks = r.n > 0 ? (r.n * p.G + p.R - 1) / p.R : 0;
+    r.blocks = r.n > 0 ? (r.n * p.G + p.R - 1) >> (31 - __clz(p.R)) : 0;  // R is a power of two
     r.steps = r.n > 0 && r.len > lo ? (r.len + kStep - 1) / kStep - r.lo_step : 0;
     return r;
 }
 
+__device__ __forceinline__ long long units_of(const AttendParams& p, int s) {
+    const SeqPlan r = plan_of(p, s);
+    if (p.b.seq_lens[s] > p.b.width * p.s.P || (p.b.cu_q && p.b.cu_q[s + 1] < p.b.cu_q[s])) report(p.b.status, NEON_KV4_BAD_LENGTH);
+    return (long long)p.s.nkv * r.blocks * r.steps;
+}
+
 // before[s] = units of the sequences before s, for s <= n; returns the units of a CTA.  The whole CTA takes part.
 __device__ __forceinline__ long long scan_units(const AttendParams& p, long long* before) {
-    for (int s = threadIdx.x; s < p.b.n; s += blockDim.x) {
-        const SeqPlan r = plan_of(p, s);
-        before[s + 1] = (long long)p.s.nkv * r.blocks * r.steps;
-        if (p.b.seq_lens[s] > p.b.width * p.s.P || (p.b.cu_q && p.b.cu_q[s + 1] < p.b.cu_q[s])) report(p.b.status, NEON_KV4_BAD_LENGTH);
+    if (p.b.n > 32) {
+        for (int s = threadIdx.x; s < p.b.n; s += blockDim.x) before[s + 1] = units_of(p, s);
+        __syncthreads();
     }
-    if (threadIdx.x == 0) before[0] = 0;
-    __syncthreads();
     if (threadIdx.x < 32) {
         long long carry = 0;
-        for (int s0 = 1; s0 <= p.b.n; s0 += 32) {
+        for (int s0 = 0; s0 < p.b.n; s0 += 32) {
             const int s = s0 + threadIdx.x;
-            long long v = s <= p.b.n ? before[s] : 0;
+            long long v = s >= p.b.n ? 0 : p.b.n > 32 ? before[s + 1] : units_of(p, s);
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
                 const long long w = __shfl_up_sync(0xffffffffu, v, o);
                 if (threadIdx.x >= o) v += w;
             }
             v += carry;
-            if (s <= p.b.n) before[s] = v;
+            if (s < p.b.n) before[s + 1] = v;
             carry = __shfl_sync(0xffffffffu, v, 31);
         }
+        if (threadIdx.x == 0) before[0] = 0;
     }
     __syncthreads();
     // few units: a step for every warp of as many CTAs as that takes, so that little is left to merge
     const long long units = before[p.b.n];
-    if (units <= 0x7fffffff) {
-        const uint32_t u = (uint32_t)units;
-        return max((u + p.grid - 1) / p.grid, (uint32_t)kAttendWarps);
-    }
+    if (units <= 0x7fffffff) return max(((uint32_t)units + p.grid - 1) / p.grid, (uint32_t)kAttendWarps);
     return (units + p.grid - 1) / p.grid;
 }
 
@@ -179,14 +183,14 @@ struct WarpSmem {
 struct Partial {  // a warp's unfinished item
     int there, starts, ends;  // whether it has the item's first, last step
     int row0, r0, rows, head;
-    const float* data;        // [rows][2 + D]: maximum, sum, output
+    const float* data;        // [R][D] outputs, [R][2] maxima and sums
 };
 __host__ __device__ constexpr int plan_bytes(int n) { return (n + 2) / 2 * 16; }
 
 template <int D, int P, int NT>
 __global__ void __launch_bounds__(kAttendWarps * 32, (D == 64 && NT <= 2) ? 2 : 1) attend_kernel(const AttendParams p) {
     using W = WarpSmem<D>;
-    constexpr int NB = W::kBlocks, R = 8 * NT, kRow = D + 2;
+    constexpr int NB = W::kBlocks, R = 8 * NT, kSlot = R * (D + 2);
     constexpr int kPages = kStep / P, kRec = P * (D + D / 16), kCodes = P * D / 2, kScales = P * D / 32;
     constexpr int TI = NT == 1 ? 4 : 2;      // 16-position tiles whose scores are held at once
     constexpr uint32_t kOnes = 0x3c003c00u;  // two f16 ones
@@ -207,13 +211,13 @@ __global__ void __launch_bounds__(kAttendWarps * 32, (D == 64 && NT <= 2) ? 2 : 
     const long long share = scan_units(p, before), units = before[p.b.n];
     const long long cta_begin = min(blockIdx.x * share, units);
     const int cta_units = (int)(min(cta_begin + share, units) - cta_begin);
-    long long u = cta_begin + (long long)cta_units * warp / kAttendWarps;
-    const long long u_end = cta_begin + (long long)cta_units * (warp + 1) / kAttendWarps;
+    const int run_begin = (int)((uint32_t)cta_units * warp / kAttendWarps), run_end = (int)((uint32_t)cta_units * (warp + 1) / kAttendWarps);
+    const long long u_end = cta_begin + run_end;
+    int left = run_end - run_begin, left_ahead = left;  // steps to multiply, to fetch
     auto block_of = [&](int i) { return (i >> 2) * 2 + (g >> 2); };  // column block of this lane's rows of output tile i
     bool timeout = false;
 
-    if (u < u_end) {
-        // ---- fetching: runs `stages` steps ahead ---------------------------------------------------------------------
+    if (left > 0) {
         struct Item { int s, head, block; };
         auto place = [&](Item& c, SeqPlan& q, long long unit) {  // returns the step
             c.s = sequence_of(before, p.b.n, unit);
@@ -221,8 +225,8 @@ __global__ void __launch_bounds__(kAttendWarps * 32, (D == 64 && NT <= 2) ? 2 : 
             const long long r = unit - before[c.s];
             if (r <= 0x7fffffff) {
                 const uint32_t r32 = (uint32_t)r, item = r32 / (uint32_t)q.steps;
-                c.head = item / (uint32_t)q.blocks;
-                c.block = item % (uint32_t)q.blocks;
+                c.head = q.blocks == 1 ? item : item / (uint32_t)q.blocks;
+                c.block = item - c.head * q.blocks;
                 return (int)(r32 - item * q.steps);
             }
             const long long item = r / q.steps;
@@ -230,95 +234,107 @@ __global__ void __launch_bounds__(kAttendWarps * 32, (D == 64 && NT <= 2) ? 2 : 
             c.block = (int)(item % q.blocks);
             return (int)(r % q.steps);
         };
-        auto next_item = [&](Item& c, SeqPlan& q, long long unit) {
+        auto next_item = [&](Item& c, SeqPlan& q, int units_left) {
             if (++c.block < q.blocks) return;
             c.block = 0;
             if (++c.head < p.s.nkv) return;
-            if (unit < u_end) place(c, q, unit);
+            if (units_left) place(c, q, u_end - units_left);
         };
         Item cur, ahead;
         SeqPlan q, qa;
-        int step = place(cur, q, u);
+        int step = place(cur, q, u_end - left);
         ahead = cur;
         qa = q;
-        long long u_ahead = u;
-        int a_step = step, id_base = -64, ids = -1;  // 32 page ids of the item that is fetched, from id_base on
-        uint32_t valid = 0;                          // which pages of a stage are there: four bits each
+        // ---- fetching: runs `stages` steps ahead ---------------------------------------------------------------------
+        int a_page = (q.lo_step + step) * kPages, a_end = (q.lo_step + q.steps) * kPages;  // of the item that is fetched
+        int id_base = -64, ids = -1;  // 32 page ids of its sequence, from id_base on
+        uint32_t holes = 0;           // which pages of a stage are missing: four bits each
         auto fetch = [&](int stage) {
-            const int first = (qa.lo_step + a_step) * kPages;
-            if (first - id_base >= 32 || first < id_base) {
-                id_base = first;
+            if ((uint32_t)(a_page - id_base) >= 32u) {
+                id_base = a_page;
                 ids = -1;
-                if ((first + lane) * P < qa.len) {
-                    ids = p.b.table[ahead.s * p.b.table_stride + first + lane];
+                if ((a_page + lane) * P < qa.len) {
+                    ids = p.b.table[ahead.s * p.b.table_stride + a_page + lane];
                     if (ids < 0 || ids >= p.b.n_pages) {
                         report(p.b.status, NEON_KV4_BAD_PAGE);
                         ids = -1;
                     }
                 }
             }
-            const int id = __shfl_sync(0xffffffffu, ids, first - id_base + (lane & (kPages - 1)));
-            const uint32_t there = __ballot_sync(0xffffffffu, id >= 0) & ((1u << kPages) - 1);
-            if (lane == 0) sm100::mbar_expect_tx(&full[stage], __popc(there) * kRec);
-            __syncwarp();
-            if (lane < kPages && id >= 0)
-                sm100::bulk_load(mine + stage * W::kRing + lane * kRec, p.cache + ((long long)id * p.s.nkv + ahead.head) * kRec, kRec, &full[stage]);
-            valid = (valid & ~(15u << (4 * stage))) | (there << (4 * stage));
-            ++u_ahead;
-            if (++a_step == qa.steps) {
-                a_step = 0;
+            unsigned char* to = mine + stage * W::kRing;
+            if constexpr (kPages == 1) {
+                const int id = __shfl_sync(0xffffffffu, ids, a_page - id_base);
+                if (lane == 0) {
+                    sm100::mbar_expect_tx(&full[stage], id >= 0 ? kRec : 0);
+                    if (id >= 0) sm100::bulk_load(to, p.cache + ((long long)id * p.s.nkv + ahead.head) * kRec, kRec, &full[stage]);
+                }
+                holes = id >= 0 ? holes & ~(15u << (4 * stage)) : holes | (1u << (4 * stage));
+            } else {
+                const int id = __shfl_sync(0xffffffffu, ids, a_page - id_base + (lane & (kPages - 1)));
+                const uint32_t there = __ballot_sync(0xffffffffu, id >= 0) & ((1u << kPages) - 1);
+                if (lane == 0) sm100::mbar_expect_tx(&full[stage], __popc(there) * kRec);
+                __syncwarp();
+                if (lane < kPages && id >= 0)
+                    sm100::bulk_load(to + lane * kRec, p.cache + ((long long)id * p.s.nkv + ahead.head) * kRec, kRec, &full[stage]);
+                holes = (holes & ~(15u << (4 * stage))) | ((there ^ ((1u << kPages) - 1)) << (4 * stage));
+            }
+            --left_ahead;
+            a_page += kPages;
+            if (a_page == a_end) {
                 const int s = ahead.s;
-                next_item(ahead, qa, u_ahead);
+                next_item(ahead, qa, left_ahead);
+                a_page = qa.lo_step * kPages;
+                a_end = a_page + qa.steps * kPages;
                 if (ahead.s != s) id_base = -64;
             }
         };
-        for (int i = 0; i < p.stages && u_ahead < u_end; ++i) fetch(i);
         int stage = 0, phase = 0;
+        bool started = false;
 
-        while (u < u_end) {
+        while (left > 0) {
             // ---- an item: its queries --------------------------------------------------------------------------------
             const int r0 = cur.block * R, rows = min(R, q.n * p.G - r0);
             uint32_t qf[NT][NB][4];  // B operands: block, two k-steps of two registers
             float qs[NT][2];         // factor of the scores of columns 2t, 2t + 1
+            uint4 raw[NT][NB];
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
-                const int r = j * 8 + g;
+                const int rr = r0 + min(j * 8 + g, rows - 1), token = p.token(rr);
+                const uint16_t* src = static_cast<const uint16_t*>(p.q) + (q.row0 + token) * p.q_stride + (cur.head * p.G + rr - token * p.G) * D + t * 8;
+#pragma unroll
+                for (int b = 0; b < NB; ++b) raw[j][b] = *reinterpret_cast<const uint4*>(src + b * 32);
+            }
+            if (!started) {  // (the queries are on their way)
+                for (int i = 0; i < p.stages && left_ahead > 0; ++i) fetch(i);
+                started = true;
+            }
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
                 float amax = 0.f, x[NB][8];
-                if (r < rows) {
-                    const int rr = r0 + r;
-                    const long long at = (q.row0 + rr / p.G) * p.q_stride + (cur.head * p.G + rr % p.G) * D;
 #pragma unroll
-                    for (int b = 0; b < NB; ++b) {
-                        if (p.half) load8(static_cast<const __half*>(p.q) + at + b * 32 + t * 8, x[b]);
-                        else load8(static_cast<const __nv_bfloat16*>(p.q) + at + b * 32 + t * 8, x[b]);
-                    }
-                } else {
-#pragma unroll
-                    for (int b = 0; b < NB; ++b)
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) x[b][i] = 0.f;
-                }
-#pragma unroll
-                for (int b = 0; b < NB; ++b)
+                for (int b = 0; b < NB; ++b) {
+                    if (p.half) load8(reinterpret_cast<const __half*>(&raw[j][b]), x[b]);
+                    else load8(reinterpret_cast<const __nv_bfloat16*>(&raw[j][b]), x[b]);
 #pragma unroll
                     for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(x[b][i]));
+                }
                 amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
                 amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
                 const int e = (int)(__float_as_uint(amax) >> 23) - 127;  // floor(log2 amax); 128 for infinities
                 const int up = amax > 0.f && e < 128 ? min(14 - e, 126) : 0;
-                const float f = pow2i(up);
+                const float f = j * 8 + g < rows ? pow2i(up) : 0.f;
 #pragma unroll
                 for (int b = 0; b < NB; ++b)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) qf[j][b][i] = pack2(x[b][2 * i] * f, x[b][2 * i + 1] * f, __half());
-                const float back = p.scale * kLog2e * pow2i(-up);
+                    for (int i = 0; i < 4; ++i) qf[j][b][i] = f == 0.f ? 0u : pack2(x[b][2 * i] * f, x[b][2 * i + 1] * f, __half());
+                const float product = p.scale * kLog2e * pow2i(-up), back = product == 0.f ? 1e-30f : product;  // (a scale of 0: all alike)
                 qs[j][0] = __shfl_sync(0xffffffffu, back, 8 * t);
                 qs[j][1] = __shfl_sync(0xffffffffu, back, 8 * t + 4);
             }
             // what column c sees: positions above sees_lo(c), up to sees_hi(c)
-            auto sees_hi = [&](int c) { return c < rows ? min(q.pos0 + (r0 + c) / p.G, q.len - 1) : -1; };
-            auto sees_lo = [&](int c) { return p.window > 0 ? q.pos0 + (r0 + c) / p.G - p.window : -1; };
-            const int pos_lo = q.pos0 + r0 / p.G, pos_hi = min(q.pos0 + (r0 + rows - 1) / p.G, q.len - 1);
+            auto sees_hi = [&](int c) { return c < rows ? min(q.pos0 + p.token(r0 + c), q.len - 1) : -1; };
+            auto sees_lo = [&](int c) { return p.window > 0 ? q.pos0 + p.token(r0 + c) - p.window : -1; };
+            const int pos_lo = q.pos0 + p.token(r0), pos_hi = min(q.pos0 + p.token(r0 + rows - 1), q.len - 1);
             const int first = p.window > 0 ? max(pos_lo - p.window + 1, 0) : 0;
             float o[NT][D / 16][4], l[NT][4], m[NT][2];
 #pragma unroll
@@ -331,24 +347,25 @@ __global__ void __launch_bounds__(kAttendWarps * 32, (D == 64 && NT <= 2) ? 2 : 
             int ve[NB];  // largest value scale so far (its byte), per block
 #pragma unroll
             for (int b = 0; b < NB; ++b) ve[b] = 0;
-            const int n = (int)min((long long)(q.steps - step), u_end - u);
+            const int n = min(q.steps - step, left);
             const bool starts = step == 0, ends = step + n == q.steps;
+            // steps that any row sees a position of; steps of which every row sees every position
+            const int see_begin = first / kStep, see_end = pos_hi < 0 ? 0 : pos_hi / kStep + 1;
+            const int open_begin = p.window > 0 ? ((pos_hi - p.window) >> 6) + 1 : 0, open_end = (min(pos_lo, q.len - 1) + 1) >> 6;
 
-            for (int k = 0; k < n; ++k) {
-                const int p0 = (q.lo_step + step + k) * kStep;  // first position of the step
+            for (int at_step = q.lo_step + step, end_step = at_step + n; at_step < end_step; ++at_step) {
+                const int p0 = at_step * kStep;  // first position of the step
                 if (!wait_bounded(&full[stage], phase)) {
                     timeout = true;
                     break;
                 }
                 const unsigned char* st = mine + stage * W::kRing;
-                const uint32_t there = (valid >> (4 * stage)) & 15u;
-                // every position of the step is seen by every row
-                const bool open = there == (1u << kPages) - 1 && p0 + kStep - 1 <= pos_lo && p0 + kStep <= q.len &&
-                                  (p.window <= 0 || p0 > pos_hi - p.window);
-                if (p0 <= pos_hi && p0 + kStep > first) {
+                const uint32_t there = ~(holes >> (4 * stage)) & ((1u << kPages) - 1);
+                const bool open = at_step >= open_begin && at_step < open_end && there == (1u << kPages) - 1;
+                if (at_step >= see_begin && at_step < see_end) {
                     // ---- scales: lane l takes positions 2l and 2l + 1 -------------------------------------------------
                     int vb[NB][2];
-                    bool special = false;
+                    uint32_t below = 0;  // the scales' distances from the largest, or'ed
                     {
                         const int q0 = 2 * lane, pg = q0 / P, in = q0 % P;
                         const unsigned char* sc = st + pg * kRec + 2 * kCodes + in * NB;
@@ -378,10 +395,10 @@ __global__ void __launch_bounds__(kAttendWarps * 32, (D == 64 && NT <= 2) ? 2 : 
 #pragma unroll
                         for (int b = 0; b < NB; ++b)
 #pragma unroll
-                            for (int i = 0; i < 2; ++i) special = special || (uint32_t)(ve[b] - vb[b][i]) > (uint32_t)kSpread;
+                            for (int i = 0; i < 2; ++i) below |= (uint32_t)(ve[b] - vb[b][i]);
                     }
                     bool plain = true;  // f16 operands do
-                    if (__any_sync(0xffffffffu, special)) {
+                    if (__any_sync(0xffffffffu, below > (uint32_t)kSpread)) {  // (kSpread has all its bits set)
 #pragma unroll
                         for (int b = 0; b < NB; ++b) {
                             int top = __reduce_max_sync(0xffffffffu, max(vb[b][0], vb[b][1]));
@@ -421,13 +438,13 @@ __global__ void __launch_bounds__(kAttendWarps * 32, (D == 64 && NT <= 2) ? 2 : 
                             plain = plain && ve[b] - low <= kSpread;
                         }
                     }
-                    // scales relative to the largest: 1 .. 2^-6 (anything finite where no row looks)
+                    // scales relative to the largest: 1 .. 2^-7 (anything finite where no row looks)
 #pragma unroll
                     for (int b = 0; b < NB; ++b)
 #pragma unroll
                         for (int i = 0; i < 2; ++i) {
                             const int in = (2 * lane + i) & 15;
-                            const int h = vb[b][i] < 0 ? 0 : (vb[b][i] - ve[b] + 15) * 1024;
+                            const int h = max(vb[b][i] - ve[b] + 15, 0) * 1024;
                             reinterpret_cast<uint16_t*>(vs)[((b * 4 + (lane >> 3)) * 4 + (in & 3)) * 4 + (in >> 2)] = (uint16_t)h;
                         }
                     __syncwarp();
@@ -458,34 +475,27 @@ __global__ void __launch_bounds__(kAttendWarps * 32, (D == 64 && NT <= 2) ? 2 : 
                                 }
                             }
                         }
-                        uint32_t seen[NT];  // bit 4 i + c: position of sc[j][i][c] is seen by its column
+                        if (!open) {  // what a column does not see scores -infinity (columns' factors are never zero)
 #pragma unroll
-                        for (int j = 0; j < NT; ++j) seen[j] = 0xffffu;
-                        if (!open) {
-#pragma unroll
-                            for (int j = 0; j < NT; ++j) {
-                                seen[j] = 0;
+                            for (int j = 0; j < NT; ++j)
 #pragma unroll
                                 for (int c = 0; c < 2; ++c) {
                                     const int hi = sees_hi(j * 8 + 2 * t + c), lo = sees_lo(j * 8 + 2 * t + c);
+                                    const float never = qs[j][c] > 0.f ? -INFINITY : INFINITY;
 #pragma unroll
                                     for (int i = 0; i < TI; ++i)
 #pragma unroll
                                         for (int h = 0; h < 2; ++h) {
                                             const int pos = p0 + 16 * (i0 + i) + at + 8 * h;
-                                            if (((there >> (16 * (i0 + i) / P)) & 1) && pos <= hi && pos > lo) seen[j] |= 1u << (4 * i + 2 * h + c);
+                                            if (!((there >> (16 * (i0 + i) / P)) & 1) || pos > hi || pos <= lo) sc[j][i][2 * h + c] = never;
                                         }
                                 }
-                            }
                         }
                         // ---- probabilities -----------------------------------------------------------------------------------
-                        auto argument = [&](int j, int i, int c) {
-                            const float x = fmaf(sc[j][i][c], qs[j][c & 1], -m[j][c & 1]);
-                            return open || ((seen[j] >> (4 * i + c)) & 1) ? x : -INFINITY;
-                        };
-                        uint32_t pf[NT][TI][2];
-                        for (int round = 0; round < 2; ++round) {
-                            uint32_t top = 0;
+                        auto argument = [&](int j, int i, int c) { return fmaf(sc[j][i][c], qs[j][c & 1], -m[j][c & 1]); };
+                        uint32_t pf[NT][TI][2], top = 0;
+                        auto weigh = [&] {
+                            top = 0;
 #pragma unroll
                             for (int j = 0; j < NT; ++j)
 #pragma unroll
@@ -495,18 +505,18 @@ __global__ void __launch_bounds__(kAttendWarps * 32, (D == 64 && NT <= 2) ? 2 : 
                                         pf[j][i][h] = pack2(ex2(argument(j, i, 2 * h)), ex2(argument(j, i, 2 * h + 1)), __half());
                                         top = max_f16x2(top, pf[j][i][h]);  // passes over NaN
                                     }
-                            // probabilities are not negative: their bits are in order
-                            if (!__any_sync(0xffffffffu, max(top & 0xffffu, top >> 16) > kRaise)) break;
+                        };
+                        weigh();
+                        // probabilities are not negative: their bits are in order
+                        if (__any_sync(0xffffffffu, max(top & 0xffffu, top >> 16) > kRaise)) {
 #pragma unroll
                             for (int j = 0; j < NT; ++j)
 #pragma unroll
                                 for (int c = 0; c < 2; ++c) {
-                                    float x = -INFINITY;
+                                    float x = -INFINITY, factor = qs[j][c];
+                                    asm volatile("" : "+f"(factor));  // keeps these products out of the steps that need none
 #pragma unroll
-                                    for (int i = 0; i < TI; ++i)
-#pragma unroll
-                                        for (int h = 0; h < 2; ++h)
-                                            if (open || ((seen[j] >> (4 * i + 2 * h + c)) & 1)) x = fmaxf(x, sc[j][i][2 * h + c] * qs[j][c]);
+                                    for (int i = 0; i < TI; ++i) x = fmaxf(x, fmaxf(sc[j][i][c] * factor, sc[j][i][c + 2] * factor));
 #pragma unroll
                                     for (int off = 4; off < 32; off <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, off));
                                     const float now = fmaxf(m[j][c], x), f = ex2(m[j][c] - now);
@@ -515,6 +525,7 @@ __global__ void __launch_bounds__(kAttendWarps * 32, (D == 64 && NT <= 2) ? 2 : 
 #pragma unroll
                                     for (int i = 0; i < D / 16; ++i) { o[j][i][c] *= f; o[j][i][c + 2] *= f; }
                                 }
+                            weigh();
                         }
                         // ---- values ------------------------------------------------------------------------------------------
                         if (plain) {
@@ -596,7 +607,7 @@ __global__ void __launch_bounds__(kAttendWarps * 32, (D == 64 && NT <= 2) ? 2 : 
                     }
                 }
                 __syncwarp();  // the stage and the tables are read
-                if (u_ahead < u_end) fetch(stage);
+                if (left_ahead > 0) fetch(stage);
                 if (++stage == p.stages) { stage = 0; phase ^= 1; }
             }
             if (timeout) {
@@ -605,21 +616,19 @@ __global__ void __launch_bounds__(kAttendWarps * 32, (D == 64 && NT <= 2) ? 2 : 
                     wait_bounded(&full[(stage + i) % p.stages], stage + i < p.stages ? phase : phase ^ 1);
                 break;
             }
-            u += n;
+            left -= n;
             // ---- the item's result: finished, or in the ring (the run is over), or in global memory ------------------------
-            float* slot = u == u_end ? reinterpret_cast<float*>(mine) : p.part + (((long long)p.grid * 2 + blockIdx.x * kAttendWarps + warp) * R) * kRow;
+            float* slot = left == 0 ? reinterpret_cast<float*>(mine) : p.part + ((long long)p.grid * 2 + blockIdx.x * kAttendWarps + warp) * kSlot;
+            const bool whole = starts && ends;
 #pragma unroll
             for (int j = 0; j < NT; ++j)
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
                     const int col = j * 8 + 2 * t + c;
                     if (col >= rows) continue;
-                    const int rr = r0 + col, head = cur.head * p.G + rr % p.G;
-                    const float inv = starts && ends ? inverse(l[j][c] + sink_of(p, head, m[j][c])) : 1.f;
-                    if (!(starts && ends) && g == 0) {
-                        slot[col * kRow] = m[j][c];
-                        slot[col * kRow + 1] = l[j][c];
-                    }
+                    const int token = p.token(r0 + col), head = cur.head * p.G + r0 + col - token * p.G;
+                    const float inv = whole ? inverse(l[j][c] + sink_of(p, head, m[j][c])) : 1.f;
+                    if (!whole && g == 0) *reinterpret_cast<float2*>(slot + R * D + col * 2) = make_float2(m[j][c], l[j][c]);
 #pragma unroll
                     for (int w = 0; w < NB / 2; ++w) {
                         const int blk = w * 2 + (g >> 2);
@@ -633,67 +642,76 @@ __global__ void __launch_bounds__(kAttendWarps * 32, (D == 64 && NT <= 2) ? 2 : 
                             x[2 * i] = o[j][w * 4 + i][c] * f;
                             x[2 * i + 1] = o[j][w * 4 + i][c + 2] * f;
                         }
-                        if (starts && ends) {
-                            store_out(p, ((long long)(q.row0 + rr / p.G) * p.s.nq + head) * D + w * 64 + g * 8, x);
-                        } else {
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) *reinterpret_cast<float2*>(slot + col * kRow + 2 + w * 64 + g * 8 + 2 * i) = make_float2(x[2 * i], x[2 * i + 1]);
-                        }
+                        if (whole) store_out(p, ((long long)(q.row0 + token) * p.s.nq + head) * D + w * 64 + g * 8, x);
+                        else store8(slot + col * D + w * 64 + g * 8, x);
                     }
                 }
-            if (!(starts && ends) && lane == 0) parts[warp * 2 + starts] = {1, starts, ends, q.row0, r0, rows, cur.head, slot};
+            if (!whole && lane == 0) parts[warp * 2 + starts] = {1, starts, ends, q.row0, r0, rows, cur.head, slot};
             // to the next item
             step += n;
             if (step == q.steps) {
                 step = 0;
-                next_item(cur, q, u);
+                next_item(cur, q, left);
             }
         }
     }
     __syncthreads();
-    // ---- the CTA's unfinished items: runs of its warps' partial results, in order -----------------------------------------
-    for (int a = 0; a < 2 * kAttendWarps;) {
-        if (!parts[a].there) { ++a; continue; }
-        int b = a, used[kAttendWarps + 1], n = 0;  // a .. b belong to one item
-        for (;; ++b) {
-            if (parts[b].there) {
-                if (n > 0 && parts[b].starts) break;  // the next item's
-                used[n++] = b;
-                if (parts[b].ends) { ++b; break; }
-            }
-            if (b + 1 == 2 * kAttendWarps) { ++b; break; }
-        }
+    // ---- the CTA's unfinished items: runs of its warps' partial results, in order.  A run ends with a part that has the
+    // item's last step, or before one that has the next item's first.
+    const Partial* part_of = &parts[lane & (2 * kAttendWarps - 1)];
+    const uint32_t all = (1u << 2 * kAttendWarps) - 1, is = __ballot_sync(0xffffffffu, part_of->there) & all;
+    const uint32_t first_of = __ballot_sync(0xffffffffu, part_of->there && part_of->starts) & all;
+    const uint32_t last_of = __ballot_sync(0xffffffffu, part_of->there && part_of->ends) & all;
+    for (uint32_t rest = is; rest;) {
+        const int a = __ffs(rest) - 1;
+        const uint32_t from = ~((1u << a) - 1), after = from & ~(1u << a);
+        int end = 2 * kAttendWarps;
+        if (last_of & from) end = min(end, __ffs(last_of & from));
+        if (first_of & after) end = min(end, __ffs(first_of & after) - 1);
+        const uint32_t members = is & from & ((1u << end) - 1);
+        rest &= ~members;
         const Partial& f = parts[a];
-        const bool starts = f.starts, ends = parts[used[n - 1]].ends;
-        float* slot = p.part + ((long long)blockIdx.x * 2 + starts) * R * kRow;
+        const bool starts = f.starts, ends = (last_of & members) != 0;
+        float* slot = p.part + ((long long)blockIdx.x * 2 + starts) * kSlot;
         for (int i = threadIdx.x; i < f.rows * (D / 8); i += kAttendWarps * 32) {
             const int col = i / (D / 8), c8 = i % (D / 8) * 8;
-            float M = kNoMax, den = 0.f, x[8] = {};
-            for (int k = 0; k < n; ++k) M = fmaxf(M, parts[used[k]].data[col * kRow]);
-            for (int k = 0; k < n; ++k) {
-                const float* src = parts[used[k]].data + col * kRow;
-                const float e = ex2(src[0] - M);
-                den = fmaf(src[1], e, den);
+            const float* src[kAttendWarps];
+            float2 ml[kAttendWarps];
+            float M = kNoMax;
+            uint32_t todo = members;
 #pragma unroll
-                for (int h = 0; h < 4; ++h) {
-                    const float2 v = *reinterpret_cast<const float2*>(src + 2 + c8 + 2 * h);
-                    x[2 * h] = fmaf(v.x, e, x[2 * h]);
-                    x[2 * h + 1] = fmaf(v.y, e, x[2 * h + 1]);
+            for (int k = 0; k < kAttendWarps; ++k) {
+                src[k] = nullptr;
+                ml[k] = make_float2(kNoMax, 0.f);
+                if (todo) {
+                    src[k] = parts[__ffs(todo) - 1].data;
+                    todo &= todo - 1;
+                    ml[k] = *reinterpret_cast<const float2*>(src[k] + R * D + col * 2);
+                    M = fmaxf(M, ml[k].x);
                 }
             }
+            float den = 0.f, x[8] = {};
+#pragma unroll
+            for (int k = 0; k < kAttendWarps; ++k)
+                if (src[k]) {
+                    const float e = ex2(ml[k].x - M);
+                    float v[8];
+                    load8(src[k] + col * D + c8, v);
+                    den = fmaf(ml[k].y, e, den);
+#pragma unroll
+                    for (int h = 0; h < 8; ++h) x[h] = fmaf(v[h], e, x[h]);
+                }
             if (starts && ends) {
-                const int rr = f.r0 + col, head = f.head * p.G + rr % p.G;
+                const int token = p.token(f.r0 + col), head = f.head * p.G + f.r0 + col - token * p.G;
                 const float inv = inverse(den + sink_of(p, head, M));
 #pragma unroll
                 for (int h = 0; h < 8; ++h) x[h] *= inv;
-                store_out(p, ((long long)(f.row0 + rr / p.G) * p.s.nq + head) * D + c8, x);
+                store_out(p, ((long long)(f.row0 + token) * p.s.nq + head) * D + c8, x);
             } else {
-                if (c8 == 0) { slot[col * kRow] = M; slot[col * kRow + 1] = den; }
-#pragma unroll
-                for (int h = 0; h < 4; ++h) *reinterpret_cast<float2*>(slot + col * kRow + 2 + c8 + 2 * h) = make_float2(x[2 * h], x[2 * h + 1]);
+                if (c8 == 0) *reinterpret_cast<float2*>(slot + R * D + col * 2) = make_float2(M, den);
+                store8(slot + col * D + c8, x);
             }
         }
-        a = b;
     }
 }
 
@@ -707,10 +725,10 @@ __global__ void __launch_bounds__(256) merge_kernel(const AttendParams p) {
     const int lane = threadIdx.x & 31;
     const long long task = (long long)blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
     const int row = (int)(task / p.s.nq), head = (int)(task % p.s.nq);
-    // the batch may be what the kernel before attend_kernel wrote: both have to be over
-    pdl_wait();
+    // This kernel starts once every CTA of attend_kernel has found what ran before it complete, so the batch may be read
+    // at once; the partial results only after pdl_wait().
     const long long share = scan_units(p, before);
-    if (row >= p.b.rows) return;
+    if (row >= p.b.rows) { pdl_wait(); return; }  // (every thread waits: this kernel is not over before attend_kernel is)
     // the row's sequence: the last whose first row is not behind it
     int s = row;
     if (p.b.cu_q) {
@@ -721,31 +739,34 @@ __global__ void __launch_bounds__(256) merge_kernel(const AttendParams p) {
         }
         s = lo;
     }
-    if (s >= p.b.n) return;
+    if (s >= p.b.n) { pdl_wait(); return; }
     const SeqPlan q = plan_of(p, s);
-    if (row < q.row0 || row >= q.row0 + q.n) return;
-    const int kvh = head / p.G, rr = (row - q.row0) * p.G + head % p.G, block = rr / p.R, col = rr % p.R;
+    if (row < q.row0 || row >= q.row0 + q.n) { pdl_wait(); return; }
+    const int kvh = p.token(head), rr = (row - q.row0) * p.G + head - kvh * p.G, block = rr >> (31 - __clz(p.R)), col = rr & (p.R - 1);
     const long long at = ((long long)row * p.s.nq + head) * D + lane * C;
     auto put = [&](int i, float x) {
         if (p.half) static_cast<__half*>(p.out)[at + i] = __float2half_rn(x);
         else static_cast<__nv_bfloat16*>(p.out)[at + i] = __float2bfloat16_rn(x);
     };
-    if (q.steps == 0) {
-#pragma unroll
-        for (int i = 0; i < C; ++i) put(i, 0.f);
-        return;
-    }
     const long long u0 = before[s] + ((long long)kvh * q.blocks + block) * q.steps, u1 = u0 + q.steps;
     const int c0 = u0 <= 0x7fffffff && share <= 0x7fffffff ? (int)((uint32_t)u0 / (uint32_t)share) : (int)(u0 / share);
-    if ((c0 + 1) * share >= u1) return;  // one CTA had all of it and wrote the result
-    // contributors: CTA c0 with its second slot (or its first, if the item began before it, which it does not), then first slots
-    const long long stride = 2ll * p.R * (D + 2);
-    const float* base = p.part + c0 * stride + (long long)col * (D + 2);
-    const int n = (int)((u1 - 1 - c0 * share) / share) + 1;
+    const bool none = q.steps == 0, merge = !none && (c0 + 1) * share < u1;  // else one CTA had all of it and wrote the result
+    // contributors: CTA c0, in which the item begins, with its second slot, then the following ones' first slots
+    const long long slot = (long long)p.R * (D + 2);
+    const float* base = p.part + c0 * 2 * slot;
+    const int n = merge ? (uint64_t)(u1 - 1 - c0 * share) <= 0x7fffffff && share <= 0x7fffffff ? (int)((uint32_t)(u1 - 1 - c0 * share) / (uint32_t)share) + 1
+                                                                                            : (int)((u1 - 1 - c0 * share) / share) + 1
+                        : 0;
+    pdl_wait();
+    if (none) {  // zeros only now: what ran before attend_kernel may still have read the buffer
+#pragma unroll
+        for (int i = 0; i < C; ++i) put(i, 0.f);
+    }
+    if (!merge) return;
     float M = kNoMax, den = 0.f, acc[C] = {};
     for (int k0 = 0; k0 < n; k0 += 32) {
         const int k = k0 + lane;
-        const float* src = base + k * stride + (k == 0 ? (long long)p.R * (D + 2) : 0);
+        const float* src = base + (k == 0 ? slot : 2 * k * slot) + p.R * D + col * 2;
         const float m = k < n ? src[0] : kNoMax, l = k < n ? src[1] : 0.f;
         float now = fmaxf(M, m);
 #pragma unroll
@@ -760,7 +781,7 @@ __global__ void __launch_bounds__(256) merge_kernel(const AttendParams p) {
         const int here = min(32, n - k0);
 #pragma unroll 4
         for (int j = 0; j < here; ++j) {
-            const float* from = base + (k0 + j) * stride + (k0 + j == 0 ? (long long)p.R * (D + 2) : 0) + 2 + lane * C;
+            const float* from = base + (k0 + j == 0 ? slot : 2 * (k0 + j) * slot) + col * D + lane * C;
             const float w = __shfl_sync(0xffffffffu, f, j);
 #pragma unroll
             for (int i = 0; i < C; ++i) acc[i] = fmaf(from[i], w, acc[i]);

@@ -164,6 +164,7 @@ int launch_attend(const Shape& s, const Batch& b, const uint8_t* cache, int dtyp
     const int nt = column_groups(s, max_rows);
     p.grid = attend_grid(s, b, nt);
     p.R = 8 * nt;
+    p.G_inverse = (uint32_t)((0x100000000ull + p.G - 1) / p.G);
     each_variant([&](int dim, int page, int groups, auto variant) {
         return dim == s.D && page == s.P && groups == nt ? variant(&p, st) : cudaSuccess;
     });
