@@ -17,15 +17,12 @@ from . import _lib
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
+_stream_of = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 def _need(ok: bool, what: str) -> None:
     if not ok:
         raise ValueError(what)
-
-
-def _ints(t, name: str, dims: int):
-    _need(t.is_cuda and t.dtype == torch.int32 and t.dim() == dims and (t.shape[-1] <= 1 or t.stride(-1) == 1),
-          f"{name}: a contiguous int32 CUDA tensor of {dims} dimension(s)")
-    return t.data_ptr()
 
 
 class Kv4Batch:
@@ -33,26 +30,27 @@ class Kv4Batch:
     are read when the kernels run; they may be rewritten in place between the replays of a captured graph."""
 
     def __init__(self, seq_lens, page_table, cu_q=None):
-        n = seq_lens.shape[0]
-        _need(page_table.dim() == 2 and page_table.shape[0] == n, "page_table: [batch, pages]")
-        _need(cu_q is None or cu_q.shape[0] == n + 1, "cu_q: [batch + 1]")
-        _need(all(t is None or t.device == seq_lens.device for t in (page_table, cu_q)), "the batch's tensors are on several devices")
+        shape, stride = page_table.shape, page_table.stride()
+        if seq_lens.dtype is not torch.int32 or seq_lens.dim() != 1 or not seq_lens.is_contiguous() or not seq_lens.is_cuda:
+            raise ValueError("seq_lens: contiguous int32 [batch] in device memory")
+        n, index = seq_lens.shape[0], seq_lens.get_device()
+        if page_table.dtype is not torch.int32 or len(shape) != 2 or shape[0] != n or (stride[1] != 1 and shape[1] > 1) \
+                or page_table.get_device() != index:
+            raise ValueError("page_table: int32 [batch, pages], rows contiguous, where seq_lens is")
+        if cu_q is not None and (cu_q.dtype is not torch.int32 or cu_q.shape != (n + 1,) or not cu_q.is_contiguous() or cu_q.get_device() != index):
+            raise ValueError("cu_q: contiguous int32 [batch + 1] where seq_lens is")
         self._keep = (seq_lens, page_table, cu_q)
-        self.device = seq_lens.device
-        self.batch = n
-        self.one_each = cu_q is None
-        self._c = _lib.NeonKv4Batch(_ints(seq_lens, "seq_lens", 1), None if cu_q is None else _ints(cu_q, "cu_q", 1),
-                                    _ints(page_table, "page_table", 2), page_table.stride(0) if n > 1 else page_table.shape[1],
-                                    page_table.shape[1], n, 0)
+        self.device_index, self.batch, self.one_each = index, n, cu_q is None
+        self._c = _lib.NeonKv4Batch(seq_lens.data_ptr(), None if cu_q is None else cu_q.data_ptr(), page_table.data_ptr(),
+                                    stride[0] if n > 1 else shape[1], shape[1], n, 0)
         self._ref = ctypes.byref(self._c)
-        self._scratch = {}
 
 
 class Kv4Cache:
     def __init__(self, n_q_heads: int, n_kv_heads: int, head_dim: int, page_size: int = 64, device: int = 0):
         self._lib = _lib.load()
         self.n_q_heads, self.n_kv_heads, self.head_dim, self.page_size = int(n_q_heads), int(n_kv_heads), int(head_dim), int(page_size)
-        self.device = torch.device("cuda", int(device))
+        self.device, self._index = torch.device("cuda", int(device)), int(device)
         cfg = _lib.NeonKv4Config(self.n_q_heads, self.n_kv_heads, self.head_dim, self.page_size, int(device))
         handle = ctypes.c_void_p()
         rc = self._lib.neon_kv4_create(ctypes.byref(cfg), ctypes.byref(handle))
@@ -65,23 +63,21 @@ class Kv4Cache:
         if rc != 0:
             raise RuntimeError(f"{what} failed ({rc}): {self._lib.neon_kv4_last_error(self._h).decode()}")
 
-    def _stream(self, stream) -> int:
-        return (torch.cuda.current_stream(self.device) if stream is None else stream).cuda_stream
-
     def _place(self, batch: Kv4Batch, cache) -> int:
-        _need(cache.dtype == torch.uint8 and cache.dim() == 3 and cache.shape[1] == self.n_kv_heads and cache.shape[2] == self.record_bytes
-              and cache.is_contiguous(), f"cache: contiguous uint8 [n_pages, {self.n_kv_heads}, {self.record_bytes}]")
-        _need(cache.device == self.device and batch.device == self.device, f"cache and batch have to be on {self.device}")
-        batch._c.n_pages = cache.shape[0]
+        shape = cache.shape
+        if cache.dtype is not torch.uint8 or len(shape) != 3 or shape[1] != self.n_kv_heads or shape[2] != self.record_bytes \
+                or not cache.is_contiguous() or cache.get_device() != self._index or batch.device_index != self._index:
+            raise ValueError(f"cache: contiguous uint8 [n_pages, {self.n_kv_heads}, {self.record_bytes}] on {self.device}, where the batch is")
+        batch._c.n_pages = shape[0]
         return cache.data_ptr()
 
-    def _rows(self, t, heads: int, name: str, rows=None) -> int:
-        """Checks [rows, heads, head_dim] with whole rows apart by any stride; returns the stride in elements."""
-        _need(t.dim() == 3 and t.shape[1] == heads and t.shape[2] == self.head_dim and (rows is None or t.shape[0] == rows),
-              f"{name}: [rows, {heads}, {self.head_dim}]")
-        _need(t.stride(2) == 1 and (heads == 1 or t.stride(1) == self.head_dim), f"{name}: the heads of a row have to be contiguous")
-        _need(t.device == self.device, f"{name} has to be on {self.device}")
-        return t.stride(0) if t.shape[0] > 1 else heads * self.head_dim
+    def _rows(self, t, heads: int, rows: int, name: str) -> int:
+        """Checks [rows, heads, head_dim] with whole rows any stride apart; returns the stride in elements."""
+        stride = t.stride()
+        if t.shape != (rows, heads, self.head_dim) or stride[2] != 1 or (stride[1] != self.head_dim and heads > 1) \
+                or t.get_device() != self._index:
+            raise ValueError(f"{name}: [{rows}, {heads}, {self.head_dim}] on {self.device}, the heads of a row contiguous")
+        return stride[0] if rows > 1 else heads * self.head_dim
 
     # -- caches and batches ----------------------------------------------------------------
     def new_cache(self, n_pages: int):
@@ -97,23 +93,26 @@ class Kv4Cache:
         their rows' positions and writes ``k`` and ``v`` to the pages.  Returns the rotated queries (bf16, or fp16 for fp16
         input, or ``out``'s type); ``q`` may be None."""
         rows = k.shape[0]
-        ks, vs = self._rows(k, self.n_kv_heads, "k"), self._rows(v, self.n_kv_heads, "v", rows)
-        _need(k.dtype in _DTYPES and v.dtype == k.dtype and (q is None or q.dtype == k.dtype), "q, k and v: one of float32, bfloat16, float16")
-        _need(inv_freq.dtype == torch.float32 and inv_freq.shape == (self.head_dim // 2,) and inv_freq.is_contiguous()
-              and inv_freq.device == self.device, f"inv_freq: float32 [{self.head_dim // 2}]")
-        qs = 0
+        ks, vs = self._rows(k, self.n_kv_heads, rows, "k"), self._rows(v, self.n_kv_heads, rows, "v")
+        dtype = k.dtype
+        _need(dtype in _DTYPES and v.dtype is dtype and (q is None or q.dtype is dtype), "q, k and v: one of float32, bfloat16, float16")
+        _need(inv_freq.dtype is torch.float32 and inv_freq.shape == (self.head_dim // 2,) and inv_freq.is_contiguous()
+              and inv_freq.get_device() == self._index, f"inv_freq: float32 [{self.head_dim // 2}]")
+        qs = out_dtype = 0
+        q_ptr = out_ptr = None
         if q is not None:
-            qs = self._rows(q, self.n_q_heads, "q", rows)
+            qs = self._rows(q, self.n_q_heads, rows, "q")
             if out is None:
-                out = torch.empty((rows, self.n_q_heads, self.head_dim), dtype=torch.float16 if q.dtype == torch.float16 else torch.bfloat16,
+                out = torch.empty((rows, self.n_q_heads, self.head_dim), dtype=torch.float16 if dtype is torch.float16 else torch.bfloat16,
                                   device=self.device)
-            self._rows(out, self.n_q_heads, "out", rows)
-            _need(out.dtype in (torch.bfloat16, torch.float16) and out.is_contiguous(), "out: contiguous, bfloat16 or float16")
-        cache_ptr = self._place(batch, cache)
-        self._check(self._lib.neon_kv4_append(
-            self._h, batch._ref, cache_ptr, rows, _DTYPES[k.dtype], None if q is None else q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs,
-            inv_freq.data_ptr(), mscale, None if q is None else out.data_ptr(), 0 if q is None else _DTYPES[out.dtype], self._stream(stream)),
-            "neon_kv4_append")
+            elif out.dtype not in (torch.bfloat16, torch.float16) or out.shape != q.shape or not out.is_contiguous() or out.get_device() != self._index:
+                raise ValueError("out: contiguous, bfloat16 or float16, q's shape")
+            q_ptr, out_ptr, out_dtype = q.data_ptr(), out.data_ptr(), _DTYPES[out.dtype]
+        rc = self._lib.neon_kv4_append(self._h, batch._ref, self._place(batch, cache), rows, _DTYPES[dtype], q_ptr, qs, k.data_ptr(), ks, v.data_ptr(),
+                                       vs, inv_freq.data_ptr(), mscale, out_ptr, out_dtype,
+                                       _stream_of(self._index) if stream is None else stream.cuda_stream)
+        if rc:
+            self._check(rc, "neon_kv4_append")
         return out if q is not None else None
 
     def read(self, batch: Kv4Batch, cache, rows: int | None = None, dtype=torch.bfloat16, out=None, stream=None):
@@ -122,43 +121,47 @@ class Kv4Cache:
         if out is None:
             rows = batch.batch if rows is None else rows
             out = [torch.zeros((rows, self.n_kv_heads, self.head_dim), dtype=dtype, device=self.device) for _ in range(2)]
-        rows = out[0].shape[0]
-        for t in out:
-            self._rows(t, self.n_kv_heads, "out", rows)
-            _need(t.dtype in (torch.bfloat16, torch.float32) and t.dtype == out[0].dtype and t.is_contiguous(), "out: contiguous, bfloat16 or float32")
-        cache_ptr = self._place(batch, cache)
-        self._check(self._lib.neon_kv4_read(self._h, batch._ref, cache_ptr, rows, out[0].data_ptr(), out[1].data_ptr(), _DTYPES[out[0].dtype],
-                                            self._stream(stream)), "neon_kv4_read")
-        return out[0], out[1]
+        k, v = out
+        rows, dtype = k.shape[0], k.dtype
+        self._rows(k, self.n_kv_heads, rows, "out")
+        _need(dtype in (torch.bfloat16, torch.float32) and v.dtype is dtype and v.shape == k.shape and k.is_contiguous() and v.is_contiguous()
+              and v.get_device() == self._index, "out: two contiguous tensors of bfloat16 or float32")
+        rc = self._lib.neon_kv4_read(self._h, batch._ref, self._place(batch, cache), rows, k.data_ptr(), v.data_ptr(), _DTYPES[dtype],
+                                     _stream_of(self._index) if stream is None else stream.cuda_stream)
+        if rc:
+            self._check(rc, "neon_kv4_read")
+        return k, v
 
     def attend(self, batch: Kv4Batch, cache, q, sinks=None, window: int = 0, scale: float | None = None, max_rows: int | None = None,
                out=None, stream=None):
         """Attention of ``q`` [rows, n_q_heads, head_dim] (bf16 or fp16, rotated) over the cache; ``sinks``: bf16 [n_q_heads] logits of the
         softmax denominator; ``window`` > 0: only the last so many positions; ``scale``: default head_dim ** -0.5; ``max_rows``: the
         most rows of a sequence, if the host knows it (speed only)."""
-        rows = q.shape[0]
-        qs = self._rows(q, self.n_q_heads, "q")
-        _need(q.dtype in (torch.bfloat16, torch.float16), "q: bfloat16 or float16")
-        _need(sinks is None or (sinks.dtype == torch.bfloat16 and sinks.shape == (self.n_q_heads,) and sinks.is_contiguous()
-                                and sinks.device == self.device), f"sinks: bfloat16 [{self.n_q_heads}]")
+        rows, dtype = q.shape[0], q.dtype
+        qs = self._rows(q, self.n_q_heads, rows, "q")
+        _need(dtype is torch.bfloat16 or dtype is torch.float16, "q: bfloat16 or float16")
+        _need(sinks is None or (sinks.dtype is torch.bfloat16 and sinks.shape == (self.n_q_heads,) and sinks.is_contiguous()
+                                and sinks.get_device() == self._index), f"sinks: bfloat16 [{self.n_q_heads}]")
         if out is None:
-            out = torch.empty((rows, self.n_q_heads, self.head_dim), dtype=q.dtype, device=self.device)
-        self._rows(out, self.n_q_heads, "out", rows)
-        _need(out.dtype == q.dtype and out.is_contiguous(), "out: contiguous, q's type")
+            out = torch.empty((rows, self.n_q_heads, self.head_dim), dtype=dtype, device=self.device)
+        elif out.dtype is not dtype or out.shape != q.shape or not out.is_contiguous() or out.get_device() != self._index:
+            raise ValueError("out: contiguous, q's type and shape")
         if max_rows is None:
             max_rows = 1 if batch.one_each else rows
         cache_ptr = self._place(batch, cache)
-        size = batch._scratch.get((rows, max_rows, self._h.value))
-        if size is None:
-            size = batch._scratch[(rows, max_rows, self._h.value)] = int(self._lib.neon_kv4_attend_workspace(self._h, batch._ref, rows, max_rows))
-        st = torch.cuda.current_stream(self.device) if stream is None else stream
+        lib, handle, ref = self._lib, self._h, batch._ref
+        size = lib.neon_kv4_attend_workspace(handle, ref, rows, max_rows)
+        # allocated on the current stream, so that two calls never share it; torch reuses it in stream order
         scratch = torch.empty(size, dtype=torch.uint8, device=self.device)
-        if stream is not None:
+        if stream is None:
+            st = _stream_of(self._index)
+        else:
+            st = stream.cuda_stream
             scratch.record_stream(stream)
-        self._check(self._lib.neon_kv4_attend(
-            self._h, batch._ref, cache_ptr, rows, _DTYPES[q.dtype], q.data_ptr(), qs, None if sinks is None else sinks.data_ptr(), window,
-            self.head_dim ** -0.5 if scale is None else scale, max_rows, out.data_ptr(), scratch.data_ptr(), size, st.cuda_stream),
-            "neon_kv4_attend")
+        rc = lib.neon_kv4_attend(handle, ref, cache_ptr, rows, _DTYPES[dtype], q.data_ptr(), qs, None if sinks is None else sinks.data_ptr(), window,
+                                 self.head_dim ** -0.5 if scale is None else scale, max_rows, out.data_ptr(), scratch.data_ptr(), size, st)
+        if rc:
+            self._check(rc, "neon_kv4_attend")
         return out
 
     # -- inspection ----------------------------------------------------------------------------

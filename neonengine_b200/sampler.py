@@ -13,12 +13,13 @@ import torch
 from . import _lib
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_stream_of = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 class Sampler:
     def __init__(self, vocab: int, device: int = 0):
         self._lib = _lib.load()
-        self.vocab, self.device = int(vocab), torch.device("cuda", int(device))
+        self.vocab, self.device, self._index = int(vocab), torch.device("cuda", int(device)), int(device)
         cfg = _lib.NeonSamplerConfig(self.vocab, int(device))
         handle = ctypes.c_void_p()
         rc = self._lib.neon_sampler_create(ctypes.byref(cfg), ctypes.byref(handle))
@@ -30,7 +31,7 @@ class Sampler:
     def _vector(self, t, rows: int, dtype, name: str):
         if t is None:
             return None
-        if t.dtype != dtype or t.shape != (rows,) or t.device != self.device or not t.is_contiguous():
+        if t.dtype is not dtype or t.shape != (rows,) or t.get_device() != self._index or not t.is_contiguous():
             raise ValueError(f"{name}: contiguous {dtype} [{rows}] on {self.device}")
         return t.data_ptr()
 
@@ -38,32 +39,34 @@ class Sampler:
         """Tokens int32 [rows] of ``logits`` [rows, vocab] (fp32, bf16 or fp16; rows may be any stride apart).  ``uniform``: fp32
         [rows] in [0, 1); ``temperature``, ``top_p``, ``min_p`` fp32 [rows] and ``top_k`` int32 [rows], or None.  With ``details``
         returns (tokens, probability of each among what was kept, how many were kept)."""
-        if logits.dim() != 2 or logits.shape[1] != self.vocab or logits.dtype not in _DTYPES or logits.device != self.device or \
-                (self.vocab > 1 and logits.stride(1) != 1):
+        shape, stride, dtype, f32 = logits.shape, logits.stride(), logits.dtype, torch.float32
+        if len(shape) != 2 or shape[1] != self.vocab or dtype not in _DTYPES or logits.get_device() != self._index or (stride[1] != 1 and shape[1] > 1):
             raise ValueError(f"logits: [rows, {self.vocab}] of float32, bfloat16 or float16 on {self.device}, rows contiguous")
-        rows = logits.shape[0]
-        args = (self._vector(uniform, rows, torch.float32, "uniform"), self._vector(temperature, rows, torch.float32, "temperature"),
-                self._vector(top_k, rows, torch.int32, "top_k"), self._vector(top_p, rows, torch.float32, "top_p"),
-                self._vector(min_p, rows, torch.float32, "min_p"))
         if uniform is None:
             raise ValueError("uniform: one random number per row")
+        rows, vector = shape[0], self._vector
+        u, t, k = vector(uniform, rows, f32, "uniform"), vector(temperature, rows, f32, "temperature"), vector(top_k, rows, torch.int32, "top_k")
+        p, m = vector(top_p, rows, f32, "top_p"), vector(min_p, rows, f32, "min_p")
         size = self._scratch.get(rows)
         if size is None:
             size = self._scratch[rows] = int(self._lib.neon_sampler_workspace(self._h, rows))
-        tokens = torch.empty((rows,), dtype=torch.int32, device=self.device) if out is None else out
-        self._vector(tokens, rows, torch.int32, "out")
-        probs = kept = None
+        device = self.device
+        tokens = torch.empty(rows, dtype=torch.int32, device=device) if out is None else out
+        tokens_ptr = tokens.data_ptr() if out is None else vector(out, rows, torch.int32, "out")
+        probs = kept = probs_ptr = kept_ptr = None
         if details:
-            probs = torch.empty((rows,), dtype=torch.float32, device=self.device)
-            kept = torch.empty((rows,), dtype=torch.int32, device=self.device)
-        scratch = torch.empty(max(size, 16), dtype=torch.uint8, device=self.device)
-        if stream is not None:
+            probs, kept = torch.empty(rows, dtype=f32, device=device), torch.empty(rows, dtype=torch.int32, device=device)
+            probs_ptr, kept_ptr = probs.data_ptr(), kept.data_ptr()
+        # allocated on the current stream, so that two runs never share it; torch reuses it in stream order
+        scratch = torch.empty(size, dtype=torch.uint8, device=device)
+        if stream is None:
+            st = _stream_of(self._index)
+        else:
+            st = stream.cuda_stream
             scratch.record_stream(stream)
-        st = torch.cuda.current_stream(self.device) if stream is None else stream
-        rc = self._lib.neon_sampler_run(self._h, logits.data_ptr(), _DTYPES[logits.dtype], logits.stride(0) if rows > 1 else self.vocab, rows,
-                                        *args, tokens.data_ptr(), probs.data_ptr() if details else None, kept.data_ptr() if details else None,
-                                        scratch.data_ptr(), size, st.cuda_stream)
-        if rc != 0:
+        rc = self._lib.neon_sampler_run(self._h, logits.data_ptr(), _DTYPES[dtype], stride[0] if rows > 1 else self.vocab, rows, u, t, k, p, m,
+                                        tokens_ptr, probs_ptr, kept_ptr, scratch.data_ptr(), size, st)
+        if rc:
             raise RuntimeError(f"neon_sampler_run failed ({rc}): {self._lib.neon_sampler_last_error(self._h).decode()}")
         return (tokens, probs, kept) if details else tokens
 
