@@ -88,15 +88,27 @@ int launch(const void* logits, int dtype, long long row_stride, int vocab, int b
     p.left = reinterpret_cast<int*>(p.heads + n);
     // a warp lists some 1.4 times as many elements as lanes' maxima pass its bound; all warps' lists are to fit pick's
     p.rank = p.chunks <= 220 ? 16 : 8;
-    const unsigned grid = (unsigned)((n + kScanWarps - 1) / kScanWarps);
-    if (dtype == NEON_SAMPLER_F32) scan_kernel<0><<<grid, kScanWarps * 32, 0, st>>>(p);
-    else if (dtype == NEON_SAMPLER_BF16) scan_kernel<1><<<grid, kScanWarps * 32, 0, st>>>(p);
-    else scan_kernel<2><<<grid, kScanWarps * 32, 0, st>>>(p);
-    pick_kernel<<<batch, kPickThreads, sizeof(PickSmem), st>>>(p, 0);
+    const unsigned grid = (unsigned)std::min<size_t>((n + kScanWarps - 1) / kScanWarps, 2 * kSms);
+    void (*scan)(Params) = dtype == NEON_SAMPLER_F32 ? scan_kernel<0> : dtype == NEON_SAMPLER_BF16 ? scan_kernel<1> : scan_kernel<2>;
+    scan<<<grid, kScanWarps * 32, 0, st>>>(p);
+    // each starts while its predecessor drains and waits for it before it reads what that wrote
+    cudaLaunchConfig_t cfg{};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.blockDim = dim3(kPickThreads);
+    cfg.stream = st;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    cfg.gridDim = dim3(batch);
+    cfg.dynamicSmemBytes = sizeof(PickSmem);
+    cudaLaunchKernelEx(&cfg, pick_kernel, static_cast<const Params>(p), 0);
     if (!top_k && !top_p && !min_p) return 2;  // pick leaves nothing
     const size_t smem = whole_smem(vocab);
     const int clusters = std::min(batch, (int)(kSms / kClusterCtas * (kSharedPerSm / (smem + 1024))));
-    whole_kernel<<<std::max(clusters, 1) * kClusterCtas, kPickThreads, smem, st>>>(p);
+    cfg.gridDim = dim3(std::max(clusters, 1) * kClusterCtas);
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchKernelEx(&cfg, whole_kernel, static_cast<const Params>(p));
     return 3;
 }
 

@@ -8,8 +8,9 @@
 //   whole    a cluster per row that keeps the row in its shared memory and finds cuts and token among all of it.
 // Vocabularies that fit pick's list go to pick alone.
 //
-// Cuts and token are found in the same way: "the first key at which a running sum (of ones or of weights) reaches a
-// target" by histograms over ten bits of the key at a time - the key being the logit in descending order, or the index.
+// One histogram over the list cuts it down to what the first filter can keep.  Up to 512 elements are then sorted, one a
+// thread, and every cut is a running sum away; more are cut by histograms over ten bits of the key at a time, the key being
+// the logit in descending order (or the index).
 // Weights are integers of 2^-43 of the largest, so that sums depend on no order; a histogram keeps them as three words
 // of 15 bits each per element, which shared memory can add atomically.
 #pragma once
@@ -30,7 +31,7 @@ namespace cg = cooperative_groups;
 constexpr int kChunk = 1024;          // logits of a warp of the scan
 constexpr int kSlots = 64;            // list entries a warp can leave
 constexpr int kList = 6144;           // list entries of pick
-constexpr int kPickThreads = 512, kScanWarps = 4;
+constexpr int kPickThreads = 512, kScanWarps = 8;
 constexpr int kBins = 1024, kBinBits = 10;
 constexpr int kWeightBits = 43;       // weights are multiples of 2^-43; a row's sum stays below 2^63
 constexpr double kUnit = 8796093022208.0;  // 2^43
@@ -60,7 +61,7 @@ struct Params {
 
 struct Rule {  // a row's parameters, with what they exclude made plain
     bool greedy, by_k, by_p, by_m;
-    double c;  // log2(e) / temperature
+    double c;  // log2(e) / temperature; at least 2^-500, so that 1/c is finite
     int k;
     double p, m;
     float u;
@@ -70,7 +71,7 @@ __device__ __forceinline__ Rule rule_of(const Params& p, int row) {
     Rule r;
     const float t = p.temperature ? p.temperature[row] : 1.f;
     r.greedy = !(t > 0.f);
-    r.c = r.greedy ? 1.0 : 1.4426950408889634074 / (double)t;
+    r.c = r.greedy ? 1.0 : fmax(1.4426950408889634074 / (double)t, 0x1p-500);
     r.k = p.top_k ? p.top_k[row] : 0;
     r.by_k = r.k > 0 && r.k < p.vocab;
     const float tp = p.top_p ? p.top_p[row] : 1.f, mp = p.min_p ? p.min_p[row] : 0.f;
@@ -83,7 +84,7 @@ __device__ __forceinline__ Rule rule_of(const Params& p, int row) {
     return r;
 }
 
-__device__ __forceinline__ float clean(float x) { return x != x ? -INFINITY : x + 0.f; }  // NaN is -infinity, -0 is 0
+__device__ __forceinline__ float clean(float x) { return fmaxf(x, -INFINITY); }  // NaN is -infinity
 __device__ __forceinline__ float load1(const Params& p, long long i) {
     float x;
     if (p.dtype == 0) x = __ldg(static_cast<const float*>(p.logits) + i);
@@ -93,29 +94,43 @@ __device__ __forceinline__ float load1(const Params& p, long long i) {
 }
 // ascending keys for descending logits
 __device__ __forceinline__ uint32_t order_key(float x) {
-    const uint32_t b = __float_as_uint(x);
+    const uint32_t b = __float_as_uint(x + 0.f);  // -0 is 0
     return b & 0x80000000u ? b : ~b & 0x7fffffffu;
 }
 __device__ __forceinline__ float key_logit(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k : ~k & 0x7fffffffu); }
 
-// 2^(j/128), j < 128
+// 2^(j/64), j < 64, a copy for every lane: reads never share a bank
+constexpr int kTable = 64 * 32;
 __device__ __forceinline__ void fill_table(double* tab) {
-    for (int j = threadIdx.x; j < 128; j += blockDim.x) tab[j] = exp2(j / 128.0);
+    for (int j = threadIdx.x; j < 64; j += blockDim.x) {
+        const double v = exp2(j / 64.0);
+        for (int l = 0; l < 32; ++l) tab[j * 32 + ((l + j) & 31)] = v;
+    }
 }
-// exp of (x - top) / temperature, to 3e-12: a table of 2^(j/128) times a cubic on the remainder, whose next term is
-// (ln 2 / 256)^4 / 24 = 2.2e-12
-__device__ __forceinline__ double weight_of(float x, float top, double c, const double* tab) {
-    const double kMagic = 6755399441055744.0;  // 1.5 * 2^52: the sum's low word is the rounded integer
-    if (x == top) return 1.0;
-    const double t = ((double)x - (double)top) * c;
-    if (!(t > -64.0)) return 0.0;
-    const double kd = fma(t, 128.0, kMagic);
-    const int k = __double2loint(kd);
-    const double r = fma(kd - kMagic, -1.0 / 128.0, t);
-    const double q = r * fma(r, fma(r, 0.055504108664821580, 0.24022650695910071), 0.69314718055994531);
-    const double w = fma(tab[k & 127], q, tab[k & 127]);
-    return __hiloint2double(__double2hiint(w) + ((k >> 7) << 20), __double2loint(w));
-}
+// exp((x - top) / temperature) to 4e-11: with t = 64 (x - top) log2(e) / temperature = k + r, |r| <= 1/2, a table of 2^(k/64)
+// times a cubic in r, whose next term is (ln 2 / 128)^4 / 24 = 3.6e-11.  What is below 2^-60 counts as nothing.
+struct Weigher {
+    double c, off;  // t = c x + off
+    float top, low;
+    const double* tab;  // this lane's column
+    __device__ __forceinline__ Weigher(float top_, double log2_scale, const double* table) : top(top_), tab(table + (threadIdx.x & 31)) {
+        c = 64.0 * log2_scale;
+        off = -c * (double)top;
+        low = fmaxf((float)((double)top - 60.0 / log2_scale), kLowest);
+        if (top == INFINITY) { low = INFINITY; c = 0.0; off = 0.0; }  // infinities alone, at weight 1
+    }
+    // of an x >= low (of another: any number)
+    __device__ __forceinline__ double bare(float x) const {
+        const double kMagic = 6755399441055744.0;  // 1.5 * 2^52: the sum's low word is the rounded integer
+        const double kA = 0.010830424696249145, kB = 5.8649049505537566e-05, kC = 2.1173136998904953e-07;  // A = ln 2 / 64, A^2 / 2, A^3 / 6
+        const double t = top == INFINITY ? 0.0 : fma((double)x, c, off), kd = t + kMagic;
+        const int k = __double2loint(kd);
+        const double r = t - (kd - kMagic), v = tab[(k & 63) * 32];
+        const double w = fma(v, r * fma(r, fma(r, kC, kB), kA), v);
+        return __hiloint2double(__double2hiint(w) + ((k >> 6) << 20), __double2loint(w));
+    }
+    __device__ __forceinline__ double operator()(float x) const { return x == top ? 1.0 : x >= low ? bare(x) : 0.0; }  // exactly 1 for the largest
+};
 __device__ __forceinline__ u64 to_units(double w) {  // w <= 2^9, in 2^-43, rounded
     return (u64)(__double_as_longlong(fma(w, kUnit, 4503599627370496.0)) & 0xfffffffffffffll);
 }
@@ -134,115 +149,131 @@ __device__ __forceinline__ float warp_sorted(float v) {
     return v;
 }
 
+// Warps go through the chunks of all rows; a chunk's row, its rule and its logits are one after the other in memory, so the
+// next chunk's loads need nothing of this one's.
 template <int DT>
-__global__ void __launch_bounds__(kScanWarps * 32) scan_kernel(const Params p) {
-    __shared__ double tab[128];
+__global__ void __launch_bounds__(kScanWarps * 32, 2) scan_kernel(const Params p) {
+    __shared__ double tab[kTable];
     const int lane = threadIdx.x & 31;
-    pdl_wait();
-    pdl_launch_dependents();
     fill_table(tab);
     __syncthreads();
-    const long long task = (long long)blockIdx.x * kScanWarps + threadIdx.x / 32;
-    const int row = (int)(task / p.chunks), chunk = (int)(task % p.chunks);
-    if (row >= p.batch) return;
-    const int i0 = chunk * kChunk, n = min(kChunk, p.vocab - i0);
-    const long long base = row * p.stride + i0;
-    float x[32];  // element 4 * (32 v + lane) + c is x[4 v + c]
-    constexpr int kSize = DT == 0 ? 4 : 2;
-    if (n == kChunk && ((reinterpret_cast<uintptr_t>(p.logits) + base * kSize) & (4 * kSize - 1)) == 0) {
+    pdl_wait();
+    pdl_launch_dependents();
+    const int tasks = p.batch * p.chunks;
+    for (int task = blockIdx.x * kScanWarps + threadIdx.x / 32; task < tasks; task += gridDim.x * kScanWarps) {
+        const int row = task / p.chunks, chunk = task - row * p.chunks;
+        const int i0 = chunk * kChunk, n = min(kChunk, p.vocab - i0);
+        const long long base = row * p.stride + i0;
+        float x[32];  // element 4 * (32 v + lane) + c is x[4 v + c]
+        constexpr int kSize = DT == 0 ? 4 : 2;
+        if (n == kChunk && ((reinterpret_cast<uintptr_t>(p.logits) + base * kSize) & (4 * kSize - 1)) == 0) {
 #pragma unroll
-        for (int v = 0; v < 8; ++v) {
-            const long long at = base + 4 * (32 * v + lane);
-            if (DT == 0) {
-                const float4 f = __ldcs(reinterpret_cast<const float4*>(static_cast<const float*>(p.logits) + at));
-                x[4 * v] = f.x; x[4 * v + 1] = f.y; x[4 * v + 2] = f.z; x[4 * v + 3] = f.w;
-            } else {
-                const uint2 f = __ldcs(reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p.logits) + at));
-                const uint32_t w[2] = {f.x, f.y};
+            for (int v = 0; v < 8; ++v) {
+                const long long at = base + 4 * (32 * v + lane);
+                if (DT == 0) {
+                    const float4 f = __ldcs(reinterpret_cast<const float4*>(static_cast<const float*>(p.logits) + at));
+                    x[4 * v] = f.x; x[4 * v + 1] = f.y; x[4 * v + 2] = f.z; x[4 * v + 3] = f.w;
+                } else {
+                    const uint2 f = __ldcs(reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p.logits) + at));
+                    const uint32_t w[2] = {f.x, f.y};
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    if (DT == 1) {
-                        x[4 * v + 2 * h] = __uint_as_float(w[h] << 16);
-                        x[4 * v + 2 * h + 1] = __uint_as_float(w[h] & 0xffff0000u);
-                    } else {
-                        const float2 g = __half22float2(*reinterpret_cast<const __half2*>(&w[h]));
-                        x[4 * v + 2 * h] = g.x;
-                        x[4 * v + 2 * h + 1] = g.y;
+                    for (int h = 0; h < 2; ++h) {
+                        if (DT == 1) {
+                            x[4 * v + 2 * h] = __uint_as_float(w[h] << 16);
+                            x[4 * v + 2 * h + 1] = __uint_as_float(w[h] & 0xffff0000u);
+                        } else {
+                            const float2 g = __half22float2(*reinterpret_cast<const __half2*>(&w[h]));
+                            x[4 * v + 2 * h] = g.x;
+                            x[4 * v + 2 * h + 1] = g.y;
+                        }
                     }
                 }
             }
+#pragma unroll
+            for (int i = 0; i < 32; ++i) x[i] = clean(x[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+                const int e = 4 * (32 * (i / 4) + lane) + i % 4;
+                x[i] = e < n ? load1(p, base + e) : -INFINITY;
+            }
         }
+        const Rule r = rule_of(p, row);
+        float top = x[0], least = x[0];
 #pragma unroll
-        for (int i = 0; i < 32; ++i) x[i] = clean(x[i]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-            const int e = 4 * (32 * (i / 4) + lane) + i % 4;
-            x[i] = e < n ? load1(p, base + e) : -INFINITY;
+        for (int i = 1; i < 32; ++i) {
+            top = fmaxf(top, x[i]);
+            least = fminf(least, x[i]);
         }
-    }
-    float top = x[0];
-    int valid = 0;
+        ChunkHead head;
+        float bound = INFINITY;
+        const bool list_wanted = !r.greedy && r.filters();
+        if (list_wanted) bound = __shfl_sync(0xffffffffu, warp_sorted(top), p.rank - 1);
 #pragma unroll
-    for (int i = 0; i < 32; ++i) {
-        top = fmaxf(top, x[i]);
-        valid += x[i] > -INFINITY;
-    }
-    const Rule r = rule_of(p, row);
-    ChunkHead head;
-    float bound = INFINITY;
-    if (!r.greedy && r.filters()) bound = __shfl_sync(0xffffffffu, warp_sorted(top), p.rank - 1);
+        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        head.max = top;
+        head.valid = kChunk;
+        if (__any_sync(0xffffffffu, least == -INFINITY)) {
+            int valid = 0;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    head.max = top;
-    head.valid = __reduce_add_sync(0xffffffffu, valid);
-    // the whole row's weight counts where nothing but top_p cuts it
-    double sum = 0.0;
-    if (!r.greedy && !r.by_k && (r.by_p || !r.by_m) && top > -INFINITY) {
-#pragma unroll
-        for (int i = 0; i < 32; ++i) sum += weight_of(x[i], top, r.c, tab);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    }
-    head.weight = sum;
-    // the list
-    int listed = 0;
-    if (!r.greedy && r.filters()) {
-        bound = fmaxf(bound, kLowest);  // -infinity is not listed
-        int count = 0;
-#pragma unroll
-        for (int i = 0; i < 32; ++i) count += x[i] >= bound;
-        if (__reduce_add_sync(0xffffffffu, count) > kSlots) {  // many equal ones: those above
-            bound = bound < INFINITY ? nextafterf(bound, INFINITY) : bound;
-            count = 0;
-#pragma unroll
-            for (int i = 0; i < 32; ++i) count += x[i] >= bound;
-            if (__reduce_add_sync(0xffffffffu, count) > kSlots) bound = __int_as_float(0x7fc00000);  // none: nothing is >= NaN
+            for (int i = 0; i < 32; ++i) valid += x[i] > -INFINITY;
+            head.valid = __reduce_add_sync(0xffffffffu, valid);
         }
-        uint2* list = p.entries + ((long long)row * p.chunks + chunk) * kSlots;
+        // the whole row's weight counts where nothing but top_p cuts it
+        double sum = 0.0;
+        if (!r.greedy && !r.by_k && (r.by_p || !r.by_m) && top > -INFINITY) {
+            const Weigher weight(top, r.c, tab);
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-            const bool in = x[i] >= bound;
-            const uint32_t b = __ballot_sync(0xffffffffu, in);
-            if (in) list[listed + __popc(b & ((1u << lane) - 1))] = make_uint2(__float_as_uint(x[i]), i0 + 4 * (32 * (i / 4) + lane) + i % 4);
-            listed += __popc(b);
+            for (int i = 0; i < 32; ++i) {
+                const double w = weight.bare(x[i]);
+                if (x[i] >= weight.low) sum += w;
+            }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         }
+        head.weight = sum;
+        // the list
+        int listed = 0;
+        if (list_wanted) {
+            bound = fmaxf(bound, kLowest);  // -infinity is not listed
+            auto count = [&] {
+                int c = 0;
+#pragma unroll
+                for (int i = 0; i < 32; ++i) c += x[i] >= bound;
+                return __reduce_add_sync(0xffffffffu, c);
+            };
+            if (count() > kSlots) {  // many equal ones: those above
+                bound = bound < INFINITY ? nextafterf(bound, INFINITY) : bound;
+                if (count() > kSlots) bound = __int_as_float(0x7fc00000);  // none: nothing is >= NaN
+            }
+            uint2* list = p.entries + (long long)task * kSlots;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+                const bool in = x[i] >= bound;
+                const uint32_t b = __ballot_sync(0xffffffffu, in);
+                if (in) list[listed + __popc(b & ((1u << lane) - 1))] = make_uint2(__float_as_uint(x[i]), i0 + 4 * (32 * (i / 4) + lane) + i % 4);
+                listed += __popc(b);
+            }
+        }
+        // fewer finite logits than the bound lets through: all are listed
+        head.bound = listed == head.valid ? -INFINITY : bound;
+        head.listed = bound == bound ? listed : kList + 1;  // no list: more than pick takes
+        if (lane == 0) p.heads[task] = head;
     }
-    // fewer finite logits than the bound lets through: all are listed
-    head.bound = listed == head.valid ? -INFINITY : bound;
-    head.listed = bound == bound ? listed : kList + 1;  // no list: more than pick takes
-    if (lane == 0) p.heads[(long long)row * p.chunks + chunk] = head;
 }
 
 // ---- cuts and token among elements in shared memory ---------------------------------------------------------------------
-// The elements of a row that CTAs of a group hold, and the histogram they share.
+struct Found {
+    uint32_t key;
+    u64 before, at;  // sum of the keys before it, sum of the key itself
+};
+
+// The CTAs that hold a row's elements, and the histogram they share.
 template <int C>
 struct Group {
     uint32_t (*hist)[kBins];  // three words of a bin's sum
     u64* scratch;             // [64]
-    const double* tab;
-    float top;
-    double c;
+    Weigher weight;
     __device__ void sync() const {
         if constexpr (C == 1) __syncthreads();
         else cg::this_cluster().sync();
@@ -265,33 +296,21 @@ struct Group {
         }
         return s;
     }
-};
-
-struct Found {
-    uint32_t key;
-    u64 before, at;  // sum of the keys before it, sum of the key itself
-};
-
-// The first key, ascending from klo to khi, at which the running sum reaches `target` (or exceeds it, with `beyond`);
-// there has to be one.  Elements: visit(f) calls f(key, units) for each of this thread's that takes part.
-template <int C, class Visit>
-__device__ Found first_key(const Group<C>& g, uint32_t klo, uint32_t khi, u64 target, bool beyond, Visit visit) {
-    Found f{klo, 0, 0};
-    int shift = max(0, 32 - __clz(khi - klo) - kBinBits);
-    if (khi == klo) shift = 0;
-    while (true) {
-        for (int i = threadIdx.x; i < 3 * kBins; i += blockDim.x) (&g.hist[0][0])[i] = 0;
+    __device__ __forceinline__ void add(uint32_t b, u64 units) const {
+        atomicAdd(&hist[0][b], (uint32_t)units & 0x7fffu);
+        if (units >> 15) {
+            atomicAdd(&hist[1][b], (uint32_t)(units >> 15) & 0x7fffu);
+            if (units >> 30) atomicAdd(&hist[2][b], (uint32_t)(units >> 30));
+        }
+    }
+    __device__ void clear() const {
+        for (int i = threadIdx.x; i < 3 * kBins; i += blockDim.x) (&hist[0][0])[i] = 0;
         __syncthreads();
-        visit([&](uint32_t key, u64 units) {
-            if (key < klo || key > khi) return;
-            const uint32_t b = (key - klo) >> shift;
-            atomicAdd(&g.hist[0][b], (uint32_t)units & 0x7fffu);
-            if (units >> 15) {
-                atomicAdd(&g.hist[1][b], (uint32_t)(units >> 15) & 0x7fffu);
-                if (units >> 30) atomicAdd(&g.hist[2][b], (uint32_t)(units >> 30));
-            }
-        });
-        g.sync();
+    }
+    // The bin in which the running sum, from f.before on, reaches target (or exceeds it), or the last that is not empty; f.before
+    // and f.at become the sums before it and of it.  Begins and ends with a barrier of the group.
+    __device__ uint32_t reach(Found& f, u64 target, bool beyond) const {
+        sync();
         // two neighbouring bins a thread, their running sums
         constexpr int kPer = kBins / kPickThreads;
         u64 bin[kPer], mine = 0;
@@ -299,8 +318,10 @@ __device__ Found first_key(const Group<C>& g, uint32_t klo, uint32_t khi, u64 ta
         for (int j = 0; j < kPer; ++j) {
             const int b = threadIdx.x * kPer + j;
             bin[j] = 0;
+#pragma unroll
             for (int r = 0; r < C; ++r) {
-                const uint32_t* h = C == 1 ? &g.hist[0][0] : cg::this_cluster().map_shared_rank(&g.hist[0][0], r);
+                const uint32_t* h = &hist[0][0];
+                if constexpr (C > 1) h = cg::this_cluster().map_shared_rank(h, r);
                 bin[j] += (u64)h[b] + ((u64)h[kBins + b] << 15) + ((u64)h[2 * kBins + b] << 30);
             }
             mine += bin[j];
@@ -311,115 +332,145 @@ __device__ Found first_key(const Group<C>& g, uint32_t klo, uint32_t khi, u64 ta
             const u64 v = __shfl_up_sync(0xffffffffu, run, o);
             if ((threadIdx.x & 31) >= o) run += v;
         }
-        if ((threadIdx.x & 31) == 31) g.scratch[threadIdx.x >> 5] = run;
+        if ((threadIdx.x & 31) == 31) scratch[threadIdx.x >> 5] = run;
         __syncthreads();
-        u64 start = f.before + run - mine;
-        for (int w = 0; w < (int)(threadIdx.x >> 5); ++w) start += g.scratch[w];
+        u64 start = f.before + run - mine, end_of_all = f.before;
+        for (int w = 0; w < kPickThreads / 32; ++w) {
+            if (w < (int)(threadIdx.x >> 5)) start += scratch[w];
+            end_of_all += scratch[w];
+        }
+        const u64 goal = beyond ? min(target, end_of_all - 1) : min(target, end_of_all);
 #pragma unroll
         for (int j = 0; j < kPer; ++j) {
             const u64 end = start + bin[j];
-            const bool before_it = beyond ? start <= target : start < target, reached = beyond ? end > target : end >= target;
-            if (before_it && reached && bin[j]) {  // one bin of all
-                g.scratch[16] = threadIdx.x * kPer + j;
-                g.scratch[17] = start;
-                g.scratch[18] = bin[j];
+            if (bin[j] && (beyond ? start <= goal && end > goal : start < goal && end >= goal)) {  // one bin of all
+                scratch[16] = threadIdx.x * kPer + j;
+                scratch[17] = start;
+                scratch[18] = bin[j];
             }
             start = end;
         }
-        g.sync();  // also: everybody has read everybody's histogram
-        const uint32_t b = (uint32_t)g.scratch[16];
-        f.before = g.scratch[17];
-        f.at = g.scratch[18];
+        sync();  // also: everybody has read everybody's histogram
+        f.before = scratch[17];
+        f.at = scratch[18];
+        const uint32_t b = (uint32_t)scratch[16];
+        __syncthreads();
+        return b;
+    }
+};
+
+// The first key, ascending from klo to khi, at which the running sum (of what comes before klo, `before`, on) reaches
+// `target` (or exceeds it, with `beyond`); the last key if none does.  Elements: visit(f) calls f(key, units) for each of this
+// thread's that takes part, units being a function.
+template <int C, class Visit>
+__device__ Found first_key(const Group<C>& g, uint32_t klo, uint32_t khi, u64 target, bool beyond, Visit visit, u64 before = 0) {
+    Found f{klo, before, 0};
+    int shift = max(0, 32 - __clz(khi - klo) - kBinBits);
+    if (khi == klo) shift = 0;
+    while (true) {
+        for (int i = threadIdx.x; i < 3 * kBins; i += blockDim.x) (&g.hist[0][0])[i] = 0;
+        __syncthreads();
+        visit([&](uint32_t key, auto units) {
+            if (key >= klo && key <= khi) g.add((key - klo) >> shift, units());
+        });
+        const uint32_t b = g.reach(f, target, beyond);
         klo += b << shift;
         khi = min(khi, klo + ((1u << shift) - 1));
         f.key = klo;
-        __syncthreads();
         if (shift == 0) return f;
         shift = max(0, shift - kBinBits);
     }
 }
 
-// Cuts and token of a row whose elements the group holds: each(f) calls f(logit, index) for this thread's.  whole_weight: of
-// all tokens (used where top_p is the first cut).  bound: elements below it may be missing.  False: they are needed.
+// Smallest of a value that every thread of the group has; slot as for Group::total.
+template <int C>
+__device__ uint32_t group_min(const Group<C>& g, uint32_t v, int slot) {
+    v = __reduce_min_sync(0xffffffffu, v);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) g.scratch[threadIdx.x >> 5] = v;
+    __syncthreads();
+    for (int w = 0; w < (int)blockDim.x / 32; ++w) v = min(v, (uint32_t)g.scratch[w]);
+    if constexpr (C > 1) {
+        if (threadIdx.x == 0) g.scratch[32 + slot] = v;
+        g.sync();
+        for (int r = 0; r < C; ++r) v = min(v, (uint32_t)*cg::this_cluster().map_shared_rank(g.scratch + 32 + slot, r));
+    }
+    return v;
+}
+
+struct Cut {  // the last kept token: its key, and its index among equals
+    uint32_t key, index;
+    __device__ __forceinline__ bool keeps(uint32_t k, uint32_t i) const { return k < key || (k == key && i <= index); }
+};
+
+// top_k's and top_p's cut of a row whose elements the group holds: each(f) calls f(logit, index) for this thread's, `have` are
+// listed in all.  whole: the weight of all tokens.  Elements below `bound` may be missing; false: they are needed.
 template <int C, class Each>
-__device__ bool draw_row(const Group<C>& g, const Params& p, int row, const Rule& r, u64 whole_weight, float bound, float lowest, Each each) {
-    uint32_t cut_key = 0xffffffffu, cut_index = 0xffffffffu;  // the last kept one
-    auto kept = [&](float x, uint32_t i) {
-        const uint32_t k = order_key(x);
-        return k < cut_key || (k == cut_key && i <= cut_index);
-    };
-    auto units = [&](float x) { return to_units(weight_of(x, g.top, g.c, g.tab)); };
+__device__ bool find_cut(const Group<C>& g, const Params& p, const Rule& r, u64 have, u64 whole, float bound, float lowest, Each each, Cut& cut) {
+    cut = {0xffffffffu, 0xffffffffu};
+    auto one = [] { return 1ull; };
     // the last of `n` among the equal ones at a key
     auto cut_ties = [&](uint32_t key, u64 n) {
         return first_key<C>(g, 0, p.vocab - 1, n, false, [&](auto f) {
-            each([&](float x, uint32_t i) { if (order_key(x) == key && kept(x, i)) f(i, 1); });
+            each([&](float x, uint32_t i) { if (order_key(x) == key && cut.keeps(key, i)) f(i, one); });
         }).key;
     };
-    const uint32_t first = order_key(g.top), last = order_key(lowest);
+    const uint32_t first = order_key(g.weight.top), last = order_key(lowest);
     if (r.by_k) {
-        const u64 have = g.total([&] { u64 n = 0; each([&](float, uint32_t) { ++n; }); return n; }(), 0);
         if (have > (u64)r.k) {
-            const Found f = first_key<C>(g, first, last, r.k, false, [&](auto f) { each([&](float x, uint32_t) { f(order_key(x), 1); }); });
+            const Found f = first_key<C>(g, first, last, r.k, false, [&](auto f) { each([&](float x, uint32_t) { f(order_key(x), one); }); });
             if (!(key_logit(f.key) >= bound)) return false;
             const u64 n = r.k - f.before;
-            const uint32_t ci = n < f.at ? cut_ties(f.key, n) : 0xffffffffu;
-            cut_key = f.key;
-            cut_index = ci;
+            const uint32_t index = n < f.at ? cut_ties(f.key, n) : 0xffffffffu;
+            cut = {f.key, index};
         } else if (bound > -INFINITY) {
             return false;
         }
     }
     if (r.by_p) {
-        u64 mass = whole_weight;
-        if (r.by_k || whole_weight == 0)
-            mass = g.total([&] { u64 s = 0; each([&](float x, uint32_t i) { if (kept(x, i)) s += units(x); }); return s; }(), 1);
+        u64 mass = whole;
+        if (r.by_k) mass = g.total([&] { u64 s = 0; each([&](float x, uint32_t i) { if (cut.keeps(order_key(x), i)) s += to_units(g.weight(x)); }); return s; }(), 1);
         const u64 target = min(max((u64)ceil(r.p * (double)mass), 1ull), mass);
-        bool all = false;
-        if (!r.by_k && bound > -INFINITY) {  // does the list reach that far?
-            const u64 have = g.total([&] { u64 s = 0; each([&](float x, uint32_t) { s += units(x); }); return s; }(), 2);
-            if (have < target) return false;
-        } else if (!r.by_k) {
-            // rounding of the parts may leave the sum a few units short of `mass`
-            const u64 have = g.total([&] { u64 s = 0; each([&](float x, uint32_t) { s += units(x); }); return s; }(), 2);
-            all = have < target;
-        }
-        if (!all) {
-            const Found f = first_key<C>(g, first, last, target, false, [&](auto f) {
-                each([&](float x, uint32_t i) { if (kept(x, i)) f(order_key(x), units(x)); });
+        Found f{first, 0, 0};
+        const float top = g.weight.top, range = top - fmaxf(g.weight.low, lowest), per = (float)kBins / range;
+        if (C > 1 && range > 0.f && range < INFINITY && per < INFINITY) {
+            // first by distance from the largest: a row's bulk spreads over these bins, where keys' leading bits would not part it
+            auto bin = [&](float x) { return min((uint32_t)((top - x) * per), (uint32_t)kBins - 1); };
+            g.clear();
+            each([&](float x, uint32_t i) { if (x >= g.weight.low && cut.keeps(order_key(x), i)) g.add(bin(x), to_units(g.weight(x))); });
+            const uint32_t b = g.reach(f, target, false);
+            uint32_t lo = 0xffffffffu, hi = 0;
+            each([&](float x, uint32_t i) {
+                const uint32_t k = order_key(x);
+                if (x >= g.weight.low && bin(x) == b && cut.keeps(k, i)) { lo = min(lo, k); hi = max(hi, k); }
             });
-            if (!(key_logit(f.key) >= bound)) return false;
-            const u64 one = units(key_logit(f.key)), n = one ? (target - f.before + one - 1) / one : 1, ties = one ? f.at / one : 1;
-            const uint32_t ci = n < ties ? cut_ties(f.key, n) : f.key == cut_key ? cut_index : 0xffffffffu;
-            cut_key = f.key;
-            cut_index = ci;
+            lo = group_min(g, lo, 2);
+            hi = ~group_min(g, ~hi, 3);
+            f = first_key<C>(g, lo, hi, target, false, [&](auto f) {
+                each([&](float x, uint32_t i) { if (cut.keeps(order_key(x), i)) f(order_key(x), [&] { return to_units(g.weight(x)); }); });
+            }, f.before);
+        } else {
+            f = first_key<C>(g, first, last, target, false, [&](auto f) {
+                each([&](float x, uint32_t i) { if (cut.keeps(order_key(x), i)) f(order_key(x), [&] { return to_units(g.weight(x)); }); });
+            });
         }
+        if (f.before + f.at < target) {          // not reached:
+            if (!r.by_k && bound > -INFINITY) return false;  // among those listed,
+            if (!r.by_k) return true;                        // or by the few units that the parts' sums were rounded by
+        }
+        if (!(key_logit(f.key) >= bound)) return false;
+        const u64 each_one = to_units(g.weight(key_logit(f.key))), n = (target - f.before + each_one - 1) / each_one;
+        const uint32_t index = n < f.at / each_one ? cut_ties(f.key, n) : f.key == cut.key ? cut.index : 0xffffffffu;
+        cut = {f.key, index};
     }
-    if (r.by_m && !r.by_k && !r.by_p && bound > -INFINITY && !(weight_of(bound, g.top, g.c, g.tab) < r.m)) return false;
-    auto drawn = [&](float x, uint32_t i) { return kept(x, i) && (!r.by_m || weight_of(x, g.top, g.c, g.tab) >= r.m); };
-    u64 s = 0, n = 0;
-    each([&](float x, uint32_t i) { if (drawn(x, i)) { s += units(x); ++n; } });
-    s = g.total(s, 3);
-    n = g.total(n, 4);
-    const u64 target = min((u64)((double)r.u * (double)s), s - 1);
-    const Found f = first_key<C>(g, 0, p.vocab - 1, target, true, [&](auto f) {
-        each([&](float x, uint32_t i) { if (drawn(x, i)) f(i, units(x)); });
-    });
-    if (threadIdx.x == 0 && (C == 1 || cg::this_cluster().block_rank() == 0)) {
-        p.tokens[row] = (int)f.key;
-        if (p.probs) p.probs[row] = (float)((double)f.at / (double)s);
-        if (p.kept) p.kept[row] = (int)n;
-    }
-    return true;
+    return !(r.by_m && !r.by_k && !r.by_p && bound > -INFINITY && g.weight(bound) >= r.m);
 }
 
-// ---- pick ---------------------------------------------------------------------------------------------------------------
-struct PickSmem {
-    uint32_t hist[3][kBins];
-    u64 scratch[64];
-    double tab[128];
-    float x[kList];
-    uint32_t index[kList];
-};
+__device__ __forceinline__ void answer(const Params& p, int row, int token, float prob, int kept) {
+    p.tokens[row] = token;
+    if (p.probs) p.probs[row] = prob;
+    if (p.kept) p.kept[row] = kept;
+}
 
 // Sum over the CTA's threads before this one, and all of it in `all`.
 __device__ __forceinline__ u64 prefix(u64 v, u64* scratch, u64& all) {
@@ -442,20 +493,128 @@ __device__ __forceinline__ u64 prefix(u64 v, u64* scratch, u64& all) {
     return before + run - v;
 }
 
+// One value a thread, smallest first, of which those of threads >= n are the largest there are.
+template <class T>
+__device__ __forceinline__ T sorted(T v, int n, T* shared) {
+    const int tid = threadIdx.x;
+    for (int k = 2; k < 2 * n || k <= 32; k <<= 1)
+        for (int j = k >> 1; j > 0; j >>= 1) {
+            T o;
+            if (j >= 32) {
+                __syncthreads();
+                shared[tid] = v;
+                __syncthreads();
+                o = shared[tid ^ j];
+            } else {
+                o = __shfl_xor_sync(0xffffffffu, v, j);
+            }
+            v = ((tid & k) == 0) == ((tid & j) == 0) ? min(v, o) : max(v, o);
+        }
+    __syncthreads();
+    return v;
+}
+
+// ---- pick ---------------------------------------------------------------------------------------------------------------
+struct PickSmem {
+    uint32_t hist[3][kBins];
+    u64 scratch[64];
+    double tab[kTable];
+    float x[kList];
+    uint32_t index[kList];
+};
+enum Outcome { kDone, kTooMany, kNeedsMore };
+
+// A row of which one histogram's bins leave at most 512 elements to look at.
+__device__ Outcome pick_few(const Group<1>& g, PickSmem& s, const Params& p, int row, const Rule& r, int have, u64 whole, float bound, float lowest) {
+    const int tid = threadIdx.x, lane = tid & 31;
+    const uint32_t first = order_key(g.weight.top), last = order_key(lowest);
+    uint32_t keep_to = last;  // key of the last element that may matter
+    if (r.by_k ? have > r.k : r.by_p) {
+        const int shift = max(0, 32 - __clz(last - first) - kBinBits);
+        const u64 target = r.by_k ? (u64)r.k : min(max((u64)ceil(r.p * (double)whole), 1ull), whole);
+        g.clear();
+        for (int i = tid; i < have; i += kPickThreads)
+            if (s.x[i] > -INFINITY) {
+                const uint32_t b = (order_key(s.x[i]) - first) >> shift;
+                if (r.by_k) atomicAdd(&g.hist[0][b], 1u);
+                else g.add(b, to_units(g.weight(s.x[i])));
+            }
+        Found f{first, 0, 0};
+        const uint32_t b = g.reach(f, target, false);
+        if (f.before + f.at < target) {
+            if (bound > -INFINITY) return kNeedsMore;
+        } else {
+            keep_to = min(last, first + (b << shift) + ((1u << shift) - 1));
+        }
+    } else if (r.by_k && bound > -INFINITY) {
+        return kNeedsMore;
+    }
+    const bool by_m_alone = r.by_m && !r.by_k && !r.by_p;
+    if (by_m_alone && bound > -INFINITY && g.weight(bound) >= r.m) return kNeedsMore;
+    // what is left, side by side in the histogram's place
+    u64* list = reinterpret_cast<u64*>(&g.hist[0][0]);
+    int* count = reinterpret_cast<int*>(g.scratch + 48);
+    __syncthreads();
+    if (tid == 0) *count = 0;
+    __syncthreads();
+    for (int i0 = 0; i0 < have; i0 += kPickThreads) {
+        const int i = i0 + tid;
+        const float x = i < have ? s.x[i] : -INFINITY;
+        const bool take = x > -INFINITY && order_key(x) <= keep_to && (!by_m_alone || g.weight(x) >= r.m);
+        const uint32_t b = __ballot_sync(0xffffffffu, take);
+        int at = 0;
+        if (lane == 0 && b) at = atomicAdd(count, __popc(b));
+        at = __shfl_sync(0xffffffffu, at, 0) + __popc(b & ((1u << lane) - 1));
+        if (take && at < kPickThreads) list[at] = (u64)order_key(x) << 32 | s.index[i];
+    }
+    __syncthreads();
+    const int n = *count;
+    if (n > kPickThreads) return kTooMany;
+    u64 v = tid < n ? list[tid] : ~0ull;
+    v = sorted(v, n, list);
+    // thread i has the row's i-th token
+    u64 *sums = list + kPickThreads, *weights = sums + kPickThreads, all;
+    const float x = key_logit((uint32_t)(v >> 32));
+    const double w = tid < n ? g.weight(x) : 0.0;
+    const u64 units = tid < n ? to_units(w) : 0;
+    const u64 before = prefix(units, g.scratch, all);
+    list[tid] = v;
+    sums[tid] = before + units;
+    weights[tid] = units;
+    __syncthreads();
+    auto enough = [&](int rank) { return key_logit((uint32_t)(list[rank] >> 32)) >= bound; };
+    int kept = n;
+    if (r.by_k && n > r.k) kept = r.k;
+    if (r.by_k && bound > -INFINITY && !enough(kept - 1)) return kNeedsMore;
+    if (r.by_p) {
+        const u64 mass = r.by_k ? sums[kept - 1] : whole, target = min(max((u64)ceil(r.p * (double)mass), 1ull), mass);
+        kept = __syncthreads_count(tid < kept && before < target);
+        if (bound > -INFINITY && !enough(kept - 1)) return kNeedsMore;
+    }
+    if (r.by_m) kept = __syncthreads_count(tid < kept && w >= r.m);
+    const u64 sum = sums[kept - 1], goal = min((u64)((double)r.u * (double)sum), sum - 1);
+    // the kept ones by index
+    uint32_t c = tid < kept ? (uint32_t)v << 9 | tid : 0xffffffffu;
+    static_assert(kPickThreads == 512 && NEON_SAMPLER_MAX_VOCAB <= 1 << 23, "index and rank share a word");
+    c = sorted(c, kept, reinterpret_cast<uint32_t*>(list));
+    const u64 mine = tid < kept ? weights[c & 511] : 0, at = prefix(mine, g.scratch, all);
+    if (at <= goal && at + mine > goal) answer(p, row, (int)(c >> 9), (float)((double)mine / (double)sum), kept);
+    return kDone;
+}
+
 // `direct`: the vocabulary fits the list and there was no scan.
 __global__ void __launch_bounds__(kPickThreads) pick_kernel(const Params p, int direct) {
     extern __shared__ __align__(16) unsigned char raw[];
     PickSmem& s = *reinterpret_cast<PickSmem*>(raw);
     const int row = blockIdx.x, tid = threadIdx.x;
+    fill_table(s.tab);
     pdl_wait();
     pdl_launch_dependents();
-    fill_table(s.tab);
     const Rule r = rule_of(p, row);
     const ChunkHead* heads = p.heads + (long long)row * p.chunks;
     const long long base = row * p.stride;
     static_assert(NEON_SAMPLER_MAX_VOCAB <= kChunk * kPickThreads, "a thread takes a head");
     static_assert(NEON_SAMPLER_MAX_VOCAB / kChunk <= kBins, "the histogram holds the chunks' list lengths");
-    if (tid == 0 && p.left) p.left[row] = 0;
     // the largest logit, the highest of the bounds, and a bound of all that is listed
     float top = -INFINITY, bound = -INFINITY, low = INFINITY;
     ChunkHead mine{-INFINITY, -INFINITY, 0, 0, 0.0};
@@ -465,6 +624,7 @@ __global__ void __launch_bounds__(kPickThreads) pick_kernel(const Params p, int 
             s.index[i] = i;
             top = fmaxf(top, s.x[i]);
         }
+        low = kLowest;
     } else if (tid < p.chunks) {
         mine = heads[tid];
         top = mine.max;
@@ -482,33 +642,16 @@ __global__ void __launch_bounds__(kPickThreads) pick_kernel(const Params p, int 
     __syncthreads();
     for (int w = 0; w < kPickThreads / 32; ++w) { top = fmaxf(top, fs[w]); bound = fmaxf(bound, fs[32 + w]); low = fminf(low, fs[64 + w]); }
     __syncthreads();
-    auto answer = [&](int token, float prob, int kept) {
-        p.tokens[row] = token;
-        if (p.probs) p.probs[row] = prob;
-        if (p.kept) p.kept[row] = kept;
-    };
+    if (tid == 0 && p.left) p.left[row] = 0;
     if (top == -INFINITY) {
-        if (tid == 0) answer(-1, 0.f, 0);
+        if (tid == 0) answer(p, row, -1, 0.f, 0);
         return;
     }
-    Group<1> g{s.hist, s.scratch, s.tab, top, r.c};
-    if (direct) {
-        auto each = [&](auto f) {
-            for (int i = tid; i < p.vocab; i += kPickThreads)
-                if (s.x[i] > -INFINITY) f(s.x[i], s.index[i]);
-        };
-        if (r.greedy) {
-            const Found f = first_key<1>(g, 0, p.vocab - 1, 0, true, [&](auto f) { each([&](float x, uint32_t i) { if (x == top) f(i, 1); }); });
-            if (tid == 0) answer((int)f.key, 1.f, 1);
-            return;
-        }
-        draw_row<1>(g, p, row, r, 0, -INFINITY, kLowest, each);
-        return;
-    }
-    if (r.greedy || !r.filters()) {
+    const Weigher weight(top, r.c, s.tab);
+    if (!direct && (r.greedy || !r.filters())) {
         // weights of the chunks, in order; greedily: the first chunk that has the maximum
         u64 w = r.greedy ? (u64)(mine.max == top) : 0ull, all;
-        if (!r.greedy && mine.max > -INFINITY) w = (u64)(mine.weight * weight_of(mine.max, top, r.c, s.tab) * kUnit);
+        if (!r.greedy && mine.max > -INFINITY) w = (u64)(mine.weight * weight(mine.max) * kUnit);
         const u64 run = prefix(w, s.scratch, all);
         const u64 target = r.greedy ? 0 : min((u64)((double)r.u * (double)all), all - 1);
         if (run <= target && run + w > target) {
@@ -517,55 +660,94 @@ __global__ void __launch_bounds__(kPickThreads) pick_kernel(const Params p, int 
         }
         u64 n_valid;
         prefix(mine.valid, s.scratch, n_valid);
-        const int chunk = (int)s.scratch[40], i0 = chunk * kChunk;
+        const int i0 = (int)s.scratch[40] * kChunk;
         const u64 rest = s.scratch[41];
         // the token in it: two neighbouring elements a thread
         constexpr int kEach = kChunk / kPickThreads;
-        float x[kEach];
         u64 e[kEach], part = 0, have;
 #pragma unroll
         for (int j = 0; j < kEach; ++j) {
             const int i = i0 + tid * kEach + j;
-            x[j] = i < p.vocab ? load1(p, base + i) : -INFINITY;
-            e[j] = r.greedy ? (u64)(x[j] == top) : x[j] > -INFINITY ? to_units(weight_of(x[j], top, r.c, s.tab)) : 0;
+            const float x = i < p.vocab ? load1(p, base + i) : -INFINITY;
+            e[j] = r.greedy ? (u64)(x == top) : to_units(weight(x));
             part += e[j];
         }
         u64 at = prefix(part, s.scratch, have);
         const u64 goal = min(rest, have ? have - 1 : 0);  // the chunk's sum may differ from its elements' by their rounding
 #pragma unroll
         for (int j = 0; j < kEach; ++j) {
-            if (at <= goal && at + e[j] > goal) answer(i0 + tid * kEach + j, r.greedy ? 1.f : (float)((double)e[j] / (double)all), r.greedy ? 1 : (int)n_valid);
+            if (at <= goal && at + e[j] > goal)
+                answer(p, row, i0 + tid * kEach + j, r.greedy ? 1.f : (float)((double)e[j] / (double)all), r.greedy ? 1 : (int)n_valid);
             at += e[j];
         }
         return;
     }
-    // the listed elements, side by side
-    u64 n64, whole_all;
-    const uint32_t at = (uint32_t)prefix(mine.listed, s.scratch, n64);
-    prefix(mine.max > -INFINITY ? (u64)(mine.weight * weight_of(mine.max, top, r.c, s.tab) * kUnit) : 0ull, s.scratch, whole_all);
-    const int n = (int)n64;
-    bool fits = n <= kList;
-    if (fits) {
-        uint32_t* starts = &s.hist[0][0];  // where each chunk's entries go, and how many they are
-        if (tid < p.chunks) {
-            starts[tid] = at;
-            starts[kBins + tid] = (uint32_t)mine.listed;
+    const Group<1> g{s.hist, s.scratch, weight};
+    auto one = [] { return 1ull; };
+    if (r.greedy) {
+        const Found f = first_key<1>(g, 0, p.vocab - 1, 0, true, [&](auto f) {
+            for (int i = tid; i < p.vocab; i += kPickThreads) if (s.x[i] == top) f((uint32_t)i, one);
+        });
+        if (tid == 0) answer(p, row, (int)f.key, 1.f, 1);
+        return;
+    }
+    u64 n64 = p.vocab, whole = 0;
+    bool fits = true;
+    if (direct) {
+        if (r.by_p && !r.by_k) {
+            u64 sum = 0;
+            for (int i = tid; i < p.vocab; i += kPickThreads) sum += to_units(weight(s.x[i]));
+            whole = g.total(sum, 0);
         }
-        __syncthreads();
-        const uint2* lists = p.entries + (long long)row * p.chunks * kSlots;
-        for (int i = tid; i < p.chunks * kSlots; i += kPickThreads) {
-            const int c = i / kSlots, e = i % kSlots;
-            if (e < (int)starts[kBins + c]) {
-                const uint2 v = lists[i];
-                s.x[starts[c] + e] = __uint_as_float(v.x);
-                s.index[starts[c] + e] = v.y;
+    } else {
+        // the listed elements, side by side
+        const uint32_t at = (uint32_t)prefix(mine.listed, s.scratch, n64);
+        prefix(mine.max > -INFINITY ? (u64)(mine.weight * weight(mine.max) * kUnit) : 0ull, s.scratch, whole);
+        fits = n64 > 0 && n64 <= kList;
+        if (fits) {
+            uint32_t* starts = &s.hist[0][0];  // where each chunk's entries go, and how many they are
+            if (tid < p.chunks) {
+                starts[tid] = at;
+                starts[kBins + tid] = (uint32_t)mine.listed;
+            }
+            __syncthreads();
+            const uint2* lists = p.entries + (long long)row * p.chunks * kSlots;
+            for (int i = tid; i < p.chunks * kSlots; i += kPickThreads) {
+                const int c = i / kSlots, e = i % kSlots;
+                if (e < (int)starts[kBins + c]) {
+                    const uint2 v = lists[i];
+                    s.x[starts[c] + e] = __uint_as_float(v.x);
+                    s.index[starts[c] + e] = v.y;
+                }
+            }
+            __syncthreads();
+        }
+    }
+    if (fits) {
+        const int n = (int)n64;
+        Outcome outcome = r.filters() ? pick_few(g, s, p, row, r, n, whole, bound, low) : kTooMany;
+        if (outcome == kTooMany) {
+            auto each = [&](auto f) {
+                for (int i = tid; i < n; i += kPickThreads)
+                    if (s.x[i] > -INFINITY) f(s.x[i], s.index[i]);
+            };
+            Cut cut;
+            const u64 have = direct && r.by_k ? g.total([&] { u64 c = 0; each([&](float, uint32_t) { ++c; }); return c; }(), 1) : n64;
+            outcome = find_cut<1>(g, p, r, have, whole, bound, low, each, cut) ? kDone : kNeedsMore;
+            if (outcome == kDone) {
+                auto drawn = [&](float x, uint32_t i) { return cut.keeps(order_key(x), i) && (!r.by_m || weight(x) >= r.m); };
+                u64 sum = 0, count = 0;
+                each([&](float x, uint32_t i) { if (drawn(x, i)) { sum += to_units(weight(x)); ++count; } });
+                sum = g.total(sum, 3);
+                count = g.total(count, 4);
+                const u64 goal = min((u64)((double)r.u * (double)sum), sum - 1);
+                const Found f = first_key<1>(g, 0, p.vocab - 1, goal, true, [&](auto f) {
+                    each([&](float x, uint32_t i) { if (drawn(x, i)) f(i, [&] { return to_units(weight(x)); }); });
+                });
+                if (tid == 0) answer(p, row, (int)f.key, (float)((double)f.at / (double)sum), (int)count);
             }
         }
-        __syncthreads();
-        auto each = [&](auto f) {
-            for (int i = tid; i < n; i += kPickThreads) f(s.x[i], s.index[i]);
-        };
-        fits = n > 0 && draw_row<1>(g, p, row, r, whole_all, bound, low, each);
+        fits = outcome == kDone;
     }
     if (!fits && tid == 0) p.left[row] = 1;
 }
@@ -574,42 +756,108 @@ __global__ void __launch_bounds__(kPickThreads) pick_kernel(const Params p, int 
 struct WholeSmem {
     uint32_t hist[3][kBins];
     u64 scratch[64];
-    double tab[128];
+    u64 parts[2][kPickThreads / 32];  // weights and counts of the warps' stretches
+    double tab[kTable];
 };
 
-// Rows that pick left, one after the other on each cluster.  A CTA keeps its share of the row in shared memory.
+// Rows that pick left, one after the other on each cluster.  A CTA keeps its share of the row in shared memory, a warp's
+// stretch of it is contiguous.
 __global__ void __cluster_dims__(kClusterCtas, 1, 1) __launch_bounds__(kPickThreads) whole_kernel(const Params p) {
     extern __shared__ __align__(16) unsigned char raw[];
     WholeSmem& s = *reinterpret_cast<WholeSmem*>(raw);
     float* xs = reinterpret_cast<float*>(raw + sizeof(WholeSmem));
-    const int rank = (int)cg::this_cluster().block_rank(), tid = threadIdx.x;
+    constexpr int kWarps = kPickThreads / 32;
+    const cg::cluster_group cluster = cg::this_cluster();
+    const int rank = (int)cluster.block_rank(), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int share = (p.vocab + kClusterCtas - 1) / kClusterCtas, i0 = min(rank * share, p.vocab), n = min(share, p.vocab - i0);
-    pdl_wait();
+    const int stretch = (share + kWarps - 1) / kWarps, w0 = min(warp * stretch, n), w1 = min(w0 + stretch, n);
     fill_table(s.tab);
+    pdl_wait();
     for (int row = blockIdx.x / kClusterCtas; row < p.batch; row += gridDim.x / kClusterCtas) {
         if (!p.left[row]) continue;  // the same for the whole cluster
         const Rule r = rule_of(p, row);
         const ChunkHead* heads = p.heads + (long long)row * p.chunks;
         __syncthreads();
         float top = -INFINITY;
+#pragma unroll 8
         for (int i = tid; i < n; i += kPickThreads) xs[i] = load1(p, row * p.stride + i0 + i);
-        for (int c = tid; c < p.chunks; c += kPickThreads) top = fmaxf(top, heads[c].max);
+        ChunkHead mine{-INFINITY, -INFINITY, 0, 0, 0.0};
+        if (tid < p.chunks) mine = heads[tid];
+        top = mine.max;
         float* fs = reinterpret_cast<float*>(s.scratch);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        if ((tid & 31) == 0) fs[tid >> 5] = top;
+        if (lane == 0) fs[warp] = top;
         __syncthreads();
-        for (int w = 0; w < kPickThreads / 32; ++w) top = fmaxf(top, fs[w]);
+        for (int w = 0; w < kWarps; ++w) top = fmaxf(top, fs[w]);
         __syncthreads();
-        Group<kClusterCtas> g{s.hist, s.scratch, s.tab, top, r.c};
+        const Weigher weight(top, r.c, s.tab);
+        const Group<kClusterCtas> g{s.hist, s.scratch, weight};
+        u64 whole, have;
+        prefix(mine.max > -INFINITY ? (u64)(mine.weight * weight(mine.max) * kUnit) : 0ull, s.scratch, whole);
+        prefix(mine.valid, s.scratch, have);
         auto each = [&](auto f) {
             for (int i = tid; i < n; i += kPickThreads)
                 if (xs[i] > -INFINITY) f(xs[i], (uint32_t)(i0 + i));
         };
-        draw_row<kClusterCtas>(g, p, row, r, 0, -INFINITY, kLowest, each);
-        g.sync();
+        Cut cut;
+        find_cut<kClusterCtas>(g, p, r, have, whole, -INFINITY, kLowest, each, cut);
+        // by index: the warps' stretches, then the token in one of them
+        auto units = [&](int i) -> u64 {
+            const float x = xs[i];
+            if (!(x > -INFINITY) || !cut.keeps(order_key(x), i0 + i)) return 0;
+            const double w = weight(x);
+            return !r.by_m || w >= r.m ? to_units(w) : 0;
+        };
+        u64 sum = 0, count = 0;
+        for (int i = w0 + lane; i < w1; i += 32) {
+            const float x = xs[i];
+            if (!(x > -INFINITY) || !cut.keeps(order_key(x), i0 + i)) continue;
+            const double w = weight(x);
+            if (r.by_m && !(w >= r.m)) continue;
+            sum += to_units(w);
+            ++count;
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            count += __shfl_xor_sync(0xffffffffu, count, o);
+        }
+        if (lane == 0) { s.parts[0][warp] = sum; s.parts[1][warp] = count; }
+        cluster.sync();
+        u64 part = 0, number = 0, all, kept;
+        if (tid < kClusterCtas * kWarps) {
+            const u64* theirs = cluster.map_shared_rank(&s.parts[0][0], tid / kWarps);
+            part = theirs[tid % kWarps];
+            number = theirs[kWarps + tid % kWarps];
+        }
+        const u64 before = prefix(part, s.scratch, all);
+        const u64 goal = min((u64)((double)r.u * (double)all), all - 1);
+        if (before <= goal && before + part > goal) {
+            s.scratch[40] = tid;
+            s.scratch[41] = goal - before;
+        }
+        prefix(number, s.scratch, kept);
+        if ((int)s.scratch[40] == rank * kWarps + warp) {
+            u64 run = 0;
+            const u64 rest = s.scratch[41];
+            for (int i = w0; i < w1; i += 32) {
+                const u64 mine_units = i + lane < w1 ? units(i + lane) : 0;
+                u64 upto = mine_units;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const u64 v = __shfl_up_sync(0xffffffffu, upto, o);
+                    if (lane >= o) upto += v;
+                }
+                upto += run;
+                if (upto > rest && upto - mine_units <= rest) answer(p, row, i0 + i + lane, (float)((double)mine_units / (double)all), (int)kept);
+                run = __shfl_sync(0xffffffffu, upto, 31);
+                if (run > rest) break;
+            }
+        }
+        cluster.sync();  // the stretches' sums are read
     }
-    cg::this_cluster().sync();  // nobody leaves while others read its shared memory
+    cluster.sync();  // nobody leaves while others read its shared memory
 }
 
 }  // namespace sampler
