@@ -50,7 +50,7 @@ namespace sampler {
 namespace {
 constexpr int kSms = 148, kSharedPerSm = 227 * 1024;
 int chunks_of(int vocab) { return vocab <= kList ? 0 : (vocab + kChunk - 1) / kChunk; }
-size_t whole_smem(int vocab) { return sizeof(WholeSmem) + (size_t)((vocab + kClusterCtas - 1) / kClusterCtas) * sizeof(float); }
+size_t whole_smem(int vocab) { return sizeof(WholeSmem) + (size_t)whole_share(vocab) * sizeof(float); }
 size_t round16(size_t n) { return (n + 15) / 16 * 16; }
 }  // namespace
 

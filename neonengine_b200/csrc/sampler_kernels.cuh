@@ -8,9 +8,9 @@
 //   whole    a cluster per row that keeps the row in its shared memory and finds cuts and token among all of it.
 // Vocabularies that fit pick's list go to pick alone.
 //
-// One histogram over the list cuts it down to what the first filter can keep.  Up to 512 elements are then sorted, one a
-// thread, and every cut is a running sum away; more are cut by histograms over ten bits of the key at a time, the key being
-// the logit in descending order (or the index).
+// One histogram over the list cuts it down to what the first filter can keep.  With up to 512 elements every thread then has
+// one, and finds its rank and the weight ahead of it by looking at the others; more are cut by histograms over ten bits of the
+// key at a time, the key being the logit in descending order (or the index).
 // Weights are integers of 2^-43 of the largest, so that sums depend on no order; a histogram keeps them as three words
 // of 15 bits each per element, which shared memory can add atomically.
 #pragma once
@@ -117,17 +117,17 @@ struct Weigher {
         c = 64.0 * log2_scale;
         off = -c * (double)top;
         low = fmaxf((float)((double)top - 60.0 / log2_scale), kLowest);
-        if (top == INFINITY) { low = INFINITY; c = 0.0; off = 0.0; }  // infinities alone, at weight 1
+        if (top == INFINITY) low = INFINITY;  // infinities alone, at weight 1
     }
-    // of an x >= low (of another: any number)
+    // of an x >= low, where top is finite (of another: any number)
     __device__ __forceinline__ double bare(float x) const {
         const double kMagic = 6755399441055744.0;  // 1.5 * 2^52: the sum's low word is the rounded integer
         const double kA = 0.010830424696249145, kB = 5.8649049505537566e-05, kC = 2.1173136998904953e-07;  // A = ln 2 / 64, A^2 / 2, A^3 / 6
-        const double t = top == INFINITY ? 0.0 : fma((double)x, c, off), kd = t + kMagic;
+        const double t = fma((double)x, c, off), kd = t + kMagic;
         const int k = __double2loint(kd);
         const double r = t - (kd - kMagic), v = tab[(k & 63) * 32];
         const double w = fma(v, r * fma(r, fma(r, kC, kB), kA), v);
-        return __hiloint2double(__double2hiint(w) + ((k >> 6) << 20), __double2loint(w));
+        return __hiloint2double(__double2hiint(w) + (k & ~63) * (1 << 14), __double2loint(w));
     }
     __device__ __forceinline__ double operator()(float x) const { return x == top ? 1.0 : x >= low ? bare(x) : 0.0; }  // exactly 1 for the largest
 };
@@ -159,13 +159,13 @@ __global__ void __launch_bounds__(kScanWarps * 32, 2) scan_kernel(const Params p
     __syncthreads();
     pdl_wait();
     pdl_launch_dependents();
-    const int tasks = p.batch * p.chunks;
-    for (int task = blockIdx.x * kScanWarps + threadIdx.x / 32; task < tasks; task += gridDim.x * kScanWarps) {
-        const int row = task / p.chunks, chunk = task - row * p.chunks;
-        const int i0 = chunk * kChunk, n = min(kChunk, p.vocab - i0);
+    const int tasks = p.batch * p.chunks, step = gridDim.x * kScanWarps;
+    constexpr int kSize = DT == 0 ? 4 : 2;
+    // element 4 * (32 v + lane) + c of a chunk is x[4 v + c]
+    auto fetch = [&](float (&x)[32], int task) {
+        if (task >= tasks) return;
+        const int row = task / p.chunks, i0 = (task - row * p.chunks) * kChunk, n = min(kChunk, p.vocab - i0);
         const long long base = row * p.stride + i0;
-        float x[32];  // element 4 * (32 v + lane) + c is x[4 v + c]
-        constexpr int kSize = DT == 0 ? 4 : 2;
         if (n == kChunk && ((reinterpret_cast<uintptr_t>(p.logits) + base * kSize) & (4 * kSize - 1)) == 0) {
 #pragma unroll
             for (int v = 0; v < 8; ++v) {
@@ -189,8 +189,6 @@ __global__ void __launch_bounds__(kScanWarps * 32, 2) scan_kernel(const Params p
                     }
                 }
             }
-#pragma unroll
-            for (int i = 0; i < 32; ++i) x[i] = clean(x[i]);
         } else {
 #pragma unroll
             for (int i = 0; i < 32; ++i) {
@@ -198,6 +196,15 @@ __global__ void __launch_bounds__(kScanWarps * 32, 2) scan_kernel(const Params p
                 x[i] = e < n ? load1(p, base + e) : -INFINITY;
             }
         }
+    };
+    int task = blockIdx.x * kScanWarps + threadIdx.x / 32;
+    float x[32], ahead[32];
+    fetch(ahead, task);
+    for (; task < tasks; task += step) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) x[i] = clean(ahead[i]);
+        fetch(ahead, task + step);  // on their way while this chunk is looked at
+        const int row = task / p.chunks, i0 = (task - row * p.chunks) * kChunk;
         const Rule r = rule_of(p, row);
         float top = x[0], least = x[0];
 #pragma unroll
@@ -223,10 +230,13 @@ __global__ void __launch_bounds__(kScanWarps * 32, 2) scan_kernel(const Params p
         double sum = 0.0;
         if (!r.greedy && !r.by_k && (r.by_p || !r.by_m) && top > -INFINITY) {
             const Weigher weight(top, r.c, tab);
+            // (where logits are so large that `low` is rounded to the largest, it would not be nothing)
+            if (top < INFINITY && head.valid == kChunk && weight.bare(weight.low) < 1e-15) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-                const double w = weight.bare(x[i]);
-                if (x[i] >= weight.low) sum += w;
+                for (int i = 0; i < 32; ++i) sum += weight.bare(fmaxf(x[i], weight.low));  // 2^-60 for nothing
+            } else {
+#pragma unroll
+                for (int i = 0; i < 32; ++i) sum += weight(x[i]);
             }
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -310,50 +320,71 @@ struct Group {
     // The bin in which the running sum, from f.before on, reaches target (or exceeds it), or the last that is not empty; f.before
     // and f.at become the sums before it and of it.  Begins and ends with a barrier of the group.
     __device__ uint32_t reach(Found& f, u64 target, bool beyond) const {
+        constexpr int kSlice = kBins / C, kPer = (kSlice + kPickThreads - 1) / kPickThreads;  // a CTA adds up a slice of the bins
+        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, rank = C == 1 ? 0 : (int)cg::this_cluster().block_rank();
         sync();
-        // two neighbouring bins a thread, their running sums
-        constexpr int kPer = kBins / kPickThreads;
         u64 bin[kPer], mine = 0;
 #pragma unroll
         for (int j = 0; j < kPer; ++j) {
             const int b = threadIdx.x * kPer + j;
             bin[j] = 0;
+            if (b < kSlice)
 #pragma unroll
-            for (int r = 0; r < C; ++r) {
-                const uint32_t* h = &hist[0][0];
-                if constexpr (C > 1) h = cg::this_cluster().map_shared_rank(h, r);
-                bin[j] += (u64)h[b] + ((u64)h[kBins + b] << 15) + ((u64)h[2 * kBins + b] << 30);
-            }
+                for (int r = 0; r < C; ++r) {
+                    const uint32_t* h = &hist[0][rank * kSlice + b];
+                    if constexpr (C > 1) h = cg::this_cluster().map_shared_rank(h, r);
+                    bin[j] += (u64)h[0] + ((u64)h[kBins] << 15) + ((u64)h[2 * kBins] << 30);
+                }
             mine += bin[j];
         }
         u64 run = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const u64 v = __shfl_up_sync(0xffffffffu, run, o);
-            if ((threadIdx.x & 31) >= o) run += v;
+            if (lane >= o) run += v;
         }
-        if ((threadIdx.x & 31) == 31) scratch[threadIdx.x >> 5] = run;
+        if (lane == 31) scratch[warp] = run;
         __syncthreads();
-        u64 start = f.before + run - mine, end_of_all = f.before;
-        for (int w = 0; w < kPickThreads / 32; ++w) {
-            if (w < (int)(threadIdx.x >> 5)) start += scratch[w];
-            end_of_all += scratch[w];
+        u64 part = lane < kPickThreads / 32 ? scratch[lane] : 0, upto = part;
+#pragma unroll
+        for (int o = 1; o < 16; o <<= 1) {
+            const u64 v = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += v;
         }
-        const u64 goal = beyond ? min(target, end_of_all - 1) : min(target, end_of_all);
+        u64 start = run - mine + __shfl_sync(0xffffffffu, upto - part, warp), all = __shfl_sync(0xffffffffu, upto, kPickThreads / 32 - 1);
+        if constexpr (C > 1) {  // the slices before this one
+            if (threadIdx.x == 0) scratch[60] = all;
+            sync();
+            u64 theirs = lane < C ? *cg::this_cluster().map_shared_rank(scratch + 60, lane) : 0, sum = theirs;
+#pragma unroll
+            for (int o = 1; o < C; o <<= 1) {
+                const u64 v = __shfl_up_sync(0xffffffffu, sum, o);
+                if (lane >= o) sum += v;
+            }
+            start += __shfl_sync(0xffffffffu, sum - theirs, rank);
+            all = __shfl_sync(0xffffffffu, sum, C - 1);
+        }
+        start += f.before;
+        const u64 end_of_all = f.before + all, goal = beyond ? min(target, end_of_all - 1) : min(target, end_of_all);
 #pragma unroll
         for (int j = 0; j < kPer; ++j) {
             const u64 end = start + bin[j];
             if (bin[j] && (beyond ? start <= goal && end > goal : start < goal && end >= goal)) {  // one bin of all
-                scratch[16] = threadIdx.x * kPer + j;
-                scratch[17] = start;
-                scratch[18] = bin[j];
+#pragma unroll
+                for (int r = 0; r < C; ++r) {  // told to everybody
+                    u64* to = scratch + 56;
+                    if constexpr (C > 1) to = cg::this_cluster().map_shared_rank(to, r);
+                    to[0] = rank * kSlice + threadIdx.x * kPer + j;
+                    to[1] = start;
+                    to[2] = bin[j];
+                }
             }
             start = end;
         }
         sync();  // also: everybody has read everybody's histogram
-        f.before = scratch[17];
-        f.at = scratch[18];
-        const uint32_t b = (uint32_t)scratch[16];
+        f.before = scratch[57];
+        f.at = scratch[58];
+        const uint32_t b = (uint32_t)scratch[56];
         __syncthreads();
         return b;
     }
@@ -484,34 +515,16 @@ __device__ __forceinline__ u64 prefix(u64 v, u64* scratch, u64& all) {
     __syncthreads();
     if (lane == 31) scratch[warp] = run;
     __syncthreads();
-    u64 before = 0;
-    all = 0;
-    for (int w = 0; w < (int)blockDim.x / 32; ++w) {
-        if (w < warp) before += scratch[w];
-        all += scratch[w];
+    const u64 part = lane < kPickThreads / 32 ? scratch[lane] : 0;
+    u64 upto = part;
+#pragma unroll
+    for (int o = 1; o < 16; o <<= 1) {
+        const u64 t = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += t;
     }
+    all = __shfl_sync(0xffffffffu, upto, kPickThreads / 32 - 1);
+    const u64 before = __shfl_sync(0xffffffffu, upto - part, warp);
     return before + run - v;
-}
-
-// One value a thread, smallest first, of which those of threads >= n are the largest there are.
-template <class T>
-__device__ __forceinline__ T sorted(T v, int n, T* shared) {
-    const int tid = threadIdx.x;
-    for (int k = 2; k < 2 * n || k <= 32; k <<= 1)
-        for (int j = k >> 1; j > 0; j >>= 1) {
-            T o;
-            if (j >= 32) {
-                __syncthreads();
-                shared[tid] = v;
-                __syncthreads();
-                o = shared[tid ^ j];
-            } else {
-                o = __shfl_xor_sync(0xffffffffu, v, j);
-            }
-            v = ((tid & k) == 0) == ((tid & j) == 0) ? min(v, o) : max(v, o);
-        }
-    __syncthreads();
-    return v;
 }
 
 // ---- pick ---------------------------------------------------------------------------------------------------------------
@@ -529,6 +542,7 @@ __device__ Outcome pick_few(const Group<1>& g, PickSmem& s, const Params& p, int
     const int tid = threadIdx.x, lane = tid & 31;
     const uint32_t first = order_key(g.weight.top), last = order_key(lowest);
     uint32_t keep_to = last;  // key of the last element that may matter
+    bool by_p_late = false;   // top_p's cut lies behind min_p's
     if (r.by_k ? have > r.k : r.by_p) {
         const int shift = max(0, 32 - __clz(last - first) - kBinBits);
         const u64 target = r.by_k ? (u64)r.k : min(max((u64)ceil(r.p * (double)whole), 1ull), whole);
@@ -541,15 +555,15 @@ __device__ Outcome pick_few(const Group<1>& g, PickSmem& s, const Params& p, int
             }
         Found f{first, 0, 0};
         const uint32_t b = g.reach(f, target, false);
-        if (f.before + f.at < target) {
-            if (bound > -INFINITY) return kNeedsMore;
+        if (f.before + f.at < target) {  // top_p reaches beyond the list; min_p may still cut within it
+            if (bound > -INFINITY && !(by_p_late = r.by_m && !(g.weight(bound) >= r.m))) return kNeedsMore;
         } else {
             keep_to = min(last, first + (b << shift) + ((1u << shift) - 1));
         }
     } else if (r.by_k && bound > -INFINITY) {
         return kNeedsMore;
     }
-    const bool by_m_alone = r.by_m && !r.by_k && !r.by_p;
+    const bool by_m_alone = r.by_m && !r.by_k && (!r.by_p || by_p_late);
     if (by_m_alone && bound > -INFINITY && g.weight(bound) >= r.m) return kNeedsMore;
     // what is left, side by side in the histogram's place
     u64* list = reinterpret_cast<u64*>(&g.hist[0][0]);
@@ -557,48 +571,77 @@ __device__ Outcome pick_few(const Group<1>& g, PickSmem& s, const Params& p, int
     __syncthreads();
     if (tid == 0) *count = 0;
     __syncthreads();
-    for (int i0 = 0; i0 < have; i0 += kPickThreads) {
+    uint32_t takes = 0;  // bit per round: this thread's element is among them
+    int upto = 0, warp_total = 0;
+    static_assert(kList <= 32 * kPickThreads, "a bit a round");
+    for (int i0 = 0, round = 0; i0 < have; i0 += kPickThreads, ++round) {
         const int i = i0 + tid;
         const float x = i < have ? s.x[i] : -INFINITY;
         const bool take = x > -INFINITY && order_key(x) <= keep_to && (!by_m_alone || g.weight(x) >= r.m);
+        if (take) takes |= 1u << round;
+        warp_total += __popc(__ballot_sync(0xffffffffu, take));
+    }
+    if (lane == 0 && warp_total) upto = atomicAdd(count, warp_total);
+    upto = __shfl_sync(0xffffffffu, upto, 0);
+    for (int i0 = 0, round = 0; i0 < have; i0 += kPickThreads, ++round) {
+        const bool take = (takes >> round) & 1;
         const uint32_t b = __ballot_sync(0xffffffffu, take);
-        int at = 0;
-        if (lane == 0 && b) at = atomicAdd(count, __popc(b));
-        at = __shfl_sync(0xffffffffu, at, 0) + __popc(b & ((1u << lane) - 1));
-        if (take && at < kPickThreads) list[at] = (u64)order_key(x) << 32 | s.index[i];
+        const int at = upto + __popc(b & ((1u << lane) - 1));
+        if (take && at < kPickThreads) list[at] = (u64)order_key(s.x[i0 + tid]) << 32 | s.index[i0 + tid];
+        upto += __popc(b);
     }
     __syncthreads();
     const int n = *count;
     if (n > kPickThreads) return kTooMany;
-    u64 v = tid < n ? list[tid] : ~0ull;
-    v = sorted(v, n, list);
-    // thread i has the row's i-th token
-    u64 *sums = list + kPickThreads, *weights = sums + kPickThreads, all;
+    u64 *weights = list + kPickThreads, all;
+    const u64 v = tid < n ? list[tid] : ~0ull;
     const float x = key_logit((uint32_t)(v >> 32));
     const double w = tid < n ? g.weight(x) : 0.0;
     const u64 units = tid < n ? to_units(w) : 0;
-    const u64 before = prefix(units, g.scratch, all);
-    list[tid] = v;
-    sums[tid] = before + units;
     weights[tid] = units;
     __syncthreads();
-    auto enough = [&](int rank) { return key_logit((uint32_t)(list[rank] >> 32)) >= bound; };
-    int kept = n;
-    if (r.by_k && n > r.k) kept = r.k;
-    if (r.by_k && bound > -INFINITY && !enough(kept - 1)) return kNeedsMore;
-    if (r.by_p) {
-        const u64 mass = r.by_k ? sums[kept - 1] : whole, target = min(max((u64)ceil(r.p * (double)mass), 1ull), mass);
-        kept = __syncthreads_count(tid < kept && before < target);
-        if (bound > -INFINITY && !enough(kept - 1)) return kNeedsMore;
+    // rank of this thread's element and the weight ahead of it, by looking at every other one
+    int rank = 0;
+    u64 before = 0;
+    if (tid < (n + 31) / 32 * 32) {
+#pragma unroll 4
+        for (int j = 0; j < n; ++j) {
+            const bool ahead = list[j] < v;
+            rank += ahead;
+            before += ahead ? weights[j] : 0;
+        }
     }
-    if (r.by_m) kept = __syncthreads_count(tid < kept && w >= r.m);
-    const u64 sum = sums[kept - 1], goal = min((u64)((double)r.u * (double)sum), sum - 1);
-    // the kept ones by index
-    uint32_t c = tid < kept ? (uint32_t)v << 9 | tid : 0xffffffffu;
-    static_assert(kPickThreads == 512 && NEON_SAMPLER_MAX_VOCAB <= 1 << 23, "index and rank share a word");
-    c = sorted(c, kept, reinterpret_cast<uint32_t*>(list));
-    const u64 mine = tid < kept ? weights[c & 511] : 0, at = prefix(mine, g.scratch, all);
-    if (at <= goal && at + mine > goal) answer(p, row, (int)(c >> 9), (float)((double)mine / (double)sum), kept);
+    // the lowest kept logit, and whether the list is sure to hold all above it
+    auto sure = [&](bool kept) { return !(bound > -INFINITY) || !__syncthreads_or(kept && !(x >= bound)); };
+    bool kept = tid < n && (!r.by_k || rank < r.k);
+    if (r.by_k && !sure(kept)) return kNeedsMore;
+    if (r.by_p && !by_p_late) {
+        u64 mass = whole;
+        if (r.by_k) prefix(kept ? units : 0, g.scratch, mass);
+        const u64 target = min(max((u64)ceil(r.p * (double)mass), 1ull), mass);
+        kept = kept && before < target;
+        if (!sure(kept)) return kNeedsMore;
+    }
+    if (r.by_m) kept = kept && w >= r.m;
+    const int number = __syncthreads_count(kept);
+    u64 sum;
+    const int slot = (int)prefix(kept ? 1 : 0, g.scratch, all);
+    prefix(kept ? units : 0, g.scratch, sum);
+    const u64 goal = min((u64)((double)r.u * (double)sum), sum - 1);
+    // the kept ones: the weight of those with lower indices
+    __syncthreads();
+    if (kept) list[slot] = (u64)(uint32_t)v << 32 | tid;
+    __syncthreads();
+    if (tid < number) {
+        const u64 me = list[tid], mine = weights[me & 511];
+        u64 at = 0;
+#pragma unroll 4
+        for (int j = 0; j < number; ++j) {
+            const u64 other = list[j];
+            if (other < me) at += weights[other & 511];
+        }
+        if (at <= goal && at + mine > goal) answer(p, row, (int)(me >> 32), (float)((double)mine / (double)sum), number);
+    }
     return kDone;
 }
 
@@ -640,8 +683,17 @@ __global__ void __launch_bounds__(kPickThreads) pick_kernel(const Params p, int 
     }
     if ((tid & 31) == 0) { fs[tid >> 5] = top; fs[32 + (tid >> 5)] = bound; fs[64 + (tid >> 5)] = low; }
     __syncthreads();
-    for (int w = 0; w < kPickThreads / 32; ++w) { top = fmaxf(top, fs[w]); bound = fmaxf(bound, fs[32 + w]); low = fminf(low, fs[64 + w]); }
+    top = fs[tid & 15];
+    bound = fs[32 + (tid & 15)];
+    low = fs[64 + (tid & 15)];
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) {
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        bound = fmaxf(bound, __shfl_xor_sync(0xffffffffu, bound, o));
+        low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
+    }
     __syncthreads();
+    static_assert(kPickThreads == 512, "sixteen warps");
     if (tid == 0 && p.left) p.left[row] = 0;
     if (top == -INFINITY) {
         if (tid == 0) answer(p, row, -1, 0.f, 0);
@@ -712,12 +764,25 @@ __global__ void __launch_bounds__(kPickThreads) pick_kernel(const Params p, int 
             }
             __syncthreads();
             const uint2* lists = p.entries + (long long)row * p.chunks * kSlots;
-            for (int i = tid; i < p.chunks * kSlots; i += kPickThreads) {
-                const int c = i / kSlots, e = i % kSlots;
-                if (e < (int)starts[kBins + c]) {
-                    const uint2 v = lists[i];
-                    s.x[starts[c] + e] = __uint_as_float(v.x);
-                    s.index[starts[c] + e] = v.y;
+            // a half warp per list, sixteen lists a round: most fit two loads
+            const int half = tid >> 4, slot = tid & 15;
+#pragma unroll 2
+            for (int c = half; c < p.chunks; c += kPickThreads / 16) {
+                const int to = starts[c], count = starts[kBins + c];
+                uint2 v[2];
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    if (16 * h + slot < count) v[h] = lists[c * kSlots + 16 * h + slot];
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    if (16 * h + slot < count) {
+                        s.x[to + 16 * h + slot] = __uint_as_float(v[h].x);
+                        s.index[to + 16 * h + slot] = v[h].y;
+                    }
+                for (int e = 32 + slot; e < count; e += 16) {
+                    const uint2 u = lists[c * kSlots + e];
+                    s.x[to + e] = __uint_as_float(u.x);
+                    s.index[to + e] = u.y;
                 }
             }
             __syncthreads();
@@ -760,6 +825,9 @@ struct WholeSmem {
     double tab[kTable];
 };
 
+// Logits of a CTA: a whole number of four.
+__host__ __device__ inline int whole_share(int vocab) { return (vocab + 4 * kClusterCtas - 1) / (4 * kClusterCtas) * 4; }
+
 // Rows that pick left, one after the other on each cluster.  A CTA keeps its share of the row in shared memory, a warp's
 // stretch of it is contiguous.
 __global__ void __cluster_dims__(kClusterCtas, 1, 1) __launch_bounds__(kPickThreads) whole_kernel(const Params p) {
@@ -769,7 +837,7 @@ __global__ void __cluster_dims__(kClusterCtas, 1, 1) __launch_bounds__(kPickThre
     constexpr int kWarps = kPickThreads / 32;
     const cg::cluster_group cluster = cg::this_cluster();
     const int rank = (int)cluster.block_rank(), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int share = (p.vocab + kClusterCtas - 1) / kClusterCtas, i0 = min(rank * share, p.vocab), n = min(share, p.vocab - i0);
+    const int share = whole_share(p.vocab), i0 = min(rank * share, p.vocab), n = min(share, p.vocab - i0);
     const int stretch = (share + kWarps - 1) / kWarps, w0 = min(warp * stretch, n), w1 = min(w0 + stretch, n);
     fill_table(s.tab);
     pdl_wait();
@@ -779,8 +847,20 @@ __global__ void __cluster_dims__(kClusterCtas, 1, 1) __launch_bounds__(kPickThre
         const ChunkHead* heads = p.heads + (long long)row * p.chunks;
         __syncthreads();
         float top = -INFINITY;
+        const long long base = row * p.stride + i0;
+        if (p.dtype == 0 && (reinterpret_cast<uintptr_t>(p.logits) + base * 4) % 16 == 0) {
+            const float4* from = reinterpret_cast<const float4*>(static_cast<const float*>(p.logits) + base);
 #pragma unroll 8
-        for (int i = tid; i < n; i += kPickThreads) xs[i] = load1(p, row * p.stride + i0 + i);
+            for (int i = tid; i < n / 4; i += kPickThreads) {
+                const float4 v = __ldcs(from + i);
+                reinterpret_cast<float4*>(xs)[i] = make_float4(clean(v.x), clean(v.y), clean(v.z), clean(v.w));
+            }
+            if (tid < n % 4) xs[n / 4 * 4 + tid] = load1(p, base + n / 4 * 4 + tid);
+        } else {
+#pragma unroll 8
+            for (int i = tid; i < n; i += kPickThreads) xs[i] = load1(p, base + i);
+        }
+        if (tid >= n % 4 && tid < 4 && n % 4) xs[n / 4 * 4 + tid] = -INFINITY;  // to a whole number of four
         ChunkHead mine{-INFINITY, -INFINITY, 0, 0, 0.0};
         if (tid < p.chunks) mine = heads[tid];
         top = mine.max;
@@ -797,8 +877,14 @@ __global__ void __cluster_dims__(kClusterCtas, 1, 1) __launch_bounds__(kPickThre
         prefix(mine.max > -INFINITY ? (u64)(mine.weight * weight(mine.max) * kUnit) : 0ull, s.scratch, whole);
         prefix(mine.valid, s.scratch, have);
         auto each = [&](auto f) {
-            for (int i = tid; i < n; i += kPickThreads)
-                if (xs[i] > -INFINITY) f(xs[i], (uint32_t)(i0 + i));
+#pragma unroll 2
+            for (int i = tid; i < (n + 3) / 4; i += kPickThreads) {
+                const float4 v = reinterpret_cast<const float4*>(xs)[i];
+                if (v.x > -INFINITY) f(v.x, (uint32_t)(i0 + 4 * i));
+                if (v.y > -INFINITY) f(v.y, (uint32_t)(i0 + 4 * i + 1));
+                if (v.z > -INFINITY) f(v.z, (uint32_t)(i0 + 4 * i + 2));
+                if (v.w > -INFINITY) f(v.w, (uint32_t)(i0 + 4 * i + 3));
+            }
         };
         Cut cut;
         find_cut<kClusterCtas>(g, p, r, have, whole, -INFINITY, kLowest, each, cut);
@@ -810,9 +896,11 @@ __global__ void __cluster_dims__(kClusterCtas, 1, 1) __launch_bounds__(kPickThre
             return !r.by_m || w >= r.m ? to_units(w) : 0;
         };
         u64 sum = 0, count = 0;
+        const float cut_logit = cut.key == 0xffffffffu ? kLowest : key_logit(cut.key);
+#pragma unroll 4
         for (int i = w0 + lane; i < w1; i += 32) {
             const float x = xs[i];
-            if (!(x > -INFINITY) || !cut.keeps(order_key(x), i0 + i)) continue;
+            if (!(x >= cut_logit) || !cut.keeps(order_key(x), i0 + i)) continue;
             const double w = weight(x);
             if (r.by_m && !(w >= r.m)) continue;
             sum += to_units(w);
