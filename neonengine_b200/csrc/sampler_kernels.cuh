@@ -42,7 +42,8 @@ typedef unsigned long long u64;
 struct ChunkHead {   // what a warp of the scan leaves about its logits
     float max, bound;   // largest; every logit >= bound is listed
     int listed, valid;  // entries; logits above -infinity
-    double weight;      // relative to max
+    double weight;      // of all, relative to 2^exponent, or (exponent = kRelative) to max
+    int exponent, pad;
 };
 
 struct Params {
@@ -131,8 +132,40 @@ struct Weigher {
     }
     __device__ __forceinline__ double operator()(float x) const { return x == top ? 1.0 : x >= low ? bare(x) : 0.0; }  // exactly 1 for the largest
 };
+// Sums of many weights, at half the instructions: 2^(x log2(e) / temperature), not relative to a largest.  The product's integer
+// part is found in f32; what is left of it is exact to 2^-25, as a fused multiply-add rounds once, and so small that the cubic can be
+// f32, too: 5e-10 of a weight, and no more than 1e-9 of a row's sum of any number of them.
+struct Adder {
+    float hi, lo, low;  // 64 log2(e) / temperature as two f32
+    const double* tab;
+    bool fits;          // the powers are within f64's range, and `low` is below the largest by what it should be
+    __device__ __forceinline__ Adder(const Weigher& w) : hi((float)w.c), lo((float)(w.c - (double)(float)w.c)), low(w.low), tab(w.tab) {
+        fits = fabs(w.off) < 64.0 * 900 && w.top < INFINITY && (double)w.top * w.c - (double)w.low * w.c > 64.0 * 55;
+    }
+    __device__ __forceinline__ float steps(float x) const { return fmaf(x, hi, 12582912.f); }  // 1.5 * 2^23 + the product's integer part
+    __device__ __forceinline__ void add(double& sum, float x) const {
+        x = fmaxf(x, low);  // 2^-60 of the largest for nothing
+        const float k = steps(x), r = fmaf(x, lo, fmaf(x, hi, 12582912.f - k));
+        const uint32_t bits = __float_as_uint(k);  // its low bits are the integer's
+        const double v = tab[(bits & 63) * 32];
+        const float q = r * fmaf(r, fmaf(r, 2.1173136998904953e-07f, 5.8649049505537566e-05f), 0.010830424696249145f);
+        const double w = __hiloint2double(__double2hiint(v) + (int)((bits & ~63u) << 14), __double2loint(v));
+        sum += fma(w, (double)q, w);
+    }
+    // 2^e of about the weight of x, and its inverse's power
+    __device__ __forceinline__ int exponent(float x) const { return (int)(__float_as_uint(steps(x)) - 0x4b400000u) >> 6; }
+};
+constexpr int kRelative = -0x7fffffff - 1;
+
 __device__ __forceinline__ u64 to_units(double w) {  // w <= 2^9, in 2^-43, rounded
     return (u64)(__double_as_longlong(fma(w, kUnit, 4503599627370496.0)) & 0xfffffffffffffll);
+}
+
+// A chunk's weight, relative to the row's largest.
+__device__ __forceinline__ u64 chunk_units(const ChunkHead& h, const Weigher& w) {
+    if (h.max == -INFINITY) return 0;
+    const double factor = h.exponent == kRelative ? w(h.max) : exp2((64.0 * h.exponent + w.off) * (1.0 / 64.0));
+    return (u64)(h.weight * factor * kUnit);
 }
 
 // ---- scan -------------------------------------------------------------------------------------------------------------
@@ -228,12 +261,17 @@ __global__ void __launch_bounds__(kScanWarps * 32, 2) scan_kernel(const Params p
         }
         // the whole row's weight counts where nothing but top_p cuts it
         double sum = 0.0;
+        head.exponent = kRelative;
+        head.pad = 0;
         if (!r.greedy && !r.by_k && (r.by_p || !r.by_m) && top > -INFINITY) {
             const Weigher weight(top, r.c, tab);
-            // (where logits are so large that `low` is rounded to the largest, it would not be nothing)
-            if (top < INFINITY && head.valid == kChunk && weight.bare(weight.low) < 1e-15) {
+            const Adder adder(weight);
+            if (adder.fits && head.valid == kChunk) {
+                double part[4] = {};
 #pragma unroll
-                for (int i = 0; i < 32; ++i) sum += weight.bare(fmaxf(x[i], weight.low));  // 2^-60 for nothing
+                for (int i = 0; i < 32; ++i) adder.add(part[i & 3], x[i]);
+                head.exponent = adder.exponent(top);
+                sum = ((part[0] + part[1]) + (part[2] + part[3])) * __hiloint2double((1023 - head.exponent) << 20, 0);
             } else {
 #pragma unroll
                 for (int i = 0; i < 32; ++i) sum += weight(x[i]);
@@ -660,7 +698,7 @@ __global__ void __launch_bounds__(kPickThreads) pick_kernel(const Params p, int 
     static_assert(NEON_SAMPLER_MAX_VOCAB / kChunk <= kBins, "the histogram holds the chunks' list lengths");
     // the largest logit, the highest of the bounds, and a bound of all that is listed
     float top = -INFINITY, bound = -INFINITY, low = INFINITY;
-    ChunkHead mine{-INFINITY, -INFINITY, 0, 0, 0.0};
+    ChunkHead mine{-INFINITY, -INFINITY, 0, 0, 0.0, kRelative, 0};
     if (direct) {
         for (int i = tid; i < p.vocab; i += kPickThreads) {
             s.x[i] = load1(p, base + i);
@@ -703,7 +741,7 @@ __global__ void __launch_bounds__(kPickThreads) pick_kernel(const Params p, int 
     if (!direct && (r.greedy || !r.filters())) {
         // weights of the chunks, in order; greedily: the first chunk that has the maximum
         u64 w = r.greedy ? (u64)(mine.max == top) : 0ull, all;
-        if (!r.greedy && mine.max > -INFINITY) w = (u64)(mine.weight * weight(mine.max) * kUnit);
+        if (!r.greedy) w = chunk_units(mine, weight);
         const u64 run = prefix(w, s.scratch, all);
         const u64 target = r.greedy ? 0 : min((u64)((double)r.u * (double)all), all - 1);
         if (run <= target && run + w > target) {
@@ -754,7 +792,7 @@ __global__ void __launch_bounds__(kPickThreads) pick_kernel(const Params p, int 
     } else {
         // the listed elements, side by side
         const uint32_t at = (uint32_t)prefix(mine.listed, s.scratch, n64);
-        prefix(mine.max > -INFINITY ? (u64)(mine.weight * weight(mine.max) * kUnit) : 0ull, s.scratch, whole);
+        prefix(chunk_units(mine, weight), s.scratch, whole);
         fits = n64 > 0 && n64 <= kList;
         if (fits) {
             uint32_t* starts = &s.hist[0][0];  // where each chunk's entries go, and how many they are
@@ -861,7 +899,7 @@ __global__ void __cluster_dims__(kClusterCtas, 1, 1) __launch_bounds__(kPickThre
             for (int i = tid; i < n; i += kPickThreads) xs[i] = load1(p, base + i);
         }
         if (tid >= n % 4 && tid < 4 && n % 4) xs[n / 4 * 4 + tid] = -INFINITY;  // to a whole number of four
-        ChunkHead mine{-INFINITY, -INFINITY, 0, 0, 0.0};
+        ChunkHead mine{-INFINITY, -INFINITY, 0, 0, 0.0, kRelative, 0};
         if (tid < p.chunks) mine = heads[tid];
         top = mine.max;
         float* fs = reinterpret_cast<float*>(s.scratch);
@@ -874,7 +912,7 @@ __global__ void __cluster_dims__(kClusterCtas, 1, 1) __launch_bounds__(kPickThre
         const Weigher weight(top, r.c, s.tab);
         const Group<kClusterCtas> g{s.hist, s.scratch, weight};
         u64 whole, have;
-        prefix(mine.max > -INFINITY ? (u64)(mine.weight * weight(mine.max) * kUnit) : 0ull, s.scratch, whole);
+        prefix(chunk_units(mine, weight), s.scratch, whole);
         prefix(mine.valid, s.scratch, have);
         auto each = [&](auto f) {
 #pragma unroll 2
