@@ -171,15 +171,18 @@ int launch_attend(const Shape& s, const Batch& b, const uint8_t* cache, int dtyp
     return 2;
 }
 
-int launch_append(const AppendParams& p, int dtype, int out_dtype, cudaStream_t st) {
-    const int units = (p.q ? p.s.nq : 0) * (p.s.D / 16) + 2 * p.s.nkv * (p.s.D / 16);
-    const int threads = std::min(512, std::max(64, (units + 31) / 32 * 32));
-#define RUN(DT)                                                                                  \
-    if (dtype == DT) {                                                                           \
-        if (out_dtype == NEON_KV4_F16) append_kernel<DT, __half><<<p.b.rows, threads, 0, st>>>(p);   \
-        else append_kernel<DT, __nv_bfloat16><<<p.b.rows, threads, 0, st>>>(p);                  \
+int launch_append(const AppendParams& given, int dtype, int out_dtype, cudaStream_t st) {
+    AppendParams p = given;
+    // a warp per row, unless there are so few rows that its ten or so rounds would be what takes the time
+    const int heads = (p.q ? p.s.nq : 0) + 2 * p.s.nkv, rounds = (heads * p.s.D / 16 + 31) / 32;
+    p.split = std::min(rounds, std::max(1, kSms * 16 / p.b.rows));
+    const unsigned grid = (unsigned)(((long long)p.b.rows * p.split + kAppendWarps - 1) / kAppendWarps);
+#define RUN(DT, DIM)                                                                                              \
+    if (dtype == DT && p.s.D == DIM) {                                                                            \
+        if (out_dtype == NEON_KV4_F16) append_kernel<DT, __half, DIM><<<grid, kAppendWarps * 32, 0, st>>>(p);     \
+        else append_kernel<DT, __nv_bfloat16, DIM><<<grid, kAppendWarps * 32, 0, st>>>(p);                        \
     }
-    RUN(NEON_KV4_F32) RUN(NEON_KV4_BF16) RUN(NEON_KV4_F16)
+    RUN(NEON_KV4_F32, 64) RUN(NEON_KV4_BF16, 64) RUN(NEON_KV4_F16, 64) RUN(NEON_KV4_F32, 128) RUN(NEON_KV4_BF16, 128) RUN(NEON_KV4_F16, 128)
 #undef RUN
     return 1;
 }
@@ -274,11 +277,11 @@ int neon_kv4_read(neon_kv4_handle* h, const neon_kv4_batch* batch, const void* c
         return fail(h, NEON_MOE_EINVAL, "k_out and v_out have to be 16-byte aligned");
     if (!k_out && !v_out) return NEON_MOE_OK;
     ON_DEVICE(h);
-    const ReadParams p{device_batch(h, batch, rows), h->shape, static_cast<const uint8_t*>(cache), k_out, v_out};
-    const int threads = std::min(256, std::max(32, 2 * h->shape.nkv * h->shape.D / 8 / 32 * 32));
+    // few rows: four warps each, so that a row's rounds do not follow one another
+    const ReadParams p{device_batch(h, batch, rows), h->shape, static_cast<const uint8_t*>(cache), k_out, v_out, rows <= 1024 ? 4 : 1};
     cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);
-    if (dtype == NEON_KV4_F32) read_kernel<float><<<rows, threads, 0, st>>>(p);
-    else read_kernel<__nv_bfloat16><<<rows, threads, 0, st>>>(p);
+    if (dtype == NEON_KV4_F32) read_kernel<float><<<((unsigned)rows * p.split + 3) / 4, 128, 0, st>>>(p);
+    else read_kernel<__nv_bfloat16><<<((unsigned)rows * p.split + 3) / 4, 128, 0, st>>>(p);
     return launched(h, 1);
 }
 
