@@ -1,0 +1,436 @@
+// Attention over the 4-bit paged cache: chunks of prompts, on the tensor cores of a CTA (tcgen05).
+//
+// An item is (sequence, key/value head, 256 rows: 32 tokens at eight query heads a key/value head), as two tiles of 128 rows.  Per
+// step of 64 positions:
+//   copies    a bulk copy per page brings the record (codes and scales) into shared memory, four steps ahead;
+//   unpacking four warps turn it into two tf32 operands: keys [64 positions][64], values transposed [64 + 16][64 positions], whose
+//             row 64 is ones, so that the softmax sum is one more column of the output;
+//   products  one thread issues S = Q K^T (f32 in tensor memory, two buffers a tile) and O += P V with P read from tensor memory;
+//   softmax   two groups of four warps, one per tile, a row a thread: no exchange between threads.  P takes the place of S.
+//             The output is rescaled (a trip through the registers) only when a row's maximum rises by 2^8.
+// tf32 holds bf16 and f16 queries, and codes times any E8M0 scale, exactly; probabilities are cut to 11 bits (a cut that the
+// sum, taken from the same operand, shares).  bf16 probabilities would be four times as coarse, f16 ones could not meet every
+// scale of values.
+// What bounds it: the special function units (16 exponentials a clock and SM: 1024 clocks a step) and, with tf32 at half the bf16
+// rate, the products (1152 clocks a step), which overlap.
+#pragma once
+#include "kv4_attend.cuh"
+
+namespace neon {
+namespace kv4 {
+
+constexpr int kPreRows = 256, kPreStages = 3, kPreRaw = 4, kPreInfo = 8, kPreN = 80;
+constexpr int kPreSoftmaxWarps = 8, kPreUnpackWarps = 4, kPreWarps = kPreSoftmaxWarps + kPreUnpackWarps + 1;
+constexpr int kPreValueScale = 252;  // value (and key) scales above 2^125 count as 2^125: what a row does not see is finite
+
+struct PrefillInfo {     // of a step
+    uint32_t missing;    // pages that are not there
+    uint32_t special;    // a value block is NaN:
+    uint32_t nan[2][2];  // which, [block][position / 32]
+};
+
+struct PrefillSmem {
+    unsigned char q[2][kPreRows * 128];               // [half of the columns][row][32 f32], 128-byte swizzle
+    unsigned char k[kPreStages][2][kStep * 128];      // [half of the columns][position][32 f32]
+    unsigned char v[kPreStages][2][kPreN * 128];      // [half of the positions][column][32 f32]
+    unsigned char raw[kPreRaw][kStep * (64 + 4)];
+    PrefillInfo info[kPreInfo];
+    uint64_t raw_full[kPreRaw], kv_full[kPreStages], kv_empty[kPreStages], s_full[2][2], p_full[2][2], pv_done[2], drained;
+    uint32_t tmem;
+    int abort, item[4];
+};
+
+// tensor memory columns: S (then P) of tile x, buffer b; O of tile x
+__device__ __forceinline__ uint32_t col_s(int x, int b) { return x * 128 + b * 64; }
+__device__ __forceinline__ uint32_t col_o(int x) { return 256 + x * kPreN; }
+
+__device__ __forceinline__ void mma_tf32_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::tf32 [%0], %1, %2, %3, p;\n\t}"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void mma_tf32_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::tf32 [%0], [%1], %2, %3, p;\n\t}"
+                 ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+// 32 columns of this warp's 32 lanes
+__device__ __forceinline__ void tmem_load32(uint32_t addr, uint32_t* r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+          "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]),
+          "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(addr));
+}
+__device__ __forceinline__ void tmem_store32(uint32_t addr, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
+        ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+          "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
+          "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_load16(uint32_t addr, uint32_t* r) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+                   "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(addr));
+}
+__device__ __forceinline__ void tmem_store16(uint32_t addr, const uint32_t* r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+                 ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+                   "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_wait_load() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// 8 codes as f32, times a power of two
+__device__ __forceinline__ void codes_to_f32(uint32_t w, float scale, float (&x)[8]) {
+    uint32_t h[4];
+    codes_to_f16(w, h);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[i]));
+        x[2 * i] = f.x * scale;
+        x[2 * i + 1] = f.y * scale;
+    }
+}
+
+template <int P>
+__global__ void __launch_bounds__(kPreWarps * 32, 1) prefill_kernel(const AttendParams p) {
+    constexpr int D = 64, kPages = kStep / P, kRec = P * (D + D / 16), kCodes = P * D / 2, kScales = P * D / 32;
+    extern __shared__ unsigned char unaligned[];
+    PrefillSmem& s = *reinterpret_cast<PrefillSmem*>((reinterpret_cast<uintptr_t>(unaligned) + 1023) & ~(uintptr_t)1023);
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    // ---- the item: the last tiles, which see the most, first --------------------------------------------------------------
+    const int kvh = blockIdx.x % p.s.nkv, order = blockIdx.x / p.s.nkv;
+    if (warp == 0) {
+        int before = 0, found = -1, tile = 0;
+        for (int s0 = 0; s0 < p.b.n; s0 += 32) {
+            const int b = p.b.n - 1 - s0 - lane;  // sequences from the last on
+            int tiles = 0;
+            if (b >= 0) {
+                tiles = (p.b.span(b).y * p.G + kPreRows - 1) / kPreRows;
+                if (p.b.seq_lens[b] > p.b.width * P || (p.b.cu_q && p.b.cu_q[b + 1] < p.b.cu_q[b])) report(p.b.status, NEON_KV4_BAD_LENGTH);
+            }
+            int upto = tiles;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int v = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += v;
+            }
+            upto += before;
+            const uint32_t hit = __ballot_sync(0xffffffffu, order >= upto - tiles && order < upto);
+            if (hit) {
+                const int l = __ffs(hit) - 1;
+                found = p.b.n - 1 - s0 - l;
+                tile = __shfl_sync(0xffffffffu, upto, l) - 1 - order;  // the sequence's last tile first
+                break;
+            }
+            before = __shfl_sync(0xffffffffu, upto, 31);
+        }
+        if (lane == 0) {
+            s.item[0] = found;
+            s.item[1] = tile;
+            s.abort = 0;
+        }
+    }
+    if (tid == 0) {
+        for (int i = 0; i < kPreRaw; ++i) sm100::mbar_init(&s.raw_full[i], 1);
+        for (int i = 0; i < kPreStages; ++i) {
+            sm100::mbar_init(&s.kv_full[i], kPreUnpackWarps * 32);
+            sm100::mbar_init(&s.kv_empty[i], 1);
+        }
+        for (int i = 0; i < 4; ++i) {
+            sm100::mbar_init(&s.s_full[0][0] + i, 1);
+            sm100::mbar_init(&s.p_full[0][0] + i, 128);
+        }
+        for (int i = 0; i < 2; ++i) sm100::mbar_init(&s.pv_done[i], 1);
+        sm100::mbar_init(&s.drained, 1);
+        sm100::fence_barrier_init();
+    }
+    if (tid < kPreInfo) s.info[tid] = {};
+    // the rows of ones and zeros behind the values
+    for (int i = tid; i < kPreStages * 2 * 16 * 32; i += kPreWarps * 32) {
+        const int at = i % 32, row = 64 + i / 32 % 16, half = i / 512 % 2, stage = i / 1024;
+        *reinterpret_cast<float*>(s.v[stage][half] + row * 128 + (((at / 4) ^ (row & 7)) * 16) + at % 4 * 4) = row == 64 ? 1.f : 0.f;
+    }
+    __syncthreads();
+    const int seq = s.item[0];
+    if (seq < 0) return;
+    AttendParams one = p;
+    one.R = kPreRows;
+    const SeqPlan q = plan_of(one, seq);
+    const int r0 = s.item[1] * kPreRows, rows = min(kPreRows, q.n * p.G - r0);
+    const int pos_lo = q.pos0 + p.token(r0), pos_hi = min(q.pos0 + p.token(r0 + rows - 1), q.len - 1);
+    const int first = p.window > 0 ? max(pos_lo - p.window + 1, 0) : 0;
+    const int step0 = first / kStep, n = pos_hi < first ? 0 : pos_hi / kStep + 1 - step0;
+    // ---- queries, as f32 --------------------------------------------------------------------------------------------------
+    const int tile = warp / 4;  // of a softmax warp
+    const int rr = r0 + tid, token = p.token(min(rr, r0 + rows - 1)), head = kvh * p.G + min(rr, r0 + rows - 1) - token * p.G;
+    if (tid < kPreRows) {
+        const uint16_t* src = static_cast<const uint16_t*>(p.q) + (q.row0 + token) * p.q_stride + (long long)head * D;
+        const float sign = tid < rows ? (p.scale < 0.f ? -1.f : 1.f) : 0.f;
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+            float x[8];
+            if (p.half) load8(reinterpret_cast<const __half*>(src) + c * 8, x);
+            else load8(reinterpret_cast<const __nv_bfloat16*>(src) + c * 8, x);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = sign == 0.f ? 0.f : x[i] * sign;
+            unsigned char* row = s.q[c / 4] + tid * 128;
+            *reinterpret_cast<float4*>(row + ((((c % 4) * 2) ^ (tid & 7)) * 16)) = make_float4(x[0], x[1], x[2], x[3]);
+            *reinterpret_cast<float4*>(row + ((((c % 4) * 2 + 1) ^ (tid & 7)) * 16)) = make_float4(x[4], x[5], x[6], x[7]);
+        }
+    }
+    if (warp == kPreWarps - 1) sm100::tmem_alloc(&s.tmem, 512);
+    sm100::fence_proxy_async();
+    sm100::tc_fence_before();
+    __syncthreads();
+    sm100::tc_fence_after();
+    const uint32_t tmem = s.tmem;
+    // by a whole warp, which goes on or gives up as one; when a wait runs out, all others are called off
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+        return (bool)__all_sync(0xffffffffu, sm100::mbar_wait(bar, parity & 1, &s.abort, p.b.status, NEON_KV4_TIMEOUT, kWaitCycles));
+    };
+
+    if (n > 0 && warp < kPreSoftmaxWarps) {
+        // ---- softmax: this thread's row ------------------------------------------------------------------------------------
+        const int hi = tid < rows ? min(q.pos0 + token, q.len - 1) : -1, lo = p.window > 0 ? q.pos0 + token - p.window : -1;
+        const float positive = fabsf(p.scale) * kLog2e, qs = positive == 0.f ? 1e-30f : positive;
+        const uint32_t lanes = tmem + ((uint32_t)(warp & 3) << 21);  // this warp's lanes: 32 * (warp % 4) in the upper half
+        float m = kNoMax;
+        bool nan[2] = {false, false}, ok = true;
+        for (int j = 0; j < n; ++j) {
+            const int p0 = (step0 + j) * kStep, buf = j & 1;
+            if (!wait(&s.s_full[tile][buf], j >> 1) || !wait(&s.kv_full[j % kPreStages], j / kPreStages)) { ok = false; break; }
+            sm100::tc_fence_after();
+            const PrefillInfo& info = s.info[j % kPreInfo];
+            uint32_t x[64];
+            tmem_load32(lanes + col_s(tile, buf), x);
+            tmem_load32(lanes + col_s(tile, buf) + 32, x + 32);
+            tmem_wait_load();
+            if (info.missing || p0 + kStep - 1 > hi || p0 <= lo) {  // not every position is seen
+                const uint32_t missing = info.missing;
+#pragma unroll
+                for (int i = 0; i < 64; ++i)
+                    if (p0 + i > hi || p0 + i <= lo || ((missing >> (i / P)) & 1)) x[i] = 0xff800000u;
+            }
+            if (info.special)
+#pragma unroll
+                for (int b = 0; b < 2; ++b)
+                    for (int h = 0; h < 2; ++h)
+                        for (uint32_t bad = info.nan[b][h]; bad; bad &= bad - 1) {
+                            const int pos = p0 + 32 * h + __ffs(bad) - 1;
+                            nan[b] = nan[b] || (pos <= hi && pos > lo);
+                        }
+            float top = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 64; ++i) top = fmaxf(top, __uint_as_float(x[i]));
+            top *= qs;
+            const bool raise = top > m + (j == 0 ? 0.f : 8.f);
+            if (__any_sync(0xffffffffu, raise)) {
+                const float now = raise ? top : m, f = ex2(m - now);
+                m = now;
+                if (j > 0) {
+                    if (!wait(&s.pv_done[tile], j - 1)) { ok = false; break; }
+                    sm100::tc_fence_after();
+#pragma unroll 1
+                    for (int c = 0; c < kPreN; c += 16) {
+                        uint32_t o[16];
+                        tmem_load16(lanes + col_o(tile) + c, o);
+                        tmem_wait_load();
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                        tmem_store16(lanes + col_o(tile) + c, o);
+                    }
+                    tmem_wait_store();
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 64; ++i) x[i] = __float_as_uint(ex2(fmaf(__uint_as_float(x[i]), qs, -m)));
+            tmem_store32(lanes + col_s(tile, buf), x);
+            tmem_store32(lanes + col_s(tile, buf) + 32, x + 32);
+            tmem_wait_store();
+            sm100::tc_fence_before();
+            sm100::mbar_arrive(&s.p_full[tile][buf]);
+        }
+        // (a phase can only be waited for once the one before it is known to be over: that of step n - 3 is, as the last scores
+        // were issued behind it)
+        if (ok && (n < 2 || wait(&s.pv_done[tile], n - 2)) && wait(&s.pv_done[tile], n - 1)) {
+            sm100::tc_fence_after();
+            uint32_t sum[16];
+            tmem_load16(lanes + col_o(tile) + 64, sum);
+            tmem_wait_load();
+            const float inv = inverse(__uint_as_float(sum[0]) + sink_of(p, head, m));
+#pragma unroll
+            for (int c = 0; c < 64; c += 16) {
+                uint32_t o[16];
+                tmem_load16(lanes + col_o(tile) + c, o);
+                tmem_wait_load();
+                if (tid < rows) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        float y[8];
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) y[i] = nan[c / 32] ? __uint_as_float(0x7fc00000u) : __uint_as_float(o[8 * h + i]) * inv;
+                        store_out(p, ((long long)(q.row0 + token) * p.s.nq + head) * D + c + 8 * h, y);
+                    }
+                }
+            }
+        }
+    } else if (n > 0 && warp < kPreSoftmaxWarps + kPreUnpackWarps) {
+        // ---- copies and unpacking ------------------------------------------------------------------------------------------
+        const int t = tid - kPreSoftmaxWarps * 32;
+        int id_base = -64, ids = -1;
+        auto fetch = [&](int j) {  // by the first of these warps
+            const int page = (step0 + j) * kPages, stage = j % kPreRaw;
+            if ((uint32_t)(page - id_base) >= 32u) {
+                id_base = page;
+                ids = -1;
+                if ((page + lane) * P < q.len) {
+                    ids = p.b.table[seq * p.b.table_stride + page + lane];
+                    if (ids < 0 || ids >= p.b.n_pages) {
+                        report(p.b.status, NEON_KV4_BAD_PAGE);
+                        ids = -1;
+                    }
+                }
+            }
+            const int id = __shfl_sync(0xffffffffu, ids, page - id_base + (lane & (kPages - 1)));
+            const uint32_t there = __ballot_sync(0xffffffffu, id >= 0) & ((1u << kPages) - 1);
+            if (lane == 0) {
+                s.info[j % kPreInfo].missing = there ^ ((1u << kPages) - 1);
+                s.info[j % kPreInfo].special = 0;
+                sm100::mbar_expect_tx(&s.raw_full[stage], __popc(there) * kRec);
+            }
+            if (lane < 4) s.info[j % kPreInfo].nan[lane / 2][lane % 2] = 0;
+            __syncwarp();
+            if (lane < kPages && id >= 0)
+                sm100::bulk_load(s.raw[stage] + lane * kRec, p.cache + ((long long)id * p.s.nkv + kvh) * kRec, kRec, &s.raw_full[stage]);
+        };
+        if (t < 32)
+            for (int j = 0; j < min(n, kPreRaw); ++j) fetch(j);
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+        int fetched = min(n, kPreRaw);
+        for (int j = 0; j < n; ++j) {
+            const int stage = j % kPreStages, p0 = (step0 + j) * kStep;
+            const bool ok = wait(&s.raw_full[j % kPreRaw], j / kPreRaw) && (j < kPreStages || wait(&s.kv_empty[stage], j / kPreStages - 1));
+            const unsigned char* raw = s.raw[j % kPreRaw];
+            PrefillInfo& info = s.info[j % kPreInfo];
+            const uint32_t missing = info.missing;
+            if (ok) {   // keys: a position and half of its columns a thread
+                const int pos = t & 63, b = t >> 6, pg = pos / P;
+                const bool live = !((missing >> pg) & 1) && p0 + pos < q.len;
+                const unsigned char* rec = raw + pg * kRec;
+                const int byte = live ? rec[2 * kCodes + pos % P * 2 + b] : 0;
+                const float scale = byte == 255 ? __uint_as_float(0x7fc00000u) : live ? pow2i(min(byte, kPreValueScale) - 127) : 0.f;
+                const uint4 w = live ? *reinterpret_cast<const uint4*>(rec + pos % P * (D / 2) + b * 16) : make_uint4(0u, 0u, 0u, 0u);
+                const uint32_t word[4] = {w.x, w.y, w.z, w.w};
+                unsigned char* row = s.k[stage][b] + pos * 128;
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    float x[8];
+                    codes_to_f32(word[c], scale, x);
+                    *reinterpret_cast<float4*>(row + (((2 * c) ^ (pos & 7)) * 16)) = make_float4(x[0], x[1], x[2], x[3]);
+                    *reinterpret_cast<float4*>(row + (((2 * c + 1) ^ (pos & 7)) * 16)) = make_float4(x[4], x[5], x[6], x[7]);
+                }
+            }
+            if (ok) {   // values: four positions and eight columns a thread
+                const int group = (t & 7) + (t >> 6) * 8, word = (t >> 3) & 7, b = word >> 2;
+                float x[4][8];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int pos = group * 4 + i, pg = pos / P;
+                    const bool live = !((missing >> pg) & 1) && p0 + pos < q.len;
+                    const unsigned char* rec = raw + pg * kRec;
+                    const int byte = live ? rec[2 * kCodes + kScales + pos % P * 2 + b] : 0;
+                    if (byte == 255 && (word & 3) == 0) {
+                        atomicOr(&info.special, 1u);
+                        atomicOr(&info.nan[b][pos / 32], 1u << (pos % 32));
+                    }
+                    const float scale = !live || byte == 255 ? 0.f : pow2i(min(byte, kPreValueScale) - 127);
+                    codes_to_f32(live ? *reinterpret_cast<const uint32_t*>(rec + kCodes + pos % P * (D / 2) + word * 4) : 0u, scale, x[i]);
+                }
+                unsigned char* base = s.v[stage][group >> 3] + word * 8 * 128;
+#pragma unroll
+                for (int c = 0; c < 8; ++c)
+                    *reinterpret_cast<float4*>(base + c * 128 + (((group & 7) ^ c) * 16)) = make_float4(x[0][c], x[1][c], x[2][c], x[3][c]);
+            }
+            sm100::fence_proxy_async();
+            if (ok) sm100::mbar_arrive(&s.kv_full[stage]);
+            // the record is read; the four warps go on or give up as one
+            uint32_t all;
+            asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.and.pred q, 1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+                         : "=r"(all) : "r"((uint32_t)ok) : "memory");
+            if (!all) break;
+            if (t < 32 && j + kPreRaw < n) {
+                fetch(j + kPreRaw);
+                fetched = j + kPreRaw + 1;
+            }
+        }
+        if (s.abort && t < 32)  // no copy may land after the CTA is gone
+            for (int j = max(0, fetched - kPreRaw); j < fetched; ++j) wait_bounded(&s.raw_full[j % kPreRaw], (j / kPreRaw) & 1);
+    } else if (n > 0 && warp == kPreWarps - 1) {
+        // ---- products ------------------------------------------------------------------------------------------------------
+        const uint32_t idesc = (1u << 4) | (2u << 7) | (2u << 10) | ((128u >> 4) << 24);  // f32 += tf32 * tf32, 128 rows, both K-major
+        const uint32_t idesc_s = idesc | ((kStep / 8) << 17), idesc_o = idesc | ((kPreN / 8) << 17);
+        const bool issue = sm100::elect_one();
+        auto scores = [&](int j) {
+            const int stage = j % kPreStages;
+            for (int x = 0; x < 2; ++x) {
+                if (issue) {
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        const uint32_t a = sm100::smem_u32(s.q[k / 4]) + x * 128 * 128 + k % 4 * 32, b = sm100::smem_u32(s.k[stage][k / 4]) + k % 4 * 32;
+                        mma_tf32_ss(tmem + col_s(x, j & 1), sm100::make_sw128_desc(a), sm100::make_sw128_desc(b), idesc_s, k > 0);
+                    }
+                    sm100::tc_commit(&s.s_full[x][j & 1]);
+                }
+                __syncwarp();
+            }
+        };
+        bool ok = wait(&s.kv_full[0], 0);
+        sm100::tc_fence_after();
+        if (ok) scores(0);
+        for (int j = 0; j < n && ok; ++j) {
+            const int stage = j % kPreStages;
+            if (j + 1 < n) {
+                ok = wait(&s.kv_full[(j + 1) % kPreStages], (j + 1) / kPreStages);
+                if (!ok) break;
+                sm100::tc_fence_after();
+                scores(j + 1);
+            }
+            for (int x = 0; x < 2 && ok; ++x) {
+                ok = wait(&s.p_full[x][j & 1], j >> 1);
+                if (!ok) break;
+                sm100::tc_fence_after();
+                if (issue) {
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        const uint32_t b = sm100::smem_u32(s.v[stage][k / 4]) + k % 4 * 32;
+                        mma_tf32_ts(tmem + col_o(x), tmem + col_s(x, j & 1) + k * 8, sm100::make_sw128_desc(b), idesc_o, j > 0 || k > 0);
+                    }
+                    sm100::tc_commit(&s.pv_done[x]);
+                    if (x == 1) sm100::tc_commit(&s.kv_empty[stage]);
+                }
+                __syncwarp();
+            }
+        }
+        if (!ok) {  // what was issued has to end before tensor memory is given back
+            if (issue) sm100::tc_commit(&s.drained);
+            __syncwarp();
+            wait_bounded(&s.drained, 0);
+        }
+    }
+    if (n == 0 && tid < rows)
+        for (int c = 0; c < D; c += 8) {
+            const float zero[8] = {};
+            store_out(p, ((long long)(q.row0 + token) * p.s.nq + head) * D + c, zero);
+        }
+    sm100::tc_fence_before();
+    __syncthreads();
+    if (warp == kPreWarps - 1) sm100::tmem_dealloc(tmem, 512);
+}
+
+}  // namespace kv4
+}  // namespace neon

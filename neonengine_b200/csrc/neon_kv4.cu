@@ -12,6 +12,7 @@
 
 #include "kv4_append.cuh"
 #include "kv4_attend.cuh"
+#include "kv4_prefill.cuh"
 #include "kv4_launch.h"
 
 using namespace neon;
@@ -128,6 +129,20 @@ cudaError_t attend_variant(const AttendParams* run, cudaStream_t st) {
     with_pdl(merge_kernel<DIM>, (unsigned)((tasks + 7) / 8), 256, plan, st, p);
     return cudaSuccess;
 }
+// Chunks of prompts: 256 rows of a key/value head at a time on tcgen05.  Heads of 64 only: at 128 columns queries, operands
+// and outputs would not fit a CTA.
+constexpr int kPrefillRows = 64;  // rows a sequence from which it is faster (see kv4_prefill.cuh)
+bool prefills(const Shape& s, int max_rows) { return s.D == 64 && (long long)max_rows * (s.nq / s.nkv) >= kPrefillRows; }
+
+template <int PAGE>
+cudaError_t prefill_variant(const AttendParams* run, cudaStream_t st) {
+    constexpr int kSmem = sizeof(PrefillSmem) + 1024;
+    if (!run) return cudaFuncSetAttribute(prefill_kernel<PAGE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    const long long tiles = (long long)run->b.rows * run->G / kPreRows + run->b.n;  // as many as there can be
+    prefill_kernel<PAGE><<<(unsigned)(tiles * run->s.nkv), kPreWarps * 32, kSmem, st>>>(*run);
+    return cudaSuccess;
+}
+
 // Calls f with every variant that there is; the one of a shape and a number of column groups.
 template <class F>
 cudaError_t each_variant(const F& f) {
@@ -147,11 +162,15 @@ cudaError_t configure_attend() {
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess || done[dev & 63]) return e;
     e = each_variant([](int, int, int, auto variant) { return variant(nullptr, nullptr); });
+    if (e == cudaSuccess) e = prefill_variant<16>(nullptr, nullptr);
+    if (e == cudaSuccess) e = prefill_variant<32>(nullptr, nullptr);
+    if (e == cudaSuccess) e = prefill_variant<64>(nullptr, nullptr);
     if (e == cudaSuccess) done[dev & 63] = true;
     return e;
 }
 
 uint64_t attend_workspace(const Shape& s, const Batch& b, int max_rows) {
+    if (prefills(s, max_rows)) return 16;
     const int nt = column_groups(s, max_rows);
     return (uint64_t)attend_grid(s, b, nt) * (2 + kAttendWarps) * 8 * nt * (s.D + 2) * sizeof(float);
 }
@@ -165,6 +184,12 @@ int launch_attend(const Shape& s, const Batch& b, const uint8_t* cache, int dtyp
     p.grid = attend_grid(s, b, nt);
     p.R = 8 * nt;
     p.G_inverse = (uint32_t)((0x100000000ull + p.G - 1) / p.G);
+    if (prefills(s, max_rows)) {
+        if (s.P == 16) prefill_variant<16>(&p, st);
+        else if (s.P == 32) prefill_variant<32>(&p, st);
+        else prefill_variant<64>(&p, st);
+        return 1;
+    }
     each_variant([&](int dim, int page, int groups, auto variant) {
         return dim == s.D && page == s.P && groups == nt ? variant(&p, st) : cudaSuccess;
     });
