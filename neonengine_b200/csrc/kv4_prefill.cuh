@@ -2,8 +2,8 @@
 //
 // An item is (sequence, key/value head, 256 rows: 32 tokens at eight query heads a key/value head), as two tiles of 128 rows.  Per
 // step of 64 positions:
-//   copies    a bulk copy per page brings the record (codes and scales) into shared memory, four steps ahead;
-//   unpacking four warps turn it into two tf32 operands: keys [64 positions][64], values transposed [64 + 16][64 positions], whose
+//   copies    a warp brings each step's records (codes and scales) into shared memory, a bulk copy per page, four steps ahead;
+//   unpacking four warps make two tf32 operands of them: keys [64 positions][64], values transposed [64 + 16][64 positions], whose
 //             row 64 is ones, so that the softmax sum is one more column of the output;
 //   products  one thread issues S = Q K^T (f32 in tensor memory, two buffers a tile) and O += P V with P read from tensor memory;
 //   softmax   two groups of four warps, one per tile, a row a thread: no exchange between threads.  P takes the place of S.
@@ -20,7 +20,8 @@ namespace neon {
 namespace kv4 {
 
 constexpr int kPreRows = 256, kPreStages = 3, kPreRaw = 4, kPreInfo = 8, kPreN = 80;
-constexpr int kPreSoftmaxWarps = 8, kPreUnpackWarps = 4, kPreWarps = kPreSoftmaxWarps + kPreUnpackWarps + 1;
+constexpr int kPreSoftmaxWarps = 8, kPreUnpackWarps = 4, kPreWarps = kPreSoftmaxWarps + kPreUnpackWarps + 2;
+constexpr int kPreMmaWarp = kPreWarps - 2, kPreCopyWarp = kPreWarps - 1;
 constexpr int kPreValueScale = 252;  // value (and key) scales above 2^125 count as 2^125: what a row does not see is finite
 
 struct PrefillInfo {     // of a step
@@ -35,7 +36,7 @@ struct PrefillSmem {
     unsigned char v[kPreStages][2][kPreN * 128];      // [half of the positions][column][32 f32]
     unsigned char raw[kPreRaw][kStep * (64 + 4)];
     PrefillInfo info[kPreInfo];
-    uint64_t raw_full[kPreRaw], kv_full[kPreStages], kv_empty[kPreStages], s_full[2][2], p_full[2][2], pv_done[2], drained;
+    uint64_t raw_full[kPreRaw], raw_empty[kPreRaw], kv_full[kPreStages], kv_empty[kPreStages], s_full[2][2], p_full[2][2], pv_done[2], drained;
     uint32_t tmem;
     int abort, item[4];
 };
@@ -100,7 +101,7 @@ template <int P>
 __global__ void __launch_bounds__(kPreWarps * 32, 1) prefill_kernel(const AttendParams p) {
     constexpr int D = 64, kPages = kStep / P, kRec = P * (D + D / 16), kCodes = P * D / 2, kScales = P * D / 32;
     extern __shared__ unsigned char unaligned[];
-    PrefillSmem& s = *reinterpret_cast<PrefillSmem*>((reinterpret_cast<uintptr_t>(unaligned) + 1023) & ~(uintptr_t)1023);
+    PrefillSmem& s = *reinterpret_cast<PrefillSmem*>(unaligned + (-sm100::smem_u32(unaligned) & 1023));
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     // ---- the item: the last tiles, which see the most, first --------------------------------------------------------------
     const int kvh = blockIdx.x % p.s.nkv, order = blockIdx.x / p.s.nkv;
@@ -136,9 +137,12 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1) prefill_kernel(const Attend
         }
     }
     if (tid == 0) {
-        for (int i = 0; i < kPreRaw; ++i) sm100::mbar_init(&s.raw_full[i], 1);
+        for (int i = 0; i < kPreRaw; ++i) {
+            sm100::mbar_init(&s.raw_full[i], 1);
+            sm100::mbar_init(&s.raw_empty[i], 128);
+        }
         for (int i = 0; i < kPreStages; ++i) {
-            sm100::mbar_init(&s.kv_full[i], kPreUnpackWarps * 32);
+            sm100::mbar_init(&s.kv_full[i], 128);
             sm100::mbar_init(&s.kv_empty[i], 1);
         }
         for (int i = 0; i < 4; ++i) {
@@ -183,7 +187,7 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1) prefill_kernel(const Attend
             *reinterpret_cast<float4*>(row + ((((c % 4) * 2 + 1) ^ (tid & 7)) * 16)) = make_float4(x[4], x[5], x[6], x[7]);
         }
     }
-    if (warp == kPreWarps - 1) sm100::tmem_alloc(&s.tmem, 512);
+    if (warp == kPreMmaWarp) sm100::tmem_alloc(&s.tmem, 512);
     sm100::fence_proxy_async();
     sm100::tc_fence_before();
     __syncthreads();
@@ -280,45 +284,16 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1) prefill_kernel(const Attend
             }
         }
     } else if (n > 0 && warp < kPreSoftmaxWarps + kPreUnpackWarps) {
-        // ---- copies and unpacking ------------------------------------------------------------------------------------------
-        const int t = tid - kPreSoftmaxWarps * 32;
-        int id_base = -64, ids = -1;
-        auto fetch = [&](int j) {  // by the first of these warps
-            const int page = (step0 + j) * kPages, stage = j % kPreRaw;
-            if ((uint32_t)(page - id_base) >= 32u) {
-                id_base = page;
-                ids = -1;
-                if ((page + lane) * P < q.len) {
-                    ids = p.b.table[seq * p.b.table_stride + page + lane];
-                    if (ids < 0 || ids >= p.b.n_pages) {
-                        report(p.b.status, NEON_KV4_BAD_PAGE);
-                        ids = -1;
-                    }
-                }
-            }
-            const int id = __shfl_sync(0xffffffffu, ids, page - id_base + (lane & (kPages - 1)));
-            const uint32_t there = __ballot_sync(0xffffffffu, id >= 0) & ((1u << kPages) - 1);
-            if (lane == 0) {
-                s.info[j % kPreInfo].missing = there ^ ((1u << kPages) - 1);
-                s.info[j % kPreInfo].special = 0;
-                sm100::mbar_expect_tx(&s.raw_full[stage], __popc(there) * kRec);
-            }
-            if (lane < 4) s.info[j % kPreInfo].nan[lane / 2][lane % 2] = 0;
-            __syncwarp();
-            if (lane < kPages && id >= 0)
-                sm100::bulk_load(s.raw[stage] + lane * kRec, p.cache + ((long long)id * p.s.nkv + kvh) * kRec, kRec, &s.raw_full[stage]);
-        };
-        if (t < 32)
-            for (int j = 0; j < min(n, kPreRaw); ++j) fetch(j);
-        asm volatile("bar.sync 1, 128;" ::: "memory");
-        int fetched = min(n, kPreRaw);
+        // ---- unpacking -------------------------------------------------------------------------------------------------------
+        const int t = tid & 127;
         for (int j = 0; j < n; ++j) {
             const int stage = j % kPreStages, p0 = (step0 + j) * kStep;
-            const bool ok = wait(&s.raw_full[j % kPreRaw], j / kPreRaw) && (j < kPreStages || wait(&s.kv_empty[stage], j / kPreStages - 1));
+            if (!wait(&s.raw_full[j % kPreRaw], j / kPreRaw)) break;
+            if (j >= kPreStages && !wait(&s.kv_empty[stage], j / kPreStages - 1)) break;
             const unsigned char* raw = s.raw[j % kPreRaw];
             PrefillInfo& info = s.info[j % kPreInfo];
             const uint32_t missing = info.missing;
-            if (ok) {   // keys: a position and half of its columns a thread
+            {   // keys: a position and half of its columns a thread
                 const int pos = t & 63, b = t >> 6, pg = pos / P;
                 const bool live = !((missing >> pg) & 1) && p0 + pos < q.len;
                 const unsigned char* rec = raw + pg * kRec;
@@ -335,7 +310,7 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1) prefill_kernel(const Attend
                     *reinterpret_cast<float4*>(row + (((2 * c + 1) ^ (pos & 7)) * 16)) = make_float4(x[4], x[5], x[6], x[7]);
                 }
             }
-            if (ok) {   // values: four positions and eight columns a thread
+            {   // values: four positions and eight columns a thread
                 const int group = (t & 7) + (t >> 6) * 8, word = (t >> 3) & 7, b = word >> 2;
                 float x[4][8];
 #pragma unroll
@@ -356,21 +331,44 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1) prefill_kernel(const Attend
                 for (int c = 0; c < 8; ++c)
                     *reinterpret_cast<float4*>(base + c * 128 + (((group & 7) ^ c) * 16)) = make_float4(x[0][c], x[1][c], x[2][c], x[3][c]);
             }
+            sm100::mbar_arrive(&s.raw_empty[j % kPreRaw]);
             sm100::fence_proxy_async();
-            if (ok) sm100::mbar_arrive(&s.kv_full[stage]);
-            // the record is read; the four warps go on or give up as one
-            uint32_t all;
-            asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.and.pred q, 1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
-                         : "=r"(all) : "r"((uint32_t)ok) : "memory");
-            if (!all) break;
-            if (t < 32 && j + kPreRaw < n) {
-                fetch(j + kPreRaw);
-                fetched = j + kPreRaw + 1;
-            }
+            sm100::mbar_arrive(&s.kv_full[stage]);
         }
-        if (s.abort && t < 32)  // no copy may land after the CTA is gone
+    } else if (n > 0 && warp == kPreCopyWarp) {
+        // ---- copies ----------------------------------------------------------------------------------------------------------
+        int id_base = -64, ids = -1, fetched = 0;
+        for (int j = 0; j < n; ++j, ++fetched) {
+            const int page = (step0 + j) * kPages, stage = j % kPreRaw;
+            if ((uint32_t)(page - id_base) >= 32u) {
+                id_base = page;
+                ids = -1;
+                if ((page + lane) * P < q.len) {
+                    ids = p.b.table[seq * p.b.table_stride + page + lane];
+                    if (ids < 0 || ids >= p.b.n_pages) {
+                        report(p.b.status, NEON_KV4_BAD_PAGE);
+                        ids = -1;
+                    }
+                }
+            }
+            const int id = __shfl_sync(0xffffffffu, ids, page - id_base + (lane & (kPages - 1)));
+            const uint32_t there = __ballot_sync(0xffffffffu, id >= 0) & ((1u << kPages) - 1);
+            if (j >= kPreRaw && !wait(&s.raw_empty[stage], j / kPreRaw - 1)) break;
+            PrefillInfo& info = s.info[j % kPreInfo];
+            if (lane < 4) info.nan[lane / 2][lane % 2] = 0;
+            __syncwarp();
+            if (lane == 0) {
+                info.missing = there ^ ((1u << kPages) - 1);
+                info.special = 0;
+                sm100::mbar_expect_tx(&s.raw_full[stage], __popc(there) * kRec);
+            }
+            __syncwarp();
+            if (lane < kPages && id >= 0)
+                sm100::bulk_load(s.raw[stage] + lane * kRec, p.cache + ((long long)id * p.s.nkv + kvh) * kRec, kRec, &s.raw_full[stage]);
+        }
+        if (*(volatile int*)&s.abort)  // no copy may land after the CTA is gone
             for (int j = max(0, fetched - kPreRaw); j < fetched; ++j) wait_bounded(&s.raw_full[j % kPreRaw], (j / kPreRaw) & 1);
-    } else if (n > 0 && warp == kPreWarps - 1) {
+    } else if (n > 0 && warp == kPreMmaWarp) {
         // ---- products ------------------------------------------------------------------------------------------------------
         const uint32_t idesc = (1u << 4) | (2u << 7) | (2u << 10) | ((128u >> 4) << 24);  // f32 += tf32 * tf32, 128 rows, both K-major
         const uint32_t idesc_s = idesc | ((kStep / 8) << 17), idesc_o = idesc | ((kPreN / 8) << 17);
@@ -429,7 +427,7 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1) prefill_kernel(const Attend
         }
     sm100::tc_fence_before();
     __syncthreads();
-    if (warp == kPreWarps - 1) sm100::tmem_dealloc(tmem, 512);
+    if (warp == kPreMmaWarp) sm100::tmem_dealloc(tmem, 512);
 }
 
 }  // namespace kv4
