@@ -3,23 +3,24 @@
 // An item is (sequence, key/value head, 256 rows: 32 tokens at eight query heads a key/value head), as two tiles of 128 rows.  Per
 // step of 64 positions:
 //   copies    a warp brings each step's records (codes and scales) into shared memory, a bulk copy per page, four steps ahead;
-//   unpacking four warps make two tf32 operands of them: keys [64 positions][64], values transposed [64 + 16][64 positions], whose
-//             row 64 is ones, so that the softmax sum is one more column of the output;
+//   unpacking four warps make two operands of them: bf16 keys [64 positions][64] and, transposed, tf32 values [64][64 positions];
 //   products  one thread issues S = Q K^T (f32 in tensor memory, two buffers a tile) and O += P V with P read from tensor memory;
 //   softmax   two groups of four warps, one per tile, a row a thread: no exchange between threads.  P takes the place of S.
-//             The output is rescaled (a trip through the registers) only when a row's maximum rises by 2^8.
-// tf32 holds bf16 and f16 queries, and codes times any E8M0 scale, exactly; probabilities are cut to 11 bits (a cut that the
-// sum, taken from the same operand, shares).  bf16 probabilities would be four times as coarse, f16 ones could not meet every
-// scale of values.
-// What bounds it: the special function units (16 exponentials a clock and SM: 1024 clocks a step) and, with tf32 at half the bf16
-// rate, the products (1152 clocks a step), which overlap.
+//             The output is rescaled (a trip through the registers) only when a step's probabilities, relative to the maximum so
+//             far, reach 2^8.
+// bf16 holds codes times any E8M0 scale exactly, and queries: f16 ones as the sum of two terms, with a product each.  The other
+// product is tf32 because probabilities need more than bf16's 8 bits and f16 could not meet every scale of values; they are cut to
+// tf32's 11 bits before they are summed, so that sum and output share the cut.
+// What bounds it: the special function units (16 exponentials a clock and SM: 1024 clocks a step); the products take 900
+// clocks a step (tf32 runs at half the bf16 rate, and 64 columns make operands' reads from shared memory count), the unpacking
+// 1100 of its warps.
 #pragma once
 #include "kv4_attend.cuh"
 
 namespace neon {
 namespace kv4 {
 
-constexpr int kPreRows = 256, kPreStages = 3, kPreRaw = 4, kPreInfo = 8, kPreN = 80;
+constexpr int kPreRows = 256, kPreStages = 3, kPreRaw = 4, kPreInfo = 8, kPreN = 64;
 constexpr int kPreSoftmaxWarps = 8, kPreUnpackWarps = 4, kPreWarps = kPreSoftmaxWarps + kPreUnpackWarps + 2;
 constexpr int kPreMmaWarp = kPreWarps - 2, kPreCopyWarp = kPreWarps - 1;
 constexpr int kPreValueScale = 252;  // value (and key) scales above 2^125 count as 2^125: what a row does not see is finite
@@ -31,8 +32,8 @@ struct PrefillInfo {     // of a step
 };
 
 struct PrefillSmem {
-    unsigned char q[2][kPreRows * 128];               // [half of the columns][row][32 f32], 128-byte swizzle
-    unsigned char k[kPreStages][2][kStep * 128];      // [half of the columns][position][32 f32]
+    unsigned char q[2][kPreRows * 128];               // [term][row][64 bf16], 128-byte swizzle
+    unsigned char k[kPreStages][kStep * 128];         // [position][64 bf16]
     unsigned char v[kPreStages][2][kPreN * 128];      // [half of the positions][column][32 f32]
     unsigned char raw[kPreRaw][kStep * (64 + 4)];
     PrefillInfo info[kPreInfo];
@@ -45,8 +46,8 @@ struct PrefillSmem {
 __device__ __forceinline__ uint32_t col_s(int x, int b) { return x * 128 + b * 64; }
 __device__ __forceinline__ uint32_t col_o(int x) { return 256 + x * kPreN; }
 
-__device__ __forceinline__ void mma_tf32_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::tf32 [%0], %1, %2, %3, p;\n\t}"
+__device__ __forceinline__ void mma_bf16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
                  ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
 }
 __device__ __forceinline__ void mma_tf32_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
@@ -154,11 +155,6 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1) prefill_kernel(const Attend
         sm100::fence_barrier_init();
     }
     if (tid < kPreInfo) s.info[tid] = {};
-    // the rows of ones and zeros behind the values
-    for (int i = tid; i < kPreStages * 2 * 16 * 32; i += kPreWarps * 32) {
-        const int at = i % 32, row = 64 + i / 32 % 16, half = i / 512 % 2, stage = i / 1024;
-        *reinterpret_cast<float*>(s.v[stage][half] + row * 128 + (((at / 4) ^ (row & 7)) * 16) + at % 4 * 4) = row == 64 ? 1.f : 0.f;
-    }
     __syncthreads();
     const int seq = s.item[0];
     if (seq < 0) return;
@@ -169,22 +165,25 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1) prefill_kernel(const Attend
     const int pos_lo = q.pos0 + p.token(r0), pos_hi = min(q.pos0 + p.token(r0 + rows - 1), q.len - 1);
     const int first = p.window > 0 ? max(pos_lo - p.window + 1, 0) : 0;
     const int step0 = first / kStep, n = pos_hi < first ? 0 : pos_hi / kStep + 1 - step0;
-    // ---- queries, as f32 --------------------------------------------------------------------------------------------------
+    // ---- queries, as bf16 terms -------------------------------------------------------------------------------------------
     const int tile = warp / 4;  // of a softmax warp
     const int rr = r0 + tid, token = p.token(min(rr, r0 + rows - 1)), head = kvh * p.G + min(rr, r0 + rows - 1) - token * p.G;
     if (tid < kPreRows) {
         const uint16_t* src = static_cast<const uint16_t*>(p.q) + (q.row0 + token) * p.q_stride + (long long)head * D;
-        const float sign = tid < rows ? (p.scale < 0.f ? -1.f : 1.f) : 0.f;
 #pragma unroll
         for (int c = 0; c < 8; ++c) {
-            float x[8];
+            float x[8], y[8];
             if (p.half) load8(reinterpret_cast<const __half*>(src) + c * 8, x);
             else load8(reinterpret_cast<const __nv_bfloat16*>(src) + c * 8, x);
+            const int at = tid * 128 + ((c ^ (tid & 7)) * 16);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = sign == 0.f ? 0.f : x[i] * sign;
-            unsigned char* row = s.q[c / 4] + tid * 128;
-            *reinterpret_cast<float4*>(row + ((((c % 4) * 2) ^ (tid & 7)) * 16)) = make_float4(x[0], x[1], x[2], x[3]);
-            *reinterpret_cast<float4*>(row + ((((c % 4) * 2 + 1) ^ (tid & 7)) * 16)) = make_float4(x[4], x[5], x[6], x[7]);
+            for (int i = 0; i < 8; ++i) {
+                x[i] = tid >= rows ? 0.f : p.scale < 0.f ? -x[i] : x[i];
+                y[i] = x[i] - __bfloat162float(__float2bfloat16_rn(x[i]));
+                if (x[i] - x[i] != 0.f) y[i] = 0.f;  // infinities have no second term
+            }
+            store8(reinterpret_cast<__nv_bfloat16*>(s.q[0] + at), x);
+            if (p.half) store8(reinterpret_cast<__nv_bfloat16*>(s.q[1] + at), y);
         }
     }
     if (warp == kPreMmaWarp) sm100::tmem_alloc(&s.tmem, 512);
@@ -203,23 +202,15 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1) prefill_kernel(const Attend
         const int hi = tid < rows ? min(q.pos0 + token, q.len - 1) : -1, lo = p.window > 0 ? q.pos0 + token - p.window : -1;
         const float positive = fabsf(p.scale) * kLog2e, qs = positive == 0.f ? 1e-30f : positive;
         const uint32_t lanes = tmem + ((uint32_t)(warp & 3) << 21);  // this warp's lanes: 32 * (warp % 4) in the upper half
-        float m = kNoMax;
+        float m = kNoMax, l[4] = {0.f, 0.f, 0.f, 0.f};
         bool nan[2] = {false, false}, ok = true;
         for (int j = 0; j < n; ++j) {
             const int p0 = (step0 + j) * kStep, buf = j & 1;
             if (!wait(&s.s_full[tile][buf], j >> 1) || !wait(&s.kv_full[j % kPreStages], j / kPreStages)) { ok = false; break; }
             sm100::tc_fence_after();
             const PrefillInfo& info = s.info[j % kPreInfo];
-            uint32_t x[64];
-            tmem_load32(lanes + col_s(tile, buf), x);
-            tmem_load32(lanes + col_s(tile, buf) + 32, x + 32);
-            tmem_wait_load();
-            if (info.missing || p0 + kStep - 1 > hi || p0 <= lo) {  // not every position is seen
-                const uint32_t missing = info.missing;
-#pragma unroll
-                for (int i = 0; i < 64; ++i)
-                    if (p0 + i > hi || p0 + i <= lo || ((missing >> (i / P)) & 1)) x[i] = 0xff800000u;
-            }
+            const uint32_t missing = info.missing;
+            const bool masked = missing || p0 + kStep - 1 > hi || p0 <= lo;  // not every position is seen
             if (info.special)
 #pragma unroll
                 for (int b = 0; b < 2; ++b)
@@ -228,14 +219,44 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1) prefill_kernel(const Attend
                             const int pos = p0 + 32 * h + __ffs(bad) - 1;
                             nan[b] = nan[b] || (pos <= hi && pos > lo);
                         }
-            float top = -INFINITY;
+            uint32_t x[64];
+            float sum[4], top;
+            auto hide = [&](int from) {
+                if (masked)
 #pragma unroll
-            for (int i = 0; i < 64; ++i) top = fmaxf(top, __uint_as_float(x[i]));
-            top *= qs;
-            const bool raise = top > m + (j == 0 ? 0.f : 8.f);
-            if (__any_sync(0xffffffffu, raise)) {
-                const float now = raise ? top : m, f = ex2(m - now);
+                    for (int i = 0; i < 32; ++i)
+                        if (p0 + from + i > hi || p0 + from + i <= lo || ((missing >> ((from + i) / P)) & 1)) x[from + i] = 0xff800000u;
+            };
+            auto weigh = [&](int from) {
+#pragma unroll
+                for (int i = from; i < from + 32; ++i) {
+                    x[i] = __float_as_uint(ex2(fmaf(__uint_as_float(x[i]), qs, -m))) & 0xffffe000u;  // tf32
+                    sum[i & 3] += __uint_as_float(x[i]);
+                }
+            };
+            // probabilities relative to the maximum so far, whose sum shows whether one is out of range
+            auto read = [&](bool weighing) {
+                tmem_load32(lanes + col_s(tile, buf), x);
+                tmem_wait_load();
+                tmem_load32(lanes + col_s(tile, buf) + 32, x + 32);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sum[i] = 0.f;
+                hide(0);
+                if (weighing) weigh(0);
+                tmem_wait_load();
+                hide(32);
+                if (weighing) weigh(32);
+            };
+            read(j > 0);
+            if (j == 0 || __any_sync(0xffffffffu, !((sum[0] + sum[1]) + (sum[2] + sum[3]) < 256.f))) {
+                if (j > 0) read(false);
+                top = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < 64; ++i) top = fmaxf(top, __uint_as_float(x[i]));
+                const float now = fmaxf(m, top * qs), f = ex2(m - now);
                 m = now;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) l[i] *= f;
                 if (j > 0) {
                     if (!wait(&s.pv_done[tile], j - 1)) { ok = false; break; }
                     sm100::tc_fence_after();
@@ -250,9 +271,13 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1) prefill_kernel(const Attend
                     }
                     tmem_wait_store();
                 }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sum[i] = 0.f;
+                weigh(0);
+                weigh(32);
             }
 #pragma unroll
-            for (int i = 0; i < 64; ++i) x[i] = __float_as_uint(ex2(fmaf(__uint_as_float(x[i]), qs, -m)));
+            for (int i = 0; i < 4; ++i) l[i] += sum[i];
             tmem_store32(lanes + col_s(tile, buf), x);
             tmem_store32(lanes + col_s(tile, buf) + 32, x + 32);
             tmem_wait_store();
@@ -263,10 +288,7 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1) prefill_kernel(const Attend
         // were issued behind it)
         if (ok && (n < 2 || wait(&s.pv_done[tile], n - 2)) && wait(&s.pv_done[tile], n - 1)) {
             sm100::tc_fence_after();
-            uint32_t sum[16];
-            tmem_load16(lanes + col_o(tile) + 64, sum);
-            tmem_wait_load();
-            const float inv = inverse(__uint_as_float(sum[0]) + sink_of(p, head, m));
+            const float inv = inverse((l[0] + l[1]) + (l[2] + l[3]) + sink_of(p, head, m));
 #pragma unroll
             for (int c = 0; c < 64; c += 16) {
                 uint32_t o[16];
@@ -293,45 +315,62 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1) prefill_kernel(const Attend
             const unsigned char* raw = s.raw[j % kPreRaw];
             PrefillInfo& info = s.info[j % kPreInfo];
             const uint32_t missing = info.missing;
-            {   // keys: a position and half of its columns a thread
-                const int pos = t & 63, b = t >> 6, pg = pos / P;
-                const bool live = !((missing >> pg) & 1) && p0 + pos < q.len;
-                const unsigned char* rec = raw + pg * kRec;
-                const int byte = live ? rec[2 * kCodes + pos % P * 2 + b] : 0;
-                const float scale = byte == 255 ? __uint_as_float(0x7fc00000u) : live ? pow2i(min(byte, kPreValueScale) - 127) : 0.f;
-                const uint4 w = live ? *reinterpret_cast<const uint4*>(rec + pos % P * (D / 2) + b * 16) : make_uint4(0u, 0u, 0u, 0u);
-                const uint32_t word[4] = {w.x, w.y, w.z, w.w};
-                unsigned char* row = s.k[stage][b] + pos * 128;
+            const bool whole = missing == 0 && p0 + kStep <= q.len;  // every position is there
+            // keys: a position and half of its columns a thread.  Values: four positions and eight columns a thread.
+            const int pos = t & 63, kb = t >> 6, group = (t & 7) + (t >> 6) * 8, word = (t >> 3) & 7, vb = word >> 2;
+            auto live = [&](int at) { return whole || (!((missing >> (at / P)) & 1) && p0 + at < q.len); };
+            const unsigned char *krec = raw + pos / P * kRec, *vrec = raw + group * 4 / P * kRec;  // (four positions lie in one page)
+            uint4 kw = *reinterpret_cast<const uint4*>(krec + pos % P * (D / 2) + kb * 16);
+            int kbyte = krec[2 * kCodes + pos % P * 2 + kb], vbyte[4];
+            uint32_t vw[4];
+            bool odd = false;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int at = (group * 4 + i) % P;
+                vw[i] = *reinterpret_cast<const uint32_t*>(vrec + kCodes + at * (D / 2) + word * 4);
+                vbyte[i] = vrec[2 * kCodes + kScales + at * 2 + vb];
+                odd = odd || vbyte[i] > kPreValueScale;
+            }
+            sm100::mbar_arrive(&s.raw_empty[j % kPreRaw]);
+            if (!whole) {
+                if (!live(pos)) { kw = make_uint4(0u, 0u, 0u, 0u); kbyte = 0; }
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (!live(group * 4 + i)) { vw[i] = 0u; vbyte[i] = 0; }
+            }
+            if (odd)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (vbyte[i] == 255) {
+                        if ((word & 3) == 0) {
+                            atomicOr(&info.special, 1u);
+                            atomicOr(&info.nan[vb][(group * 4 + i) / 32], 1u << ((group * 4 + i) % 32));
+                        }
+                        vbyte[i] = 0;
+                        vw[i] = 0;
+                    }
+                    vbyte[i] = min(vbyte[i], kPreValueScale);
+                }
+            {
+                const float scale = kbyte == 255 ? __uint_as_float(0x7fc00000u) : __uint_as_float((uint32_t)min(kbyte, kPreValueScale) << 23);
+                const uint32_t w[4] = {kw.x, kw.y, kw.z, kw.w};
+                unsigned char* row = s.k[stage] + pos * 128;
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
                     float x[8];
-                    codes_to_f32(word[c], scale, x);
-                    *reinterpret_cast<float4*>(row + (((2 * c) ^ (pos & 7)) * 16)) = make_float4(x[0], x[1], x[2], x[3]);
-                    *reinterpret_cast<float4*>(row + (((2 * c + 1) ^ (pos & 7)) * 16)) = make_float4(x[4], x[5], x[6], x[7]);
+                    codes_to_f32(w[c], scale, x);
+                    store8(reinterpret_cast<__nv_bfloat16*>(row + (((4 * kb + c) ^ (pos & 7)) * 16)), x);
                 }
             }
-            {   // values: four positions and eight columns a thread
-                const int group = (t & 7) + (t >> 6) * 8, word = (t >> 3) & 7, b = word >> 2;
+            {
                 float x[4][8];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int pos = group * 4 + i, pg = pos / P;
-                    const bool live = !((missing >> pg) & 1) && p0 + pos < q.len;
-                    const unsigned char* rec = raw + pg * kRec;
-                    const int byte = live ? rec[2 * kCodes + kScales + pos % P * 2 + b] : 0;
-                    if (byte == 255 && (word & 3) == 0) {
-                        atomicOr(&info.special, 1u);
-                        atomicOr(&info.nan[b][pos / 32], 1u << (pos % 32));
-                    }
-                    const float scale = !live || byte == 255 ? 0.f : pow2i(min(byte, kPreValueScale) - 127);
-                    codes_to_f32(live ? *reinterpret_cast<const uint32_t*>(rec + kCodes + pos % P * (D / 2) + word * 4) : 0u, scale, x[i]);
-                }
+                for (int i = 0; i < 4; ++i) codes_to_f32(vw[i], __uint_as_float((uint32_t)vbyte[i] << 23), x[i]);
                 unsigned char* base = s.v[stage][group >> 3] + word * 8 * 128;
 #pragma unroll
                 for (int c = 0; c < 8; ++c)
                     *reinterpret_cast<float4*>(base + c * 128 + (((group & 7) ^ c) * 16)) = make_float4(x[0][c], x[1][c], x[2][c], x[3][c]);
             }
-            sm100::mbar_arrive(&s.raw_empty[j % kPreRaw]);
             sm100::fence_proxy_async();
             sm100::mbar_arrive(&s.kv_full[stage]);
         }
@@ -370,18 +409,21 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1) prefill_kernel(const Attend
             for (int j = max(0, fetched - kPreRaw); j < fetched; ++j) wait_bounded(&s.raw_full[j % kPreRaw], (j / kPreRaw) & 1);
     } else if (n > 0 && warp == kPreMmaWarp) {
         // ---- products ------------------------------------------------------------------------------------------------------
-        const uint32_t idesc = (1u << 4) | (2u << 7) | (2u << 10) | ((128u >> 4) << 24);  // f32 += tf32 * tf32, 128 rows, both K-major
-        const uint32_t idesc_s = idesc | ((kStep / 8) << 17), idesc_o = idesc | ((kPreN / 8) << 17);
+        // f32 += bf16 * bf16 and f32 += tf32 * tf32; 128 rows, both operands K-major
+        const uint32_t idesc_s = (1u << 4) | (1u << 7) | (1u << 10) | ((kStep / 8) << 17) | ((128u >> 4) << 24);
+        const uint32_t idesc_o = (1u << 4) | (2u << 7) | (2u << 10) | ((kPreN / 8) << 17) | ((128u >> 4) << 24);
+        const int terms = p.half ? 2 : 1;
         const bool issue = sm100::elect_one();
         auto scores = [&](int j) {
             const int stage = j % kPreStages;
             for (int x = 0; x < 2; ++x) {
                 if (issue) {
+                    for (int term = 0; term < terms; ++term)
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) {
-                        const uint32_t a = sm100::smem_u32(s.q[k / 4]) + x * 128 * 128 + k % 4 * 32, b = sm100::smem_u32(s.k[stage][k / 4]) + k % 4 * 32;
-                        mma_tf32_ss(tmem + col_s(x, j & 1), sm100::make_sw128_desc(a), sm100::make_sw128_desc(b), idesc_s, k > 0);
-                    }
+                        for (int k = 0; k < 4; ++k) {
+                            const uint32_t a = sm100::smem_u32(s.q[term]) + x * 128 * 128 + k * 32, b = sm100::smem_u32(s.k[stage]) + k * 32;
+                            mma_bf16_ss(tmem + col_s(x, j & 1), sm100::make_sw128_desc(a), sm100::make_sw128_desc(b), idesc_s, term + k > 0);
+                        }
                     sm100::tc_commit(&s.s_full[x][j & 1]);
                 }
                 __syncwarp();
