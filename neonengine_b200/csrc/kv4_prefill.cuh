@@ -4,7 +4,8 @@
 // step of 64 positions:
 //   copies    a warp brings each step's records (codes and scales) into shared memory, a bulk copy per page, four steps ahead;
 //   unpacking four warps make two operands of them: bf16 keys [64 positions][64] and, transposed, tf32 values [64][64 positions];
-//   products  one thread issues S = Q K^T (f32 in tensor memory, two buffers a tile) and O += P V with P read from tensor memory;
+//   products  one thread issues S = Q K^T (f32 in tensor memory, two buffers a tile), another O += P V with P read from tensor
+//             memory: issuing takes as long as the products do, and neither waits behind the other's barriers;
 //   softmax   two groups of four warps, one per tile, a row a thread: no exchange between threads.  P takes the place of S.
 //             The output is rescaled (a trip through the registers) only when a step's probabilities, relative to the maximum so
 //             far, reach 2^8.
@@ -21,8 +22,8 @@ namespace neon {
 namespace kv4 {
 
 constexpr int kPreRows = 256, kPreStages = 3, kPreRaw = 4, kPreInfo = 8, kPreN = 64;
-constexpr int kPreSoftmaxWarps = 8, kPreUnpackWarps = 4, kPreWarps = kPreSoftmaxWarps + kPreUnpackWarps + 2;
-constexpr int kPreMmaWarp = kPreWarps - 2, kPreCopyWarp = kPreWarps - 1;
+constexpr int kPreSoftmaxWarps = 8, kPreUnpackWarps = 4, kPreWarps = kPreSoftmaxWarps + kPreUnpackWarps + 3;
+constexpr int kPreScoreWarp = kPreWarps - 3, kPreOutputWarp = kPreWarps - 2, kPreCopyWarp = kPreWarps - 1;
 constexpr int kPreValueScale = 252;  // value (and key) scales above 2^125 count as 2^125: what a row does not see is finite
 
 struct PrefillInfo {     // of a step
@@ -37,7 +38,7 @@ struct PrefillSmem {
     unsigned char v[kPreStages][2][kPreN * 128];      // [half of the positions][column][32 f32]
     unsigned char raw[kPreRaw][kStep * (64 + 4)];
     PrefillInfo info[kPreInfo];
-    uint64_t raw_full[kPreRaw], raw_empty[kPreRaw], kv_full[kPreStages], kv_empty[kPreStages], s_full[2][2], p_full[2][2], pv_done[2], drained;
+    uint64_t raw_full[kPreRaw], raw_empty[kPreRaw], kv_full[kPreStages], kv_empty[kPreStages], s_full[2][2], p_full[2][2], pv_done[2][2], drained[2];
     uint32_t tmem;
     int abort, item[4];
 };
@@ -85,6 +86,24 @@ __device__ __forceinline__ void tmem_store16(uint32_t addr, const uint32_t* r) {
 }
 __device__ __forceinline__ void tmem_wait_load() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Waits for a barrier's phase; false when that takes kWaitCycles, or when another wait of the CTA has already given up.  The
+// hardware parks the warp for up to 4 us a try: 14 warps that probe in a loop would take a third of the issue slots.
+__device__ __forceinline__ bool parked_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* status) {
+    const long long t0 = clock64();
+    while (true) {
+        uint32_t done;
+        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                     : "=r"(done) : "r"(sm100::smem_u32(bar)), "r"(parity), "r"(4000u) : "memory");
+        if (done) return true;
+        if (*abort_flag) return false;
+        if (clock64() - t0 > kWaitCycles) {
+            *abort_flag = 1;
+            report(status, NEON_KV4_TIMEOUT);
+            return false;
+        }
+    }
+}
 
 // 8 codes as f32, times a power of two
 __device__ __forceinline__ void codes_to_f32(uint32_t w, float scale, float (&x)[8]) {
@@ -150,8 +169,8 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1) prefill_kernel(const Attend
             sm100::mbar_init(&s.s_full[0][0] + i, 1);
             sm100::mbar_init(&s.p_full[0][0] + i, 128);
         }
-        for (int i = 0; i < 2; ++i) sm100::mbar_init(&s.pv_done[i], 1);
-        sm100::mbar_init(&s.drained, 1);
+        for (int i = 0; i < 4; ++i) sm100::mbar_init(&s.pv_done[0][0] + i, 1);
+        for (int i = 0; i < 2; ++i) sm100::mbar_init(&s.drained[i], 1);
         sm100::fence_barrier_init();
     }
     if (tid < kPreInfo) s.info[tid] = {};
@@ -186,15 +205,18 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1) prefill_kernel(const Attend
             if (p.half) store8(reinterpret_cast<__nv_bfloat16*>(s.q[1] + at), y);
         }
     }
-    if (warp == kPreMmaWarp) sm100::tmem_alloc(&s.tmem, 512);
+    if (warp == kPreScoreWarp) sm100::tmem_alloc(&s.tmem, 512);
     sm100::fence_proxy_async();
     sm100::tc_fence_before();
     __syncthreads();
     sm100::tc_fence_after();
     const uint32_t tmem = s.tmem;
-    // by a whole warp, which goes on or gives up as one; when a wait runs out, all others are called off
+    // By a whole warp, which goes on or gives up as one; when a wait runs out, all others are called off.  A phase is told from the
+    // one before by a bit, so every wait here is such that the phase before is known to be over and the one after cannot be
+    // before this warp has gone on: barriers are one per buffer.
     auto wait = [&](uint64_t* bar, uint32_t parity) {
-        return (bool)__all_sync(0xffffffffu, sm100::mbar_wait(bar, parity & 1, &s.abort, p.b.status, NEON_KV4_TIMEOUT, kWaitCycles));
+        if (__all_sync(0xffffffffu, sm100::mbar_peek(bar, parity & 1))) return true;  // (a try that may park costs 200 clocks even then)
+        return (bool)__all_sync(0xffffffffu, parked_wait(bar, parity & 1, &s.abort, p.b.status));
     };
 
     if (n > 0 && warp < kPreSoftmaxWarps) {
@@ -258,7 +280,7 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1) prefill_kernel(const Attend
 #pragma unroll
                 for (int i = 0; i < 4; ++i) l[i] *= f;
                 if (j > 0) {
-                    if (!wait(&s.pv_done[tile], j - 1)) { ok = false; break; }
+                    if (!wait(&s.pv_done[tile][buf ^ 1], (j - 1) >> 1)) { ok = false; break; }
                     sm100::tc_fence_after();
 #pragma unroll 1
                     for (int c = 0; c < kPreN; c += 16) {
@@ -284,9 +306,7 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1) prefill_kernel(const Attend
             sm100::tc_fence_before();
             sm100::mbar_arrive(&s.p_full[tile][buf]);
         }
-        // (a phase can only be waited for once the one before it is known to be over: that of step n - 3 is, as the last scores
-        // were issued behind it)
-        if (ok && (n < 2 || wait(&s.pv_done[tile], n - 2)) && wait(&s.pv_done[tile], n - 1)) {
+        if (ok && wait(&s.pv_done[tile][(n - 1) & 1], (n - 1) >> 1)) {
             sm100::tc_fence_after();
             const float inv = inverse((l[0] + l[1]) + (l[2] + l[3]) + sink_of(p, head, m));
 #pragma unroll
@@ -407,59 +427,68 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1) prefill_kernel(const Attend
         }
         if (*(volatile int*)&s.abort)  // no copy may land after the CTA is gone
             for (int j = max(0, fetched - kPreRaw); j < fetched; ++j) wait_bounded(&s.raw_full[j % kPreRaw], (j / kPreRaw) & 1);
-    } else if (n > 0 && warp == kPreMmaWarp) {
-        // ---- products ------------------------------------------------------------------------------------------------------
-        // f32 += bf16 * bf16 and f32 += tf32 * tf32; 128 rows, both operands K-major
-        const uint32_t idesc_s = (1u << 4) | (1u << 7) | (1u << 10) | ((kStep / 8) << 17) | ((128u >> 4) << 24);
-        const uint32_t idesc_o = (1u << 4) | (2u << 7) | (2u << 10) | ((kPreN / 8) << 17) | ((128u >> 4) << 24);
-        const int terms = p.half ? 2 : 1;
+    } else if (n > 0 && warp == kPreScoreWarp) {
+        // ---- scores ----------------------------------------------------------------------------------------------------------
+        // f32 += bf16 * bf16; 128 rows, both operands K-major.  Descriptors differ by their start addresses (in 16 bytes) alone:
+        // 2 for a k-step, a tile, a stage.
+        const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((kStep / 8) << 17) | ((128u >> 4) << 24);
+        const uint64_t dq = sm100::make_sw128_desc(sm100::smem_u32(s.q[0])), dk = sm100::make_sw128_desc(sm100::smem_u32(s.k[0]));
+        constexpr uint32_t kTerm = kPreRows * 128 / 16, kTile = 128 * 128 / 16, kStageK = kStep * 128 / 16;
         const bool issue = sm100::elect_one();
-        auto scores = [&](int j) {
-            const int stage = j % kPreStages;
-            for (int x = 0; x < 2; ++x) {
-                if (issue) {
-                    for (int term = 0; term < terms; ++term)
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            const uint32_t a = sm100::smem_u32(s.q[term]) + x * 128 * 128 + k * 32, b = sm100::smem_u32(s.k[stage]) + k * 32;
-                            mma_bf16_ss(tmem + col_s(x, j & 1), sm100::make_sw128_desc(a), sm100::make_sw128_desc(b), idesc_s, term + k > 0);
-                        }
-                    sm100::tc_commit(&s.s_full[x][j & 1]);
-                }
-                __syncwarp();
-            }
-        };
-        bool ok = wait(&s.kv_full[0], 0);
-        sm100::tc_fence_after();
-        if (ok) scores(0);
+        bool ok = true;
         for (int j = 0; j < n && ok; ++j) {
-            const int stage = j % kPreStages;
-            if (j + 1 < n) {
-                ok = wait(&s.kv_full[(j + 1) % kPreStages], (j + 1) / kPreStages);
-                if (!ok) break;
-                sm100::tc_fence_after();
-                scores(j + 1);
-            }
+            ok = wait(&s.kv_full[j % kPreStages], j / kPreStages);
             for (int x = 0; x < 2 && ok; ++x) {
-                ok = wait(&s.p_full[x][j & 1], j >> 1);
+                if (j >= 2) ok = wait(&s.pv_done[x][j & 1], (j - 2) >> 1);  // the probabilities of step j - 2 lie where these scores go
                 if (!ok) break;
                 sm100::tc_fence_after();
                 if (issue) {
+                    const uint64_t a = dq + x * kTile, b = dk + (uint32_t)(j % kPreStages) * kStageK;
+                    const uint32_t d = tmem + col_s(x, j & 1);
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) {
-                        const uint32_t b = sm100::smem_u32(s.v[stage][k / 4]) + k % 4 * 32;
-                        mma_tf32_ts(tmem + col_o(x), tmem + col_s(x, j & 1) + k * 8, sm100::make_sw128_desc(b), idesc_o, j > 0 || k > 0);
-                    }
-                    sm100::tc_commit(&s.pv_done[x]);
-                    if (x == 1) sm100::tc_commit(&s.kv_empty[stage]);
+                    for (int k = 0; k < 4; ++k) mma_bf16_ss(d, a + 2 * k, b + 2 * k, idesc, k > 0);
+                    if (p.half)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) mma_bf16_ss(d, a + kTerm + 2 * k, b + 2 * k, idesc, 1);
+                    sm100::tc_commit(&s.s_full[x][j & 1]);
                 }
                 __syncwarp();
             }
         }
         if (!ok) {  // what was issued has to end before tensor memory is given back
-            if (issue) sm100::tc_commit(&s.drained);
+            if (issue) sm100::tc_commit(&s.drained[0]);
             __syncwarp();
-            wait_bounded(&s.drained, 0);
+            wait_bounded(&s.drained[0], 0);
+        }
+    } else if (n > 0 && warp == kPreOutputWarp) {
+        // ---- outputs: f32 += tf32 * tf32 -----------------------------------------------------------------------------------------
+        const uint32_t idesc = (1u << 4) | (2u << 7) | (2u << 10) | ((kPreN / 8) << 17) | ((128u >> 4) << 24);
+        const uint64_t dv = sm100::make_sw128_desc(sm100::smem_u32(s.v[0][0]));
+        constexpr uint32_t kHalfV = kPreN * 128 / 16;
+        const bool issue = sm100::elect_one();
+        bool ok = true;
+        for (int j = 0; j < n && ok; ++j) {
+            const int stage = j % kPreStages;
+            ok = wait(&s.kv_full[stage], j / kPreStages);
+            for (int x = 0; x < 2 && ok; ++x) {
+                ok = wait(&s.p_full[x][j & 1], j >> 1);
+                if (!ok) break;
+                sm100::tc_fence_after();
+                if (issue) {
+                    const uint64_t b = dv + (uint32_t)stage * (2 * kHalfV);
+                    const uint32_t d = tmem + col_o(x), a = tmem + col_s(x, j & 1);
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) mma_tf32_ts(d, a + k * 8, b + k / 4 * kHalfV + k % 4 * 2, idesc, j > 0 || k > 0);
+                    sm100::tc_commit(&s.pv_done[x][j & 1]);
+                    if (x == 1) sm100::tc_commit(&s.kv_empty[stage]);
+                }
+                __syncwarp();
+            }
+        }
+        if (!ok) {
+            if (issue) sm100::tc_commit(&s.drained[1]);
+            __syncwarp();
+            wait_bounded(&s.drained[1], 0);
         }
     }
     if (n == 0 && tid < rows)
@@ -469,7 +498,7 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1) prefill_kernel(const Attend
         }
     sm100::tc_fence_before();
     __syncthreads();
-    if (warp == kPreMmaWarp) sm100::tmem_dealloc(tmem, 512);
+    if (warp == kPreScoreWarp) sm100::tmem_dealloc(tmem, 512);
 }
 
 }  // namespace kv4
