@@ -13,7 +13,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 SO = os.path.join(HERE, "libneon_moe.so")
 APP = os.path.join(HERE, "moe_app")
-SOURCES = ["neon_moe.cu", "neon_decoder.cu", "neon_water.cu", "neon_svgf.cu", "neon_pt.cu", "neon_kv4.cu",
+SOURCES = ["neon_moe.cu", "neon_decoder.cu", "neon_water.cu", "neon_svgf.cu", "neon_pt.cu", "neon_kv4.cu", "neon_kv4_prefill.cu",
            "neon_sampler.cu"]
 # the water step reproduces the reference shader's float arithmetic bit for bit: no fused multiply-add there
 SOURCE_FLAGS = {"neon_water.cu": ["-fmad=false"], "neon_svgf.cu": ["-fmad=false"], "neon_pt.cu": ["-fmad=false"],

@@ -401,6 +401,7 @@ __global__ void __launch_bounds__(kAttendWarps * 32, (D == 64 && NT <= 2) ? 2 : 
                     if (__any_sync(0xffffffffu, below > (uint32_t)kSpread)) {  // (kSpread has all its bits set)
 #pragma unroll
                         for (int b = 0; b < NB; ++b) {
+                            for (int i = 0; i < 2; ++i) vb[b][i] = vb[b][i] > kTopScale && vb[b][i] < 255 ? kTopScale : vb[b][i];
                             int top = __reduce_max_sync(0xffffffffu, max(vb[b][0], vb[b][1]));
                             if (top == 255) {  // NaN blocks: no operand; the rows that see one become NaN
                                 for (int i = 0; i < 2; ++i) {
@@ -585,7 +586,8 @@ __global__ void __launch_bounds__(kAttendWarps * 32, (D == 64 && NT <= 2) ? 2 : 
                                             int e = ve[0];
 #pragma unroll
                                             for (int b = 1; b < NB; ++b) e = blk == b ? ve[b] : e;
-                                            const int byte = rp[2 * kCodes + kScales + (pos % P) * NB + blk];
+                                            const int held = rp[2 * kCodes + kScales + (pos % P) * NB + blk];
+                                            const int byte = held == 255 ? held : min(held, kTopScale);
                                             const float f = byte <= e ? pow2i(byte - e) : 0.f;  // above: seen by no row, or NaN
                                             uint32_t half2[4];
                                             codes_to_f16(*reinterpret_cast<const uint32_t*>(rp + kCodes + (pos % P) * (D / 2) + h * 32 + g * 4), half2);

@@ -11,6 +11,8 @@
 namespace neon {
 namespace kv4 {
 
+constexpr int kTopScale = 252;  // attention takes larger scales (of infinities alone: 2^125 holds the largest finite number) for 2^125
+
 struct Shape {
     int nq, nkv, D, P;
     __host__ __device__ int codes() const { return P * D / 2; }        // bytes of a record's key (or value) codes

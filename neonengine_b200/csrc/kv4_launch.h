@@ -1,4 +1,4 @@
-// What other parts of the library call of the 4-bit paged cache (neon_kv4.cu).
+// What the 4-bit paged cache's parts (neon_kv4.cu, neon_kv4_prefill.cu) call of one another, and the decoder of it.
 #pragma once
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -8,6 +8,11 @@ namespace kv4 {
 struct Shape;
 struct Batch;
 struct AppendParams;
+struct AttendParams;
+
+constexpr int kPrefillItem = 256;  // query rows of an item of the kernel for chunks of prompts
+cudaError_t configure_prefill();
+void launch_prefill(const AttendParams& p, cudaStream_t st);
 
 // Opts the attention kernels into their shared memory on the current device.
 cudaError_t configure_attend();

@@ -24,7 +24,6 @@ namespace kv4 {
 constexpr int kPreRows = 256, kPreStages = 3, kPreRaw = 4, kPreInfo = 8, kPreN = 64;
 constexpr int kPreSoftmaxWarps = 8, kPreUnpackWarps = 4, kPreWarps = kPreSoftmaxWarps + kPreUnpackWarps + 3;
 constexpr int kPreScoreWarp = kPreWarps - 3, kPreOutputWarp = kPreWarps - 2, kPreCopyWarp = kPreWarps - 1;
-constexpr int kPreValueScale = 252;  // value (and key) scales above 2^125 count as 2^125: what a row does not see is finite
 
 struct PrefillInfo {     // of a step
     uint32_t missing;    // pages that are not there
@@ -84,7 +83,20 @@ __device__ __forceinline__ void tmem_store16(uint32_t addr, const uint32_t* r) {
                    "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
                  : "memory");
 }
-__device__ __forceinline__ void tmem_wait_load() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// (the registers pass through the wait, so that nothing that uses them can come before it)
+__device__ __forceinline__ void tmem_wait_load32(uint32_t* r) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]),
+                   "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]),
+                   "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+                 ::"memory");
+}
+__device__ __forceinline__ void tmem_wait_load16(uint32_t* r) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+                 ::"memory");
+}
 __device__ __forceinline__ void tmem_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // Waits for a barrier's phase; false when that takes kWaitCycles, or when another wait of the CTA has already given up.  The
@@ -259,23 +271,24 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1) prefill_kernel(const Attend
             // probabilities relative to the maximum so far, whose sum shows whether one is out of range
             auto read = [&](bool weighing) {
                 tmem_load32(lanes + col_s(tile, buf), x);
-                tmem_wait_load();
+                tmem_wait_load32(x);
                 tmem_load32(lanes + col_s(tile, buf) + 32, x + 32);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) sum[i] = 0.f;
                 hide(0);
                 if (weighing) weigh(0);
-                tmem_wait_load();
+                tmem_wait_load32(x + 32);
                 hide(32);
                 if (weighing) weigh(32);
             };
             read(j > 0);
-            if (j == 0 || __any_sync(0xffffffffu, !((sum[0] + sum[1]) + (sum[2] + sum[3]) < 256.f))) {
+            const bool out_of_range = j == 0 || !((sum[0] + sum[1]) + (sum[2] + sum[3]) < 256.f);
+            if (__any_sync(0xffffffffu, out_of_range)) {
                 if (j > 0) read(false);
                 top = -INFINITY;
 #pragma unroll
                 for (int i = 0; i < 64; ++i) top = fmaxf(top, __uint_as_float(x[i]));
-                const float now = fmaxf(m, top * qs), f = ex2(m - now);
+                const float now = out_of_range ? fmaxf(m, top * qs) : m, f = ex2(m - now);
                 m = now;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) l[i] *= f;
@@ -286,7 +299,7 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1) prefill_kernel(const Attend
                     for (int c = 0; c < kPreN; c += 16) {
                         uint32_t o[16];
                         tmem_load16(lanes + col_o(tile) + c, o);
-                        tmem_wait_load();
+                        tmem_wait_load16(o);
 #pragma unroll
                         for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
                         tmem_store16(lanes + col_o(tile) + c, o);
@@ -313,7 +326,7 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1) prefill_kernel(const Attend
             for (int c = 0; c < 64; c += 16) {
                 uint32_t o[16];
                 tmem_load16(lanes + col_o(tile) + c, o);
-                tmem_wait_load();
+                tmem_wait_load16(o);
                 if (tid < rows) {
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
@@ -349,7 +362,7 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1) prefill_kernel(const Attend
                 const int at = (group * 4 + i) % P;
                 vw[i] = *reinterpret_cast<const uint32_t*>(vrec + kCodes + at * (D / 2) + word * 4);
                 vbyte[i] = vrec[2 * kCodes + kScales + at * 2 + vb];
-                odd = odd || vbyte[i] > kPreValueScale;
+                odd = odd || vbyte[i] > kTopScale;
             }
             sm100::mbar_arrive(&s.raw_empty[j % kPreRaw]);
             if (!whole) {
@@ -369,10 +382,10 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1) prefill_kernel(const Attend
                         vbyte[i] = 0;
                         vw[i] = 0;
                     }
-                    vbyte[i] = min(vbyte[i], kPreValueScale);
+                    vbyte[i] = min(vbyte[i], kTopScale);
                 }
             {
-                const float scale = kbyte == 255 ? __uint_as_float(0x7fc00000u) : __uint_as_float((uint32_t)min(kbyte, kPreValueScale) << 23);
+                const float scale = kbyte == 255 ? __uint_as_float(0x7fc00000u) : __uint_as_float((uint32_t)min(kbyte, kTopScale) << 23);
                 const uint32_t w[4] = {kw.x, kw.y, kw.z, kw.w};
                 unsigned char* row = s.k[stage] + pos * 128;
 #pragma unroll

@@ -12,7 +12,6 @@
 
 #include "kv4_append.cuh"
 #include "kv4_attend.cuh"
-#include "kv4_prefill.cuh"
 #include "kv4_launch.h"
 
 using namespace neon;
@@ -130,17 +129,23 @@ cudaError_t attend_variant(const AttendParams* run, cudaStream_t st) {
     return cudaSuccess;
 }
 // Chunks of prompts: 256 rows of a key/value head at a time on tcgen05.  Heads of 64 only: at 128 columns queries, operands
-// and outputs would not fit a CTA.
-constexpr int kPrefillRows = 64;  // rows a sequence from which it is faster (see kv4_prefill.cuh)
-bool prefills(const Shape& s, int max_rows) { return s.D == 64 && (long long)max_rows * (s.nq / s.nkv) >= kPrefillRows; }
-
-template <int PAGE>
-cudaError_t prefill_variant(const AttendParams* run, cudaStream_t st) {
-    constexpr int kSmem = sizeof(PrefillSmem) + 1024;
-    if (!run) return cudaFuncSetAttribute(prefill_kernel<PAGE>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
-    const long long tiles = (long long)run->b.rows * run->G / kPreRows + run->b.n;  // as many as there can be
-    prefill_kernel<PAGE><<<(unsigned)(tiles * run->s.nkv), kPreWarps * 32, kSmem, st>>>(*run);
-    return cudaSuccess;
+// and outputs would not fit a CTA.  An item walks its positions alone, 1.2 to 1.5 us a step of 64, whether or not there is work for
+// the other multiprocessors; the other kernel splits steps evenly over all of them, 2.9 ns a step of 32 rows.  So the first is faster
+// from about 480 blocks of 32 rows for every wave of items on.  At 8 key/value heads and 4096 positions (other kernel, this one):
+//   8 sequences of 128 rows (256 blocks, 1 wave)     65,  93 us       of 256 rows (512 blocks)            112,  80 us
+//   32 sequences of 64 rows (512 blocks, 2 waves)   112, 216 us       of 128 rows (1024 blocks, 2 waves)  206, 184 us
+//   one sequence of 512 rows (128 blocks, 1 wave)    39,  80 us
+// Where a window leaves a few steps only, the other kernel's split and its second launch cost more than they bring: window 128,
+// 32 sequences of 64 rows 33, 24 us; 8 sequences of 512 rows 41, 13 us; 64 sequences of 16 rows 24, 46 us (few rows: the products'
+// tiles are nearly empty).
+constexpr int kPrefillRows = 64, kPrefillSpan = 512, kPrefillBlocks = 480;
+bool prefills(const Shape& s, const Batch& b, int max_rows, int window) {
+    const int G = s.nq / s.nkv;
+    const long long most = (long long)std::min(std::max(max_rows, 1), b.rows) * G;  // rows of an item's sequence, as far as known
+    if (s.D != 64 || most < kPrefillRows) return false;
+    if (window > 0 && (long long)window + max_rows <= kPrefillSpan) return true;
+    auto count = [&](int per) { return std::min((long long)b.rows * G / per + b.n, (most + per - 1) / per * b.n) * s.nkv; };
+    return count(32) >= kPrefillBlocks * ((count(kPrefillItem) + kSms - 1) / kSms);
 }
 
 // Calls f with every variant that there is; the one of a shape and a number of column groups.
@@ -162,15 +167,13 @@ cudaError_t configure_attend() {
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess || done[dev & 63]) return e;
     e = each_variant([](int, int, int, auto variant) { return variant(nullptr, nullptr); });
-    if (e == cudaSuccess) e = prefill_variant<16>(nullptr, nullptr);
-    if (e == cudaSuccess) e = prefill_variant<32>(nullptr, nullptr);
-    if (e == cudaSuccess) e = prefill_variant<64>(nullptr, nullptr);
+    if (e == cudaSuccess) e = configure_prefill();
     if (e == cudaSuccess) done[dev & 63] = true;
     return e;
 }
 
 uint64_t attend_workspace(const Shape& s, const Batch& b, int max_rows) {
-    if (prefills(s, max_rows)) return 16;
+    if (prefills(s, b, max_rows, 0)) return 16;  // (whatever the window)
     const int nt = column_groups(s, max_rows);
     return (uint64_t)attend_grid(s, b, nt) * (2 + kAttendWarps) * 8 * nt * (s.D + 2) * sizeof(float);
 }
@@ -184,10 +187,8 @@ int launch_attend(const Shape& s, const Batch& b, const uint8_t* cache, int dtyp
     p.grid = attend_grid(s, b, nt);
     p.R = 8 * nt;
     p.G_inverse = (uint32_t)((0x100000000ull + p.G - 1) / p.G);
-    if (prefills(s, max_rows)) {
-        if (s.P == 16) prefill_variant<16>(&p, st);
-        else if (s.P == 32) prefill_variant<32>(&p, st);
-        else prefill_variant<64>(&p, st);
+    if (prefills(s, b, max_rows, window)) {
+        launch_prefill(p, st);
         return 1;
     }
     each_variant([&](int dim, int page, int groups, auto variant) {

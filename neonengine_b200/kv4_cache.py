@@ -88,10 +88,18 @@ class Kv4Cache:
         return Kv4Batch(seq_lens, page_table, cu_q)
 
     # -- execution -----------------------------------------------------------------------------
+    def _on(self, stream, call, *args):
+        """The call with ``stream`` as the current one, so that what it allocates belongs to that stream too."""
+        _need(stream.device_index == self._index, "stream: one of the cache's device")
+        with torch.cuda.stream(stream):
+            return call(*args)
+
     def append(self, batch: Kv4Batch, cache, q, k, v, inv_freq, mscale: float = 1.0, out=None, stream=None):
         """Rotates ``q`` and ``k`` [rows, heads, head_dim] (fp32, bf16 or fp16; columns of one projection's output will do) by
         their rows' positions and writes ``k`` and ``v`` to the pages.  Returns the rotated queries (bf16, or fp16 for fp16
         input, or ``out``'s type); ``q`` may be None."""
+        if stream is not None:
+            return self._on(stream, self.append, batch, cache, q, k, v, inv_freq, mscale, out)
         rows = k.shape[0]
         ks, vs = self._rows(k, self.n_kv_heads, rows, "k"), self._rows(v, self.n_kv_heads, rows, "v")
         dtype = k.dtype
@@ -110,7 +118,7 @@ class Kv4Cache:
             q_ptr, out_ptr, out_dtype = q.data_ptr(), out.data_ptr(), _DTYPES[out.dtype]
         rc = self._lib.neon_kv4_append(self._h, batch._ref, self._place(batch, cache), rows, _DTYPES[dtype], q_ptr, qs, k.data_ptr(), ks, v.data_ptr(),
                                        vs, inv_freq.data_ptr(), mscale, out_ptr, out_dtype,
-                                       _stream_of(self._index) if stream is None else stream.cuda_stream)
+                                       _stream_of(self._index))
         if rc:
             self._check(rc, "neon_kv4_append")
         return out if q is not None else None
@@ -118,6 +126,8 @@ class Kv4Cache:
     def read(self, batch: Kv4Batch, cache, rows: int | None = None, dtype=torch.bfloat16, out=None, stream=None):
         """(keys, values) [rows, n_kv_heads, head_dim] that the cache holds at the positions of the batch's rows, bf16 or
         fp32; ``out``: a pair of tensors to write to."""
+        if stream is not None:
+            return self._on(stream, self.read, batch, cache, rows, dtype, out)
         if out is None:
             rows = batch.batch if rows is None else rows
             out = [torch.zeros((rows, self.n_kv_heads, self.head_dim), dtype=dtype, device=self.device) for _ in range(2)]
@@ -127,7 +137,7 @@ class Kv4Cache:
         _need(dtype in (torch.bfloat16, torch.float32) and v.dtype is dtype and v.shape == k.shape and k.is_contiguous() and v.is_contiguous()
               and v.get_device() == self._index, "out: two contiguous tensors of bfloat16 or float32")
         rc = self._lib.neon_kv4_read(self._h, batch._ref, self._place(batch, cache), rows, k.data_ptr(), v.data_ptr(), _DTYPES[dtype],
-                                     _stream_of(self._index) if stream is None else stream.cuda_stream)
+                                     _stream_of(self._index))
         if rc:
             self._check(rc, "neon_kv4_read")
         return k, v
@@ -137,6 +147,8 @@ class Kv4Cache:
         """Attention of ``q`` [rows, n_q_heads, head_dim] (bf16 or fp16, rotated) over the cache; ``sinks``: bf16 [n_q_heads] logits of the
         softmax denominator; ``window`` > 0: only the last so many positions; ``scale``: default head_dim ** -0.5; ``max_rows``: the
         most rows of a sequence, if the host knows it (speed only)."""
+        if stream is not None:
+            return self._on(stream, self.attend, batch, cache, q, sinks, window, scale, max_rows, out)
         rows, dtype = q.shape[0], q.dtype
         qs = self._rows(q, self.n_q_heads, rows, "q")
         _need(dtype is torch.bfloat16 or dtype is torch.float16, "q: bfloat16 or float16")
@@ -153,13 +165,9 @@ class Kv4Cache:
         size = lib.neon_kv4_attend_workspace(handle, ref, rows, max_rows)
         # allocated on the current stream, so that two calls never share it; torch reuses it in stream order
         scratch = torch.empty(size, dtype=torch.uint8, device=self.device)
-        if stream is None:
-            st = _stream_of(self._index)
-        else:
-            st = stream.cuda_stream
-            scratch.record_stream(stream)
         rc = lib.neon_kv4_attend(handle, ref, cache_ptr, rows, _DTYPES[dtype], q.data_ptr(), qs, None if sinks is None else sinks.data_ptr(), window,
-                                 self.head_dim ** -0.5 if scale is None else scale, max_rows, out.data_ptr(), scratch.data_ptr(), size, st)
+                                 self.head_dim ** -0.5 if scale is None else scale, max_rows, out.data_ptr(), scratch.data_ptr(), size,
+                                 _stream_of(self._index))
         if rc:
             self._check(rc, "neon_kv4_attend")
         return out

@@ -39,6 +39,11 @@ class Sampler:
         """Tokens int32 [rows] of ``logits`` [rows, vocab] (fp32, bf16 or fp16; rows may be any stride apart).  ``uniform``: fp32
         [rows] in [0, 1); ``temperature``, ``top_p``, ``min_p`` fp32 [rows] and ``top_k`` int32 [rows], or None.  With ``details``
         returns (tokens, probability of each among what was kept, how many were kept)."""
+        if stream is not None:  # what the run allocates belongs to that stream too
+            if stream.device_index != self._index:
+                raise ValueError("stream: one of the sampler's device")
+            with torch.cuda.stream(stream):
+                return self.run(logits, uniform, temperature, top_k, top_p, min_p, out, details)
         shape, stride, dtype, f32 = logits.shape, logits.stride(), logits.dtype, torch.float32
         if len(shape) != 2 or shape[1] != self.vocab or dtype not in _DTYPES or logits.get_device() != self._index or (stride[1] != 1 and shape[1] > 1):
             raise ValueError(f"logits: [rows, {self.vocab}] of float32, bfloat16 or float16 on {self.device}, rows contiguous")
@@ -59,13 +64,8 @@ class Sampler:
             probs_ptr, kept_ptr = probs.data_ptr(), kept.data_ptr()
         # allocated on the current stream, so that two runs never share it; torch reuses it in stream order
         scratch = torch.empty(size, dtype=torch.uint8, device=device)
-        if stream is None:
-            st = _stream_of(self._index)
-        else:
-            st = stream.cuda_stream
-            scratch.record_stream(stream)
         rc = self._lib.neon_sampler_run(self._h, logits.data_ptr(), _DTYPES[dtype], stride[0] if rows > 1 else self.vocab, rows, u, t, k, p, m,
-                                        tokens_ptr, probs_ptr, kept_ptr, scratch.data_ptr(), size, st)
+                                        tokens_ptr, probs_ptr, kept_ptr, scratch.data_ptr(), size, _stream_of(self._index))
         if rc:
             raise RuntimeError(f"neon_sampler_run failed ({rc}): {self._lib.neon_sampler_last_error(self._h).decode()}")
         return (tokens, probs, kept) if details else tokens

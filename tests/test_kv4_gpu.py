@@ -155,6 +155,46 @@ def test_attend_scales_far_apart(systems, spread, rows):
     check_attention(kv, batch, table, cu, [rows] * 2, lens, cache, q, None, 0, 64 ** -0.5, out, flat=False)
 
 
+@pytest.mark.parametrize("rows", [1, 5, 80])
+def test_attend_scales_of_infinities(systems, rows):
+    """Value scales of 2^126 and 2^127 count as 2^125, in every kernel."""
+    kv, g = systems(16, 2, 64, 32), gen(rows)
+    lens = [300]
+    batch, table, cu, pages = make_batch(kv, [rows], lens, g)
+    cache = random_cache(kv, pages, g)
+    scales = ref.parts(cache, 32, 64)[3]
+    page, slot = int(table[0, 1]), 7  # every row sees it
+    cache_top = cache.clone()
+    scales[page, 0, slot, 0] = 254
+    scales[page, 1, slot, 1] = 253
+    top = ref.parts(cache_top, 32, 64)[3]
+    top[page, 0, slot, 0] = 252
+    top[page, 1, slot, 1] = 252
+    q = torch.randn((rows, 16, 64), generator=g, device=DEV).to(torch.bfloat16)
+    out, want = (kv.attend(batch, c, q, max_rows=rows) for c in (cache, cache_top))
+    assert same(out, want)
+    clear = torch.ones_like(out, dtype=torch.bool)  # columns of other blocks are untouched by them
+    clear[:, :8, :32] = clear[:, 8:, 32:] = False
+    assert out[clear].isfinite().all() and (out[clear].abs() < 100).all()
+
+
+@pytest.mark.parametrize("nq,nkv,P,dtype", [(16, 2, 16, torch.bfloat16), (64, 8, 32, torch.float16), (12, 4, 64, torch.float16), (20, 10, 16, torch.bfloat16)])
+def test_attend_long_chunks(systems, nq, nkv, P, dtype):
+    """Chunks of prompts over many steps, more items than multiprocessors, with and without a window."""
+    kv, g = systems(nq, nkv, 64, P), gen(nq + P)
+    rows, lens = [333, 1, 700, 64, 250], [5000, 4097, 731, 64, 9001]
+    batch, table, cu, pages = make_batch(kv, rows, lens, g)
+    cache = random_cache(kv, pages, g)
+    q = torch.randn((sum(rows), nq, 64), generator=g, device=DEV).to(dtype)
+    sinks = torch.randn((nq,), generator=g, device=DEV).to(torch.bfloat16)
+    for window in (0, 1000):
+        out = kv.attend(batch, cache, q, sinks=sinks, window=window, max_rows=700)
+        check_attention(kv, batch, table, cu, rows, lens, cache, q, sinks, window, 0.125, out)
+        again = kv.attend(batch, cache, q, sinks=sinks, window=window, max_rows=700)
+        assert torch.equal(out, again)
+    assert kv.status() == 0
+
+
 def test_attend_small_values_at_the_top(systems):
     """All weight on positions whose values are 2^-30 of those that the softmax suppresses: the result is theirs."""
     kv, g = systems(8, 8, 64, 64), gen(3)
@@ -443,6 +483,82 @@ def test_captured_graph_and_streams(systems):
         torch.cuda.synchronize()
         for w, out in zip(worlds, outs):
             assert torch.equal(out, step(w))
+
+
+def test_results_belong_to_the_given_stream(systems):
+    """A call on another stream while the current one still has to write to memory that it freed: the result is not in it."""
+    kv, g = systems(16, 2, 64, 32), gen(32)
+    batch, table, cu, pages = make_batch(kv, [1] * 8, [200] * 8, g, each=True)
+    cache = random_cache(kv, pages, g)
+    q = torch.randn((8, 16, 64), generator=g, device=DEV).to(torch.bfloat16)
+    want, (want_k, want_v) = kv.attend(batch, cache, q), kv.read(batch, cache)
+    other = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    freed = [torch.empty_like(t) for t in (want, want_k, want_v)]
+    torch.cuda._sleep(20000000)
+    for t in freed:
+        t.fill_(7)
+    del freed, t
+    out = kv.attend(batch, cache, q, stream=other)
+    k, v = kv.read(batch, cache, stream=other)
+    torch.cuda.synchronize()
+    assert torch.equal(out, want) and torch.equal(k, want_k) and torch.equal(v, want_v)
+
+
+class Padded:
+    """The system, with the queries of every attention call followed by rows that belong to no sequence: so many that the
+    kernel for chunks of prompts is chosen (where heads are of 64)."""
+
+    def __init__(self, kv):
+        self.kv = kv
+
+    def __getattr__(self, name):
+        return getattr(self.kv, name)
+
+    def attend(self, batch, cache, q, sinks=None, window=0, scale=None, max_rows=None, out=None):
+        n, total = q.shape[0], q.shape[0] + 40960 // self.kv.n_q_heads
+        wide = torch.full((total, *q.shape[1:]), float("nan"), dtype=q.dtype, device=DEV)
+        wide[:n] = q
+        held = torch.full_like(wide, 7.0)
+        if out is not None:
+            held[:n] = out
+        launched = self.kv.launch_count
+        self.kv.attend(batch, cache, wide, sinks, window, scale, total, held)
+        assert self.kv.launch_count == launched + 1  # the other kernel takes two
+        assert (held[n:] == 7.0).all()
+        return held[:n] if out is None else out.copy_(held[:n])
+
+
+SEVERAL = [([5, 1, 3, 0, 2], [300, 1, 3, 50, 1000], 0, True), ([4, 7], [2, 7], 0, False), ([4, 7], [2, 700], 5, True),
+           ([130, 33], [130, 641], 0, False), ([65, 40, 1], [400, 129, 90], 48, True)]
+
+
+@pytest.mark.parametrize("nq,nkv,D,P", [h for h in HEADS if h[2] == 64])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_chunk_kernel_shapes(systems, nq, nkv, D, P, dtype):
+    def padded(*shape):
+        return Padded(systems(*shape))
+    for window in (0, 37):
+        test_attend_one_token(padded, nq, nkv, D, P, dtype, window)
+    for rows, lens, window, sink in SEVERAL:
+        test_attend_several_rows(padded, nq, nkv, D, P, rows, lens, window, sink)
+
+
+@pytest.mark.parametrize("which", ["scales", "infinities", "unseen", "queries"])
+def test_chunk_kernel_values(systems, which):
+    def padded(*shape):
+        return Padded(systems(*shape))
+    if which == "scales":
+        for spread in (3, 9, 40, 100):
+            for rows in (1, 6, 70):
+                test_attend_scales_far_apart(padded, spread, rows)
+    elif which == "infinities":
+        test_attend_scales_of_infinities(padded, 5)
+    elif which == "unseen":
+        test_attend_ignores_what_it_does_not_see(padded)
+        test_attend_small_values_at_the_top(padded)
+    else:
+        test_attend_extreme_queries(padded)
 
 
 # ---- refusals ----------------------------------------------------------------------------------------------------
