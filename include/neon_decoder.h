@@ -23,6 +23,8 @@
  *     orig_ctx as in the YaRN paper; cos and sin are multiplied by 0.1*ln(factor) + 1.
  *   - Attention scores are q.k/8; the softmax denominator includes exp(sink[head]); layers with
  *     even index attend to the last `window` positions only, odd layers to the whole cache.
+ *   - Option "kv_bits" 4 holds keys and values in 4 bits (records of 64 positions as in neon_kv4.h, 1/3.76 of the
+ *     memory): rotated keys and values are rounded to them as they are appended, queries to bf16.  Everything else is the same.
  *   - K/V cache per layer (internal): keys bf16 [max_batch][n_kv_heads][max_ctx][64], values
  *     transposed [max_batch][n_kv_heads][64][max_ctx].
  *   - The MoE of a layer receives the bf16 normalised activations; its config is
@@ -102,19 +104,28 @@ int neon_decoder_load_kv(neon_decoder_handle* h, int layer, const void* k, const
 int neon_decoder_step(neon_decoder_handle* h, const int32_t* tokens, const int32_t* positions, int batch,
                       float* logits, int32_t* next_tokens, void* cuda_stream);
 
-/* Same with HOST arrays; copies tokens/positions in, next_tokens out, and waits. */
+/* Next tokens are sampled from now on (neon_sampler.h) instead of being the largest logits'.  Device arrays of at least max_batch
+ * elements that every step reads as it runs, so they may be refilled between steps: uniform fp32, numbers in [0, 1);
+ * temperature, top_p, min_p fp32, top_k int32, each NULL for none.  uniform NULL (and all others): the largest again. */
+int neon_decoder_set_sampling(neon_decoder_handle* h, const float* uniform, const float* temperature,
+                              const int32_t* top_k, const float* top_p, const float* min_p);
+
+/* Same as neon_decoder_step with HOST arrays; copies tokens/positions in, next_tokens out, and waits. */
 int neon_decoder_step_host(neon_decoder_handle* h, const int32_t* tokens, const int32_t* positions,
                            int batch, int32_t* next_tokens, void* cuda_stream);
 
 /* Test/debug read-back (blocking) of an internal buffer of the last step into host memory.
  * name: "x" fp32 [B,H] residual stream after the last layer; "xn" bf16 [B,H] last normalised
  * activations (the final norm's output); "qkv" fp32 [B,(nq+2nkv)*64] of the last layer
- * (q rotated, k/v as projected); "attn" bf16 [B,nq*64]; "moe_in" bf16 [B,H] of the last layer;
- * "moe_out" fp32 [B,H]; "logits" fp32 [B,vocab]; "inv_freq" fp32 [32]. */
+ * (q rotated, k/v as projected; with "kv_bits" 4 all as projected, in as many parts, [part][batch], as the projection's depth was cut
+ * into); "attn" bf16 [B,nq*64]; "moe_in" bf16 [B,H] of the last layer;
+ * "moe_out" fp32 [B,H]; "logits" fp32 [B,vocab]; "inv_freq" fp32 [32]; "kv4_status" int32: status bits of the
+ * 4-bit cache's attention (neon_kv4.h). */
 int neon_decoder_read(neon_decoder_handle* h, const char* name, void* dst, uint64_t bytes);
 
 /* Options: "use_graphs" (default 1), "pdl" (programmatic dependent launch, a bit per
- * kernel kind: 1 GEMV, 2 RMSNorm, 4 rotary/cache, 8 attention, 16 merge, 32 others; default 29), "moe.<option>" (passed to every layer, see neon_moe.h), "stop_after_layer" (debug: run only the first n layers
+ * kernel kind: 1 GEMV, 2 RMSNorm, 4 rotary/cache, 8 attention, 16 merge, 32 others; default 29), "moe.<option>" (passed to every layer, see neon_moe.h), "kv_bits"
+ * (16, or 4: see above; switching empties the cache and waits for the device), "stop_after_layer" (debug: run only the first n layers
  * and skip the head; 0 = all). */
 int neon_decoder_set_option(neon_decoder_handle* h, const char* name, int64_t value);
 

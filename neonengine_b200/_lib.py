@@ -122,6 +122,7 @@ DECODER_SIGNATURES = {
     "neon_decoder_set_moe": (c_int, [c_void_p, c_int] + [c_void_p] * 8 + [c_int]),
     "neon_decoder_load_kv": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_int]),
     "neon_decoder_step": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p]),
+    "neon_decoder_set_sampling": (c_int, [c_void_p] * 6),
     "neon_decoder_step_host": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p]),
     "neon_decoder_read": (c_int, [c_void_p, ctypes.c_char_p, c_void_p, ctypes.c_uint64]),
     "neon_decoder_set_option": (c_int, [c_void_p, ctypes.c_char_p, ctypes.c_int64]),

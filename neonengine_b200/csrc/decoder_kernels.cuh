@@ -19,11 +19,13 @@ __device__ __forceinline__ uint16_t f32_to_bf16_rn(float f) { return __bfloat16_
 
 // x[b, :] = embed[token[b], :] (bf16 -> fp32 residual stream).
 // Token ids outside [0, vocab) are clamped into range rather than read out of bounds.
+// lengths (may be null): what the 4-bit cache's kernels take for the positions, clamped as rope_cache_kernel does.
 __global__ void embed_kernel(const uint16_t* __restrict__ embed, const int32_t* __restrict__ tokens, int H, int vocab,
-                             float* __restrict__ x) {
+                             float* __restrict__ x, const int32_t* __restrict__ positions, int ctx, int32_t* __restrict__ lengths) {
     pdl_launch_dependents();
     pdl_wait();
     const int b = blockIdx.x;
+    if (lengths && threadIdx.x == 0) lengths[b] = min(max(positions[b], 0), ctx - 1) + 1;
     const uint16_t* row = embed + (size_t)min(max(tokens[b], 0), vocab - 1) * H;
     for (int i = threadIdx.x; i < H; i += blockDim.x) x[(size_t)b * H + i] = bf16_bits_to_float(row[i]);
 }

@@ -3,6 +3,7 @@
 // step as a fixed kernel sequence (replayed as a CUDA graph once the arguments repeat).
 // No CPU fallback exists: a step launches CUDA kernels or fails with an error code.
 #include "../../include/neon_decoder.h"
+#include "../../include/neon_sampler.h"
 
 #include <cmath>
 #include <cstdarg>
@@ -14,6 +15,9 @@
 #include <vector>
 
 #include "decoder_kernels.cuh"
+#include "kv4_append.cuh"
+#include "kv4_launch.h"
+#include "sampler_launch.h"
 
 using namespace neon;
 
@@ -22,9 +26,27 @@ thread_local std::string g_dec_create_error;
 
 struct LayerW {
     uint16_t *ln1 = nullptr, *wqkv = nullptr, *bqkv = nullptr, *sinks = nullptr, *wo = nullptr, *bo = nullptr, *ln2 = nullptr;
-    uint16_t *kc = nullptr, *vc = nullptr;
+    uint16_t *kc = nullptr, *vc = nullptr;  // bf16 cache, or:
+    uint8_t* pages = nullptr;               // 4-bit cache (neon_kv4.h), sequence b's pages in order from b * Kv4::width on
     neon_moe_handle* moe = nullptr;
     bool has_attn = false, has_moe = false;
+};
+
+// What the layers' 4-bit caches share ("kv_bits" 4).
+struct Kv4 {
+    kv4::Shape shape{};
+    int width = 0;  // pages of a sequence
+    int32_t *lengths = nullptr, *table = nullptr;
+    int* status = nullptr;
+    uint16_t* q = nullptr;      // rotated queries
+    float* scratch = nullptr;   // of the attention
+    float* no_turn = nullptr;   // frequencies of zero: loading keys that are rotated already
+    bool on() const { return lengths != nullptr; }
+    void release() {
+        for (void* p : {(void*)lengths, (void*)table, (void*)status, (void*)q, (void*)scratch, (void*)no_turn})
+            if (p) cudaFree(p);
+        *this = Kv4{};
+    }
 };
 }  // namespace
 
@@ -39,6 +61,12 @@ struct neon_decoder_handle {
     int qkv_split = 1, o_split = 1;
     uint16_t *xn = nullptr, *xn2 = nullptr, *attn = nullptr;
     int32_t *tok_dev = nullptr, *pos_dev = nullptr, *next_dev = nullptr;
+    Kv4 kv4;
+    struct {
+        const float *uniform = nullptr, *temperature = nullptr, *top_p = nullptr, *min_p = nullptr;
+        const int32_t* top_k = nullptr;
+        void* scratch = nullptr;
+    } sampling;
     float mscale = 1.f;
     int64_t launches = 0;
     int use_graphs = 1, stop_after = 0;
@@ -196,11 +224,37 @@ int launch_attention(neon_decoder_handle* h, const LayerW& L, int layer, int B, 
     return NEON_MOE_OK;
 }
 
+kv4::Batch kv4_batch(const neon_decoder_handle* h, const int32_t* lengths, const int32_t* cu_q, int batch, int rows) {
+    const Kv4& k = h->kv4;
+    return {lengths, cu_q, k.table, k.width, (long long)h->cfg.max_batch * k.width, k.width, batch, rows, k.status};
+}
+
+// The new token's keys and values into the 4-bit cache, attention over it.
+void launch_attention4(neon_decoder_handle* h, const LayerW& L, int layer, int B, cudaStream_t st) {
+    const auto& c = h->cfg;
+    const int QKV = (c.n_q_heads + 2 * c.n_kv_heads) * c.head_dim, QD = c.n_q_heads * c.head_dim;
+    const kv4::Batch batch = kv4_batch(h, h->kv4.lengths, nullptr, B, B);
+    kv4::AppendParams p{};
+    p.b = batch;
+    p.s = h->kv4.shape;
+    p.q = h->qkv; p.k = h->qkv + QD; p.v = h->qkv + QD + c.n_kv_heads * c.head_dim;
+    p.q_stride = p.k_stride = p.v_stride = QKV;
+    p.n_parts = h->qkv_split;
+    p.part_stride = (long long)B * QKV;
+    p.inv_freq = h->inv_freq; p.mscale = h->mscale;
+    p.q_out = h->kv4.q;
+    p.cache = L.pages;
+    h->launches += kv4::launch_append(p, NEON_KV4_F32, NEON_KV4_BF16, st);
+    h->launches += kv4::launch_attend(p.s, batch, L.pages, NEON_KV4_BF16, h->kv4.q, QD, L.sinks, c.window > 0 && layer % 2 == 0 ? c.window : 0,
+                                      1.f / std::sqrt((float)c.head_dim), 1, h->attn, h->kv4.scratch, st);
+}
+
 int step_eager(neon_decoder_handle* h, const int32_t* tokens, const int32_t* positions, int B, float* logits, int32_t* next,
                cudaStream_t st) {
     const auto& c = h->cfg;
     const int H = c.hidden, QKV = (c.n_q_heads + 2 * c.n_kv_heads) * c.head_dim, QD = c.n_q_heads * c.head_dim;
-    launch(h, kPdlOther, embed_kernel, dim3(B), dim3(256), 0, st, (const uint16_t*)h->embed, tokens, H, c.vocab, h->x);
+    launch(h, kPdlOther, embed_kernel, dim3(B), dim3(256), 0, st, (const uint16_t*)h->embed, tokens, H, c.vocab, h->x,
+           positions, c.max_ctx, h->kv4.lengths);
     const int n_layers = h->stop_after > 0 ? std::min(h->stop_after, c.n_layers) : c.n_layers;
     const float* pending = nullptr;  // MoE output of the previous layer, added by the next RMSNorm kernel
     for (int l = 0; l < n_layers; ++l) {
@@ -209,11 +263,15 @@ int step_eager(neon_decoder_handle* h, const int32_t* tokens, const int32_t* pos
                (const uint16_t*)L.ln1, H, c.rms_eps, h->xn);
         int rc = launch_gemv_split(h, L.wqkv, L.bqkv, h->xn, B, QKV, H, h->qkv_split, h->qkv, (long long)B * QKV, st);
         if (rc) return rc;
-        launch(h, kPdlRope, rope_cache_kernel, dim3(c.n_q_heads + 2 * c.n_kv_heads, B), dim3(64), 0, st, h->qkv, h->qkv_split,
-               (long long)B * QKV, (const float*)h->inv_freq, positions, c.n_q_heads, c.n_kv_heads, h->mscale, c.max_ctx, L.kc,
-               L.vc);
-        rc = launch_attention(h, L, l, B, positions, st);
-        if (rc) return rc;
+        if (h->kv4.on()) {
+            launch_attention4(h, L, l, B, st);
+        } else {
+            launch(h, kPdlRope, rope_cache_kernel, dim3(c.n_q_heads + 2 * c.n_kv_heads, B), dim3(64), 0, st, h->qkv, h->qkv_split,
+                   (long long)B * QKV, (const float*)h->inv_freq, positions, c.n_q_heads, c.n_kv_heads, h->mscale, c.max_ctx, L.kc,
+                   L.vc);
+            rc = launch_attention(h, L, l, B, positions, st);
+            if (rc) return rc;
+        }
         rc = launch_gemv_split(h, L.wo, L.bo, h->attn, B, H, QD, h->o_split, h->oproj, (long long)B * H, st);
         if (rc) return rc;
         // residual add of the projection's parts, then the second norm
@@ -234,8 +292,102 @@ int step_eager(neon_decoder_handle* h, const int32_t* tokens, const int32_t* pos
     float* lg = logits ? logits : h->logits;
     int rc = launch_gemv(h, h->unembed, nullptr, h->xn, B, c.vocab, H, 0, lg, st);
     if (rc) return rc;
-    if (next) launch(h, kPdlOther, argmax_kernel, dim3(B), dim3(1024), 0, st, (const float*)lg, c.vocab, next);
+    const auto& s = h->sampling;
+    if (next && s.uniform)
+        h->launches += sampler::launch(lg, NEON_SAMPLER_F32, c.vocab, c.vocab, B, s.uniform, s.temperature, s.top_k, s.top_p, s.min_p, next,
+                                       nullptr, nullptr, s.scratch, st);
+    else if (next) launch(h, kPdlOther, argmax_kernel, dim3(B), dim3(1024), 0, st, (const float*)lg, c.vocab, next);
     DCU(h, cudaGetLastError());
+    return NEON_MOE_OK;
+}
+
+// Positions [0, n_pos) of a layer's 4-bit cache from bf16 keys (rotated: appended with frequencies of zero) and values.
+int load_kv4(neon_decoder_handle* h, const LayerW& L, const void* k, const void* v, int batch, int n_pos, int on_device) {
+    if (!batch || !n_pos) return NEON_MOE_OK;
+    const auto& c = h->cfg;
+    const size_t row = (size_t)c.n_kv_heads * 64, bytes = (size_t)batch * n_pos * row * 2;
+    std::vector<int32_t> meta(batch + 1);  // where sequences start, then their lengths
+    for (int b = 0; b <= batch; ++b) meta[b] = b * n_pos;
+    meta.insert(meta.end(), batch, n_pos);
+    char* tmp = nullptr;
+    DCU(h, cudaMalloc(&tmp, (on_device ? 0 : 2 * bytes) + meta.size() * 4));
+    char* lists = tmp + (on_device ? 0 : 2 * bytes);
+    cudaError_t e = cudaMemcpy(lists, meta.data(), meta.size() * 4, cudaMemcpyHostToDevice);
+    if (!on_device) {
+        if (e == cudaSuccess) e = cudaMemcpy(tmp, k, bytes, cudaMemcpyHostToDevice);
+        if (e == cudaSuccess) e = cudaMemcpy(tmp + bytes, v, bytes, cudaMemcpyHostToDevice);
+        k = tmp;
+        v = tmp + bytes;
+    }
+    if (e == cudaSuccess) {
+        const int32_t* cu = reinterpret_cast<const int32_t*>(lists);
+        kv4::AppendParams p{};
+        p.b = kv4_batch(h, cu + batch + 1, cu, batch, batch * n_pos);
+        p.s = h->kv4.shape;
+        p.k = k; p.v = v;
+        p.k_stride = p.v_stride = (long long)row;
+        p.n_parts = 1;
+        p.inv_freq = h->kv4.no_turn; p.mscale = 1.f;
+        p.cache = L.pages;
+        h->launches += kv4::launch_append(p, NEON_KV4_BF16, NEON_KV4_BF16, nullptr);
+        e = cudaDeviceSynchronize();
+    }
+    cudaFree(tmp);
+    return e == cudaSuccess ? NEON_MOE_OK : dfail(h, NEON_MOE_ECUDA, "loading the 4-bit cache: %s", cudaGetErrorString(e));
+}
+
+// Gives the layers empty caches of the other kind; all of them, or (with an error) none.
+int set_kv_bits(neon_decoder_handle* h, int64_t bits) {
+    if (bits != 4 && bits != 16) return dfail(h, NEON_MOE_EINVAL, "kv_bits must be 4 or 16");
+    if ((bits == 4) == h->kv4.on()) return NEON_MOE_OK;
+    const auto& c = h->cfg;
+    DCU(h, cudaSetDevice(c.device));
+    DCU(h, cudaDeviceSynchronize());  // steps may still use the caches that go
+    Kv4 next;
+    std::vector<void*> caches;
+    cudaError_t e = cudaSuccess;
+    auto alloc = [&](auto& ptr, size_t bytes) {
+        if (e == cudaSuccess) e = cudaMalloc(reinterpret_cast<void**>(&ptr), bytes);
+        if (e == cudaSuccess) e = cudaMemset(ptr, 0, bytes);
+    };
+    size_t bytes = (size_t)c.max_batch * c.max_ctx * c.n_kv_heads * 64 * 2;  // one of a layer's two bf16 tensors
+    if (bits == 4) {
+        next.shape = {c.n_q_heads, c.n_kv_heads, 64, 64};
+        next.width = (c.max_ctx + 63) / 64;
+        bytes = (size_t)c.max_batch * next.width * c.n_kv_heads * next.shape.record();
+        alloc(next.lengths, c.max_batch * 4);
+        alloc(next.table, (size_t)c.max_batch * next.width * 4);
+        alloc(next.status, 4);
+        alloc(next.q, (size_t)c.max_batch * c.n_q_heads * 64 * 2);
+        alloc(next.no_turn, 32 * 4);
+        const kv4::Batch most{nullptr, nullptr, nullptr, next.width, 1, next.width, c.max_batch, c.max_batch, nullptr};
+        alloc(next.scratch, kv4::attend_workspace(next.shape, most, 1));
+        std::vector<int32_t> pages((size_t)c.max_batch * next.width);
+        for (size_t i = 0; i < pages.size(); ++i) pages[i] = (int32_t)i;
+        if (e == cudaSuccess) e = cudaMemcpy(next.table, pages.data(), pages.size() * 4, cudaMemcpyHostToDevice);
+        if (e == cudaSuccess) e = kv4::configure_attend();
+    }
+    for (int i = 0; i < c.n_layers * (bits == 4 ? 1 : 2) && e == cudaSuccess; ++i) {
+        caches.push_back(nullptr);
+        alloc(caches.back(), bytes);
+    }
+    if (e != cudaSuccess) {
+        for (void* p : caches)
+            if (p) cudaFree(p);
+        next.release();
+        cudaGetLastError();
+        return dfail(h, NEON_MOE_ECUDA, "caches of %d bits: %s", (int)bits, cudaGetErrorString(e));
+    }
+    for (int l = 0; l < c.n_layers; ++l) {
+        LayerW& L = h->layers[l];
+        for (void* p : {(void*)L.kc, (void*)L.vc, (void*)L.pages})
+            if (p) cudaFree(p);
+        L.kc = bits == 4 ? nullptr : static_cast<uint16_t*>(caches[2 * l]);
+        L.vc = bits == 4 ? nullptr : static_cast<uint16_t*>(caches[2 * l + 1]);
+        L.pages = bits == 4 ? static_cast<uint8_t*>(caches[l]) : nullptr;
+    }
+    h->kv4.release();
+    h->kv4 = next;
     return NEON_MOE_OK;
 }
 
@@ -345,14 +497,15 @@ int neon_decoder_destroy(neon_decoder_handle* h) {
     drop_graph(h);
     for (auto& L : h->layers) {
         for (void* p : {(void*)L.ln1, (void*)L.wqkv, (void*)L.bqkv, (void*)L.sinks, (void*)L.wo, (void*)L.bo, (void*)L.ln2,
-                        (void*)L.kc, (void*)L.vc})
+                        (void*)L.kc, (void*)L.vc, (void*)L.pages})
             if (p) cudaFree(p);
         if (L.moe) neon_moe_destroy(L.moe);
     }
     for (void* p : {(void*)h->embed, (void*)h->unembed, (void*)h->final_norm, (void*)h->x, (void*)h->qkv, (void*)h->moe_out,
                     (void*)h->logits, (void*)h->part, (void*)h->oproj, (void*)h->inv_freq, (void*)h->xn, (void*)h->xn2, (void*)h->attn,
-                    (void*)h->tok_dev, (void*)h->pos_dev, (void*)h->next_dev})
+                    (void*)h->tok_dev, (void*)h->pos_dev, (void*)h->next_dev, h->sampling.scratch})
         if (p) cudaFree(p);
+    h->kv4.release();
     if (h->own_stream) cudaStreamDestroy(h->own_stream);
     cudaGetLastError();
     delete h;
@@ -414,6 +567,7 @@ int neon_decoder_load_kv(neon_decoder_handle* h, int layer, const void* k, const
     if (!k || !v) return dfail(h, NEON_MOE_EINVAL, "null cache tensor");
     DCU(h, cudaSetDevice(c.device));
     LayerW& L = h->layers[layer];
+    if (h->kv4.on()) return load_kv4(h, L, k, v, batch, n_pos, on_device);
     if (batch && n_pos) {
         const size_t bytes = (size_t)batch * n_pos * c.n_kv_heads * 64 * 2;
         const size_t vecs = bytes / 16;
@@ -502,7 +656,30 @@ int neon_decoder_step_host(neon_decoder_handle* h, const int32_t* tokens, const 
     int rc = neon_decoder_step(h, h->tok_dev, h->pos_dev, batch, nullptr, h->next_dev, st);
     if (rc) return rc;
     DCU(h, cudaMemcpyAsync(next_tokens, h->next_dev, (size_t)batch * 4, cudaMemcpyDeviceToHost, st));
+    int status = 0;
+    if (h->kv4.on()) DCU(h, cudaMemcpyAsync(&status, h->kv4.status, sizeof status, cudaMemcpyDeviceToHost, st));
     DCU(h, cudaStreamSynchronize(st));
+    if (status) {
+        DCU(h, cudaMemsetAsync(h->kv4.status, 0, sizeof status, st));
+        return dfail(h, NEON_MOE_ECUDA, "the 4-bit cache's attention reported %d", status);
+    }
+    return NEON_MOE_OK;
+}
+
+int neon_decoder_set_sampling(neon_decoder_handle* h, const float* uniform, const float* temperature, const int32_t* top_k,
+                              const float* top_p, const float* min_p) {
+    if (!h) return NEON_MOE_EINVAL;
+    auto& s = h->sampling;
+    if (!uniform && (temperature || top_k || top_p || min_p)) return dfail(h, NEON_MOE_EINVAL, "sampling without uniform numbers");
+    if (uniform && h->cfg.vocab > NEON_SAMPLER_MAX_VOCAB)
+        return dfail(h, NEON_MOE_EINVAL, "sampling takes vocabularies up to %d", NEON_SAMPLER_MAX_VOCAB);
+    DCU(h, cudaSetDevice(h->cfg.device));
+    if (uniform && !s.scratch) {
+        DCU(h, sampler::configure());
+        DALLOC(h, s.scratch, sampler::workspace(h->cfg.vocab, h->cfg.max_batch));
+    }
+    drop_graph(h);
+    s.uniform = uniform; s.temperature = temperature; s.top_k = top_k; s.top_p = top_p; s.min_p = min_p;
     return NEON_MOE_OK;
 }
 
@@ -516,9 +693,10 @@ int neon_decoder_read(neon_decoder_handle* h, const char* name, void* dst, uint6
     else if (!strcmp(name, "xn")) { src = h->xn; cap = B * H * 2; }
     else if (!strcmp(name, "moe_in")) { src = h->xn2; cap = B * H * 2; }
     else if (!strcmp(name, "moe_out")) { src = h->moe_out; cap = B * H * 4; }
-    else if (!strcmp(name, "qkv")) { src = h->qkv; cap = B * (size_t)(c.n_q_heads + 2 * c.n_kv_heads) * 64 * 4; }
+    else if (!strcmp(name, "qkv")) { src = h->qkv; cap = h->qkv_split * B * (size_t)(c.n_q_heads + 2 * c.n_kv_heads) * 64 * 4; }
     else if (!strcmp(name, "attn")) { src = h->attn; cap = B * (size_t)c.n_q_heads * 64 * 2; }
     else if (!strcmp(name, "logits")) { src = h->logits; cap = B * (size_t)c.vocab * 4; }
+    else if (!strcmp(name, "kv4_status") && h->kv4.on()) { src = h->kv4.status; cap = 4; }
     else if (!strcmp(name, "inv_freq")) { src = h->inv_freq; cap = 32 * 4; }
     else return dfail(h, NEON_MOE_EINVAL, "unknown buffer '%s'", name);
     if (bytes > cap) return dfail(h, NEON_MOE_EINVAL, "'%s' holds %zu bytes, %llu asked", name, cap, (unsigned long long)bytes);
@@ -539,6 +717,7 @@ int neon_decoder_set_option(neon_decoder_handle* h, const char* name, int64_t va
             if (rc) return dfail(h, rc, "MoE option: %s", neon_moe_last_error(L.moe));
         }
     }
+    else if (!strcmp(name, "kv_bits")) return set_kv_bits(h, value);
     else if (!strcmp(name, "stop_after_layer")) h->stop_after = (int)value;
     else return dfail(h, NEON_MOE_EINVAL, "unknown option '%s'", name);
     return NEON_MOE_OK;
@@ -556,7 +735,7 @@ int neon_decoder_step_bytes(neon_decoder_handle* h, const int32_t* positions_hos
         for (int b = 0; b < batch; ++b) {
             const int p = positions_host[b];
             const int n = (c.window > 0 && l % 2 == 0) ? std::min(p + 1, c.window) : p + 1;
-            kv += (double)n * c.n_kv_heads * 64 * 2 * 2;
+            kv += (double)n * c.n_kv_heads * (h->kv4.on() ? 2 * (32 + 2) : 64 * 2 * 2);
         }
     const double per_expert = 2 * I * H / 2 + 2 * I * H / 32 + 2 * I * 2 + H * I / 2 + H * I / 32 + H * 2;
     double moe = 0;

@@ -74,6 +74,18 @@ class DecoderSystem:
                     "neon_decoder_load_kv")
 
     # -- execution -----------------------------------------------------------------------
+    def set_sampling(self, uniform=None, temperature=None, top_k=None, top_p=None, min_p=None) -> None:
+        """Next tokens are sampled from now on: device tensors of at least ``max_batch`` elements (fp32, ``top_k`` int32) that every
+        step reads as it runs and the caller may refill between steps.  Without arguments: the largest logit again."""
+        import torch
+        given = [uniform, temperature, top_k, top_p, min_p]
+        for t, dtype in zip(given, (torch.float32, torch.float32, torch.int32, torch.float32, torch.float32)):
+            if t is not None and (t.dtype is not dtype or t.numel() < self.max_batch or not t.is_contiguous() or t.get_device() != self.device):
+                raise ValueError(f"contiguous {dtype} tensors of at least {self.max_batch} elements on device {self.device}")
+        self._check(self._lib.neon_decoder_set_sampling(self._h, *[None if t is None else t.data_ptr() for t in given]),
+                    "neon_decoder_set_sampling")
+        self._sampling = given  # alive as long as steps may read them
+
     def step(self, tokens, positions, logits=None, next_tokens=None, stream=None):
         """One decode step over device tensors: ``tokens``/``positions`` torch int32 [B];
         optional ``logits`` fp32 [B, vocab] and ``next_tokens`` int32 [B] outputs."""

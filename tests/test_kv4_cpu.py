@@ -66,3 +66,8 @@ def test_restatement_stores_what_it_loads(P, D):
         # a rounding is off by at most half a step (the steps are 1/2, 1, 2 of the scale), or clips 8 to 6
         scale = ref.scale_of(byte).repeat_interleave(32, -1)
         assert ((value - x[which]).abs() <= torch.where(x[which].abs() > 6 * scale, 2.0, 1.0) * scale).all()
+
+
+def test_decoder_calls_without_a_handle(lib):
+    assert lib.neon_decoder_set_sampling(None, None, None, None, None, None) == 1
+    assert lib.neon_decoder_set_option(None, b"kv_bits", 4) == 1
