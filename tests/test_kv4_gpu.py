@@ -505,6 +505,51 @@ def test_results_belong_to_the_given_stream(systems):
     assert torch.equal(out, want) and torch.equal(k, want_k) and torch.equal(v, want_v)
 
 
+def test_captured_behind_copies_and_other_streams(systems):
+    """A graph in which append, attention and sampling follow a copy, a fill and work of another stream: each waits for them."""
+    from neonengine_b200.sampler import Sampler
+    kv, g, sampler = systems(16, 2, 64, 32), gen(33), Sampler(16 * 64)
+    batch, table, cu, pages = make_batch(kv, [1] * 8, [700] * 8, g, each=True)
+    first = random_cache(kv, pages, g)
+    given = torch.randn((8, 20, 64), generator=g, device=DEV).to(torch.bfloat16)
+    cache, x, uniform, f = torch.empty_like(first), torch.empty_like(given), torch.empty(8, device=DEV), inv_freq(64)
+    side = torch.cuda.Stream()
+
+    def run():
+        main = torch.cuda.current_stream()
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(200000)
+            cache.copy_(first)
+        x.copy_(given)
+        main.wait_stream(side)
+        q = kv.append(batch, cache, x[:, :16], x[:, 16:18], x[:, 18:], f)
+        uniform.zero_()
+        out = kv.attend(batch, cache, q)
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(200000)
+            uniform.fill_(0.5)
+        main.wait_stream(side)
+        return out, sampler.run(out.flatten(1), uniform)
+
+    out, tokens = (t.clone() for t in run())
+    torch.cuda.synchronize()
+    plain = kv.attend(batch, cache, kv.append(batch, cache, given[:, :16], given[:, 16:18], given[:, 18:], f))
+    assert torch.equal(out, plain) and torch.equal(tokens, sampler.run(out.flatten(1), torch.full((8,), 0.5, device=DEV)))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = run()
+    for _ in range(3):
+        cache.zero_()
+        x.zero_()
+        for t in held:
+            t.zero_()
+        graph.replay()
+        assert torch.equal(held[0], out) and torch.equal(held[1], tokens)
+    sampler.close()
+
+
 class Padded:
     """The system, with the queries of every attention call followed by rows that belong to no sequence: so many that the
     kernel for chunks of prompts is chosen (where heads are of 64)."""
