@@ -110,6 +110,7 @@ __global__ void __launch_bounds__(kAppendWarps * 32, 4) append_kernel(const Appe
     const int lane = threadIdx.x & 31, c = lane % kPieces;
     const int task = blockIdx.x * kAppendWarps + threadIdx.x / 32, row = task / p.split;
     pdl_wait();
+    pdl_launch_dependents();
     if (row >= p.b.rows) return;
     const int first_head = p.q ? 0 : p.s.nq, heads = p.s.nq + 2 * p.s.nkv, v_head = p.s.nq + p.s.nkv;
     // this warp's rounds of kHeads heads
@@ -232,6 +233,7 @@ template <class OutT>
 __global__ void __launch_bounds__(128) read_kernel(const ReadParams p) {
     const int task = blockIdx.x * 4 + threadIdx.x / 32, row = task / p.split, lane = threadIdx.x & 31, D = p.s.D, per_head = D / 8, units = p.s.nkv * per_head;
     pdl_wait();
+    pdl_launch_dependents();
     if (row >= p.b.rows) return;
     const int2 at = locate(p.b, row);
     if (at.x < 0 || at.y < 0) return;
