@@ -467,6 +467,25 @@ __device__ uint32_t group_min(const Group<C>& g, uint32_t v, int slot) {
     return v;
 }
 
+// A CTA's elements of one bin, by their place in its shared memory: looking at them again costs little.
+constexpr int kFew = 1024;
+struct Few {
+    uint16_t* at;
+    uint32_t* count;  // may pass kFew: then all of the CTA's elements have to be looked at
+    const float* xs;
+    uint32_t i0;      // index of the first
+    __device__ __forceinline__ void add(uint32_t index) const {
+        const uint32_t j = atomicAdd(count, 1u);
+        if (j < kFew) at[j] = (uint16_t)(index - i0);
+    }
+    template <class Each, class F>
+    __device__ __forceinline__ void each(Each all, F f) const {
+        const uint32_t n = *count;
+        if (n > kFew) return all(f);
+        for (uint32_t j = threadIdx.x; j < n; j += blockDim.x) f(xs[at[j]], i0 + at[j]);
+    }
+};
+
 struct Cut {  // the last kept token: its key, and its index among equals
     uint32_t key, index;
     __device__ __forceinline__ bool keeps(uint32_t k, uint32_t i) const { return k < key || (k == key && i <= index); }
@@ -475,7 +494,8 @@ struct Cut {  // the last kept token: its key, and its index among equals
 // top_k's and top_p's cut of a row whose elements the group holds: each(f) calls f(logit, index) for this thread's, `have` are
 // listed in all.  whole: the weight of all tokens.  Elements below `bound` may be missing; false: they are needed.
 template <int C, class Each>
-__device__ bool find_cut(const Group<C>& g, const Params& p, const Rule& r, u64 have, u64 whole, float bound, float lowest, Each each, Cut& cut) {
+__device__ bool find_cut(const Group<C>& g, const Params& p, const Rule& r, u64 have, u64 whole, float bound, float lowest, Each each, Cut& cut,
+                         const Few& few = Few{}) {
     cut = {0xffffffffu, 0xffffffffu};
     auto one = [] { return 1ull; };
     // the last of `n` among the equal ones at a key
@@ -508,15 +528,18 @@ __device__ bool find_cut(const Group<C>& g, const Params& p, const Rule& r, u64 
             g.clear();
             each([&](float x, uint32_t i) { if (x >= g.weight.low && cut.keeps(order_key(x), i)) g.add(bin(x), to_units(g.weight(x))); });
             const uint32_t b = g.reach(f, target, false);
+            if (threadIdx.x == 0) *few.count = 0;
+            __syncthreads();
             uint32_t lo = 0xffffffffu, hi = 0;
             each([&](float x, uint32_t i) {
+                if (!(x >= g.weight.low) || bin(x) != b) return;
                 const uint32_t k = order_key(x);
-                if (x >= g.weight.low && bin(x) == b && cut.keeps(k, i)) { lo = min(lo, k); hi = max(hi, k); }
+                if (cut.keeps(k, i)) { lo = min(lo, k); hi = max(hi, k); few.add(i); }
             });
-            lo = group_min(g, lo, 2);
+            lo = group_min(g, lo, 2);  // (with barriers: the list is complete)
             hi = ~group_min(g, ~hi, 3);
             f = first_key<C>(g, lo, hi, target, false, [&](auto f) {
-                each([&](float x, uint32_t i) { if (cut.keeps(order_key(x), i)) f(order_key(x), [&] { return to_units(g.weight(x)); }); });
+                few.each(each, [&](float x, uint32_t i) { if (cut.keeps(order_key(x), i)) f(order_key(x), [&] { return to_units(g.weight(x)); }); });
             }, f.before);
         } else {
             f = first_key<C>(g, first, last, target, false, [&](auto f) {
@@ -860,6 +883,8 @@ struct WholeSmem {
     uint32_t hist[3][kBins];
     u64 scratch[64];
     u64 parts[2][kPickThreads / 32];  // weights and counts of the warps' stretches
+    uint16_t few[kFew];
+    uint32_t n_few[4];
     double tab[kTable];
 };
 
@@ -925,7 +950,7 @@ __global__ void __cluster_dims__(kClusterCtas, 1, 1) __launch_bounds__(kPickThre
             }
         };
         Cut cut;
-        find_cut<kClusterCtas>(g, p, r, have, whole, -INFINITY, kLowest, each, cut);
+        find_cut<kClusterCtas>(g, p, r, have, whole, -INFINITY, kLowest, each, cut, Few{s.few, s.n_few, xs, (uint32_t)i0});
         // by index: the warps' stretches, then the token in one of them
         auto units = [&](int i) -> u64 {
             const float x = xs[i];
@@ -964,22 +989,23 @@ __global__ void __cluster_dims__(kClusterCtas, 1, 1) __launch_bounds__(kPickThre
             s.scratch[41] = goal - before;
         }
         prefix(number, s.scratch, kept);
-        if ((int)s.scratch[40] == rank * kWarps + warp) {
-            u64 run = 0;
+        const int owner = (int)s.scratch[40];
+        if (owner / kWarps == rank) {  // this CTA has the stretch: a few in a row to every thread
             const u64 rest = s.scratch[41];
-            for (int i = w0; i < w1; i += 32) {
-                const u64 mine_units = i + lane < w1 ? units(i + lane) : 0;
-                u64 upto = mine_units;
-#pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const u64 v = __shfl_up_sync(0xffffffffu, upto, o);
-                    if (lane >= o) upto += v;
+            const int o0 = min(owner % kWarps * stretch, n), o1 = min(o0 + stretch, n), each_has = (stretch + kPickThreads - 1) / kPickThreads;
+            const int t0 = min(o0 + tid * each_has, o1), t1 = min(t0 + each_has, o1);
+            u64 have_units = 0, of_stretch;
+            for (int i = t0; i < t1; ++i) have_units += units(i);
+            u64 run = prefix(have_units, s.scratch, of_stretch);
+            if (run <= rest && run + have_units > rest)
+                for (int i = t0; i < t1; ++i) {
+                    const u64 here = units(i);
+                    if (run + here > rest) {
+                        answer(p, row, i0 + i, (float)((double)here / (double)all), (int)kept);
+                        break;
+                    }
+                    run += here;
                 }
-                upto += run;
-                if (upto > rest && upto - mine_units <= rest) answer(p, row, i0 + i + lane, (float)((double)mine_units / (double)all), (int)kept);
-                run = __shfl_sync(0xffffffffu, upto, 31);
-                if (run > rest) break;
-            }
         }
         cluster.sync();  // the stretches' sums are read
     }
