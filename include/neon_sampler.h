@@ -19,8 +19,8 @@
  *   - The token is the first, by INDEX, whose running sum of kept weights exceeds uniform * (their sum); numbers
  *     outside [0, 1) are moved to its nearer end.
  *   - A row of which nothing can be drawn (all -infinity) gives token -1, probability 0, kept 0.
- * Weights are computed to 4e-11, rounded to 2^-43 of the largest and summed in 64-bit integers, so the result depends neither on the order of sums
- * nor on the batch around a row.
+ * Weights are computed to 4e-11 of their value (sums over all of a row: to 1e-9), rounded to 2^-43 of the largest and summed in
+ * 64-bit integers, so the result depends neither on the order of sums nor on the batch around a row.
  *
  * All functions return 0 or a NEON_MOE_E* code (neon_moe.h); none throws or aborts.
  */

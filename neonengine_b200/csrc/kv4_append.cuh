@@ -100,7 +100,8 @@ __device__ __forceinline__ uint32_t quantise8(const float (&x)[8], int& byte) {
 // The angle position * inv_freq is exact in 53 bits; it is reduced to a fraction of a turn before sine and cosine are
 // taken, so its error is 1e-16 of a turn per turn.  Keys are rotated in double precision: a code next to a rounding
 // border is then that of the formula, whatever the position (queries are rounded to 16 bits right away and take f32).
-// Memory bound from some hundred rows on: 15 KB a row at 64 + 8 + 8 heads of 64.  A row's chain of loads (offsets, length, page)
+// Memory bound from some hundred rows on (19 KB a row at 64 + 8 + 8 heads of 64; 13320 rows take 53 us, 4.8 TB/s; 8 rows 3.3 us, a chain
+// of loads).  A row's chain of loads (offsets, length, page)
 // and the sines hide behind the loads of the first pieces, and behind other warps: no barrier, no shared memory.
 constexpr int kAppendWarps = 4;
 template <int DT, class OutT, int D>
@@ -228,7 +229,8 @@ struct ReadParams {
     int split;  // warps per row
 };
 
-// A warp (or `split` of them) per row; a lane turns eight codes into values, 32 pieces of the row's heads at a time.
+// A warp (or `split` of them) per row; a lane turns eight codes into values, 32 pieces of the row's heads at a time.  Memory bound: 13320
+// rows of 8 + 8 heads of 64 to bf16 take 15 us (2.6 KB a row, 2.3 TB/s); a few rows 2 us.
 template <class OutT>
 __global__ void __launch_bounds__(128) read_kernel(const ReadParams p) {
     const int task = blockIdx.x * 4 + threadIdx.x / 32, row = task / p.split, lane = threadIdx.x & 31, D = p.s.D, per_head = D / 8, units = p.s.nkv * per_head;

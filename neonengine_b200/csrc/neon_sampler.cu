@@ -86,7 +86,8 @@ int launch(const void* logits, int dtype, long long row_stride, int vocab, int b
     p.entries = static_cast<uint2*>(workspace);
     p.heads = reinterpret_cast<ChunkHead*>(p.entries + n * kSlots);
     p.left = reinterpret_cast<int*>(p.heads + n);
-    // a warp lists some 1.4 times as many elements as lanes' maxima pass its bound; all warps' lists are to fit pick's
+    // A warp lists some 1.4 times as many elements as lanes' maxima pass its bound.  Longer lists let pick settle more rows, but all
+    // warps' together have to fit its list.
     p.rank = p.chunks <= 220 ? 16 : 8;
     const unsigned grid = (unsigned)std::min<size_t>((n + kScanWarps - 1) / kScanWarps, 2 * kSms);
     void (*scan)(Params) = dtype == NEON_SAMPLER_F32 ? scan_kernel<0> : dtype == NEON_SAMPLER_BF16 ? scan_kernel<1> : scan_kernel<2>;
