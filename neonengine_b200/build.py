@@ -16,9 +16,7 @@ APP = os.path.join(HERE, "moe_app")
 SOURCES = ["neon_moe.cu", "neon_decoder.cu", "neon_water.cu", "neon_svgf.cu", "neon_pt.cu", "neon_kv4.cu", "neon_kv4_prefill.cu",
            "neon_sampler.cu"]
 # the water step reproduces the reference shader's float arithmetic bit for bit: no fused multiply-add there
-SOURCE_FLAGS = {"neon_water.cu": ["-fmad=false"], "neon_svgf.cu": ["-fmad=false"], "neon_pt.cu": ["-fmad=false"],
-                # fifteen attention variants: compiled side by side
-                "neon_kv4.cu": ["-split-compile", "8"]}
+SOURCE_FLAGS = {"neon_water.cu": ["-fmad=false"], "neon_svgf.cu": ["-fmad=false"], "neon_pt.cu": ["-fmad=false"]}
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "-Xcompiler", "-fPIC", "-cudart", "static"]
 if os.environ.get("NEON_MOE_INSTRUMENT"):   # measurement aids (clock stamps, debug options); never in the shipped library
