@@ -15,7 +15,7 @@
 // What bounds it: neither pipe alone but the chain between them.  A step (256 rows, 64 positions) takes some 2400 clocks; the special
 // function units need 1024 of them for its exponentials, the products 900 (tf32 runs at half the bf16 rate, and 64 columns make
 // operands' reads from shared memory count), and some 5300 instructions go out, 0.55 a clock and scheduler.  Without the softmax's
-// arithmetic a step takes 1700.  Two prompts' chunks of 2048 rows over up to 8192 positions, 64 and 8 heads: 694 us, 0.47 PFLOP/s.
+// arithmetic a step takes 1700.  Two prompts' chunks of 2048 rows over up to 8192 positions, 64 and 8 heads: 692 us, 0.47 PFLOP/s.
 #pragma once
 #include "kv4_attend.cuh"
 
