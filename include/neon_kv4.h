@@ -27,11 +27,12 @@
  * before position 0 or behind the last sequence are not looked at; of the former attention writes
  * zeros, the latter are left as they were.  A page id outside [0, n_pages) or a length beyond the
  * table (table_width * P positions) never reaches memory: such positions are neither written nor
- * attended to, and neon_kv4_status() reports it.
+ * attended to, and neon_kv4_status() reports it.  Sequences may share pages (a common prefix), but no two rows of an
+ * append may stand at one place of the cache.  Outputs overlap no inputs.
  *
  * Calls only enqueue work and keep nothing between calls: any number of them may run at once on
  * several streams, and be captured into graphs, as long as no append writes pages that another
- * call reads.  All functions return 0 or a NEON_MOE_E* code (neon_moe.h); none throws or aborts.
+ * call reads.  A handle's calls come from one host thread at a time (its error text is one).  All functions return 0 or a NEON_MOE_E* code (neon_moe.h); none throws or aborts.
  */
 #ifndef NEON_KV4_H
 #define NEON_KV4_H

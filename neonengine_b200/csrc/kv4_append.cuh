@@ -132,7 +132,7 @@ __global__ void __launch_bounds__(kAppendWarps * 32, 4) append_kernel(const Appe
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int i = 0; i < (int)sizeof(Raw) / 32; ++i) r.v[h * (sizeof(Raw) / 32) + i] = __ldg(reinterpret_cast<const uint4*>(src + h * half) + i);
+            for (int i = 0; i < (int)sizeof(Raw) / 32; ++i) r.v[h * (sizeof(Raw) / 32) + i] = reinterpret_cast<const uint4*>(src + h * half)[i];
         return r;
     };
     Raw raw[kAhead];
@@ -249,8 +249,8 @@ __global__ void __launch_bounds__(128) read_kernel(const ReadParams p) {
         if (!o) continue;
         const uint8_t* rec = p.cache + (page * p.s.nkv + head) * p.s.record();
         uint32_t f[4];
-        codes_to_f16(__ldg(reinterpret_cast<const uint32_t*>(rec + is_v * p.s.codes() + slot * (D / 2) + c * 4)), f);
-        const float scale = scales_to_f32(__ldg(rec + 2 * p.s.codes() + is_v * p.s.scales() + slot * (D / 32) + c / 4)).x;
+        codes_to_f16(*reinterpret_cast<const uint32_t*>(rec + is_v * p.s.codes() + slot * (D / 2) + c * 4), f);
+        const float scale = scales_to_f32(rec[2 * p.s.codes() + is_v * p.s.scales() + slot * (D / 32) + c / 4]).x;
         float x[8];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {

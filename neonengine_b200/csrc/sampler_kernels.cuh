@@ -92,7 +92,7 @@ __device__ __forceinline__ Rule rule_of(const Params& p, int row) {
 __device__ __forceinline__ float clean(float x) { return fmaxf(x, -INFINITY); }  // NaN is -infinity
 __device__ __forceinline__ float load1(const Params& p, long long i) {
     float x;
-    if (p.dtype == 0) x = __ldg(static_cast<const float*>(p.logits) + i);
+    if (p.dtype == 0) x = static_cast<const float*>(p.logits)[i];
     else if (p.dtype == 1) x = __bfloat162float(static_cast<const __nv_bfloat16*>(p.logits)[i]);
     else x = __half2float(static_cast<const __half*>(p.logits)[i]);
     return clean(x);

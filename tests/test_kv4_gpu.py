@@ -505,6 +505,49 @@ def test_results_belong_to_the_given_stream(systems):
     assert torch.equal(out, want) and torch.equal(k, want_k) and torch.equal(v, want_v)
 
 
+@pytest.mark.parametrize("nq,nkv,D,P,n", [(8, 2, 64, 16, 1024), (128, 128, 64, 64, 3), (32, 1, 128, 32, 1024)])
+def test_largest_batches_and_head_counts(systems, nq, nkv, D, P, n):
+    """As many sequences and key/value heads as there can be: appended, read back, attended to, by chunks too."""
+    kv, g = systems(nq, nkv, D, P), gen(n + nq)
+    lens = [1 + i * 7 % 90 for i in range(n)]
+    batch, table, cu, pages = make_batch(kv, [1] * n, lens, g, each=True)
+    cache = random_cache(kv, pages, g)
+    x = torch.randn((n, nq + 2 * nkv, D), generator=g, device=DEV).to(torch.bfloat16)
+    f = inv_freq(D)
+    q = kv.append(batch, cache, x[:, :nq], x[:, nq:nq + nkv], x[:, nq + nkv:], f)
+    vals, _, value = ref.quantise(x[:, nq + nkv:].double())
+    assert torch.equal(kv.read(batch, cache, dtype=torch.float32)[1].double(), value)
+    some = torch.tensor([0, 1, 2, n // 2, n - 1], device=DEV).unique()
+    outs = [kv.attend(batch, cache, q)]
+    if D == 64:  # behind a window that hides nothing the chunk kernel is chosen
+        wide, held, launched = torch.zeros((n + 64, nq, D), dtype=q.dtype, device=DEV), torch.full((n + 64, nq, D), 7.0, dtype=q.dtype, device=DEV), kv.launch_count
+        wide[:n] = q
+        outs.append(kv.attend(batch, cache, wide, window=100, max_rows=64, out=held)[:n])
+        assert kv.launch_count == launched + 1 and (held[n:] == 7.0).all()
+    for out in outs:
+        for b in some.tolist():
+            page = table[b, :-(-lens[b] // P)].long()
+            k, v = (ref.load(cache, P, D, page, lens[b], i) for i in range(2))
+            want, mass = ref.attend(q[b:b + 1], k, v, torch.tensor([lens[b] - 1], device=DEV), None, 0, D ** -0.5)
+            tol = 2 ** -8 * want.abs() + (2 ** -11 + 2 ** -13) * mass * 1.01 + lens[b] * 2 ** -25 * v.abs().amax()
+            assert ((out[b:b + 1].double() - want).abs() <= tol).all()
+
+
+def test_sequences_share_pages(systems):
+    """A common prefix: two tables name the same pages, and each sequence has a last page of its own."""
+    kv, g = systems(8, 2, 64, 32), gen(34)
+    cache = random_cache(kv, 5, g)
+    lens, table = [70, 75], torch.tensor([[3, 1, 0], [3, 1, 4]], dtype=torch.int32, device=DEV)
+    cu = torch.tensor([0, 1, 2], dtype=torch.int32, device=DEV)
+    batch = kv.batch(torch.tensor(lens, dtype=torch.int32, device=DEV), table)
+    x = torch.randn((2, 12, 64), generator=g, device=DEV).to(torch.bfloat16)
+    before = cache.clone()
+    q = kv.append(batch, cache, x[:, :8], x[:, 8:10], x[:, 10:], inv_freq(64))
+    assert torch.equal(cache[[1, 2, 3]], before[[1, 2, 3]])
+    out = kv.attend(batch, cache, q)
+    check_attention(kv, batch, table, cu, [1, 1], lens, cache, q, None, 0, 0.125, out)
+
+
 def test_captured_behind_copies_and_other_streams(systems):
     """A graph in which append, attention and sampling follow a copy, a fill and work of another stream: each waits for them."""
     from neonengine_b200.sampler import Sampler

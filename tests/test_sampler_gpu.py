@@ -139,6 +139,22 @@ def test_special_values(samplers, vocab):
     check(s, x, u, p=[-1.0] * 14)
 
 
+@pytest.mark.parametrize("vocab", [20011, 201088])
+def test_few_values_and_extreme_temperatures(samplers, vocab):
+    """Thousands of equal logits about the cut, and temperatures from next to nothing to infinity."""
+    n = 9
+    g = torch.Generator(device=DEV)
+    g.manual_seed(vocab)
+    x = -0.5 * torch.randint(0, 4, (n, vocab), generator=g, device=DEV).float()
+    x[5:] = torch.randn((n - 5, vocab), generator=g, device=DEV)
+    u = torch.rand((n,), generator=g, device=DEV).tolist()
+    t = [1.0, 0.3, 5.0, float("inf"), 1e-30, 1e-38, 1e30, float("inf"), 1e-3]
+    p = [0.9, 0.4, 0.97, 0.5, 0.5, 0.3, 0.9, 0.25, 0.9]
+    check(samplers(vocab), x, u, t=t, p=p)
+    check(samplers(vocab), x, u, t=t, p=p, k=[0, 30000, 0, 9000, 0, 7, 0, 12345, 0])
+    check(samplers(vocab), x, u, t=t)
+
+
 @pytest.mark.parametrize("order", ["descending", "ascending", "one chunk"])
 def test_likely_tokens_side_by_side(samplers, order):
     """The largest logits lie together, where a warp's list cannot hold them."""
