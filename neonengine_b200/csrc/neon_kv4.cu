@@ -87,14 +87,14 @@ constexpr int kSms = 148, kSharedPerSm = 227 * 1024;
 
 // Columns of an item's products, in groups of eight.  More of them read, convert and scale the cache less often; fewer need fewer
 // registers, so that two CTAs fit a multiprocessor.  64 sequences of 4000 positions, 8 key/value heads, us by groups of columns:
-//   heads of 64    8 rows an item: 48 (1), 100 (4)    16 rows: 83 (1), 91 (2), 104 (4)    32 rows: 149 (1), 110 (4)
-//   heads of 128   8 rows: 80 (1), 102 (2)            16 rows: 144 (1), 111 (2)
+//   heads of 64    8 rows an item: 46 (1), 101 (4)    16 rows: 80 (1), 86 (2), 107 (4)    32 rows: 143 (1), 146 (2), 111 (4)
+//   heads of 128   8 rows: 77 (1), 102 (2)            16 rows: 142 (1), 106 (2)
 int column_groups(const Shape& s, int max_rows) {
     const long long rows = (long long)std::max(max_rows, 1) * (s.nq / s.nkv);
     if (s.D == 128) return rows <= 8 ? 1 : 2;
     return rows <= 16 ? 1 : 4;
 }
-// one instead of two, with eight rows of 64: 55 us instead of 48
+// one instead of two, with eight rows of 64: 54 us instead of 46
 int ctas_per_sm(const Shape& s, int nt) { return s.D == 64 && nt == 1 ? 2 : 1; }
 int attend_grid(const Shape& s, const Batch& b, int nt) {
     const long long steps = ((long long)b.width * s.P + kStep - 1) / kStep;
