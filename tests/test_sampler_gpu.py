@@ -231,6 +231,24 @@ def test_captured_and_on_two_streams(samplers):
             assert all(torch.equal(a, b) for a, b in zip(out, s.run(*w, details=True)))
 
 
+def test_results_belong_to_the_given_stream(samplers):
+    """A run on another stream while the current one still has to write to memory that it freed: the result is not in it."""
+    x, u = rows_of(8, 20011, 77)
+    u = f32(u)
+    s, other = samplers(20011), torch.cuda.Stream()
+    want = s.run(x, u, top_p=f32([0.9] * 8), details=True)
+    p = f32([0.9] * 8)
+    torch.cuda.synchronize()
+    freed = [torch.empty_like(t) for t in want]
+    torch.cuda._sleep(20000000)
+    for t in freed:
+        t.fill_(3)
+    del freed, t
+    got = s.run(x, u, top_p=p, details=True, stream=other)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def test_refusals(samplers):
     s = samplers(1000)
     x, u = torch.zeros((3, 1000), device=DEV), torch.zeros((3,), device=DEV)
