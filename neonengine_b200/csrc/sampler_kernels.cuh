@@ -165,9 +165,10 @@ __device__ __forceinline__ u64 to_units(double w) {  // w <= 2^9, in 2^-43, roun
     return (u64)(__double_as_longlong(fma(w, kUnit, 4503599627370496.0)) & 0xfffffffffffffll);
 }
 
-// A chunk's weight, relative to the row's largest.
+// A chunk's weight, relative to the row's largest.  Nothing where its largest logit rounds to nothing, since no token of it can be drawn
+// then: the sum is one of weights that are not rounded.
 __device__ __forceinline__ u64 chunk_units(const ChunkHead& h, const Weigher& w) {
-    if (h.max == -INFINITY) return 0;
+    if (h.max == -INFINITY || to_units(w(h.max)) == 0) return 0;
     const double factor = h.exponent == kRelative ? w(h.max) : exp2((64.0 * h.exponent + w.off) * (1.0 / 64.0));
     return (u64)(h.weight * factor * kUnit);
 }
