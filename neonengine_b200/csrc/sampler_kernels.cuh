@@ -142,9 +142,9 @@ struct Weigher {
 struct Adder {
     float hi, lo, low;  // 64 log2(e) / temperature as two f32
     const double* tab;
-    bool fits;          // the powers are within f64's range, and `low` is below the largest by what it should be
+    bool fits;          // the powers are within f64's range and the scale within f32's, and `low` is below the largest by what it should be
     __device__ __forceinline__ Adder(const Weigher& w) : hi((float)w.c), lo((float)(w.c - (double)(float)w.c)), low(w.low), tab(w.tab) {
-        fits = fabs(w.off) < 64.0 * 900 && w.top < INFINITY && (double)w.top * w.c - (double)w.low * w.c > 64.0 * 55;
+        fits = hi < INFINITY && fabs(w.off) < 64.0 * 900 && w.top < INFINITY && (double)w.top * w.c - (double)w.low * w.c > 64.0 * 55;
     }
     __device__ __forceinline__ float steps(float x) const { return fmaf(x, hi, 12582912.f); }  // 1.5 * 2^23 + the product's integer part
     __device__ __forceinline__ void add(double& sum, float x) const {

@@ -74,3 +74,26 @@ def test_light_logits_before_behind_and_between(vocab):
     token, _, kept = run(s, x, u, top_p=f32([0.999999] * n))
     assert token == [5000] * n and kept == [2] * n
     s.close()
+
+
+@pytest.mark.parametrize("vocab", [7169, 20011, 201088])
+@pytest.mark.parametrize("t", [1e-36, 1e-37, 2e-38, 1e-38, 1e-44])
+def test_temperatures_whose_scale_leaves_f32(vocab, t):
+    """The largest logit is exactly zero and the temperature next to nothing: the zeros share everything."""
+    from neonengine_b200.sampler import Sampler
+    g = torch.Generator(device=DEV)
+    g.manual_seed(vocab)
+    zeros = sorted({1, 1500, vocab // 2, vocab - 3})
+    x = -1 - torch.rand((6, vocab), generator=g, device=DEV)
+    x[:, zeros] = 0.0
+    u = [0.0, 0.2, 0.3, 0.6, 0.8, 0.999]
+    want = [zeros[int(v * len(zeros))] for v in u]
+    s = Sampler(vocab)
+    temperature = f32([t] * 6)
+    token, prob, kept = run(s, x, u, temperature=temperature)
+    assert token == want and all(abs(p - 1 / len(zeros)) < 1e-7 for p in prob) and kept == [vocab] * 6
+    token, prob, kept = run(s, x, u, temperature=temperature, top_p=f32([0.9] * 6))
+    assert token == want and kept == [len(zeros)] * 6
+    token, prob, kept = run(s, x, u, temperature=temperature, top_p=f32([0.4] * 6))  # reached by the second of them
+    assert token == [zeros[int(v * 2)] for v in u] and kept == [2] * 6
+    s.close()
