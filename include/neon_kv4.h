@@ -108,10 +108,12 @@ uint64_t neon_kv4_attend_workspace(neon_kv4_handle* h, const neon_kv4_batch* bat
  * p <= the row's own (and > own - window where window > 0); query head j reads key/value head
  * j / (n_q_heads / n_kv_heads).  q (rows q_stride elements apart) and out ([rows, n_q_heads, D] contiguous):
  * dtype BF16 or F16.  sinks: bf16 [n_q_heads] or NULL.  Rows that see no position get zeros.
- * Value scales above 2^125, which only infinities give, count as 2^125.  From scores or values of about 2^110 on a row's
- * sums may leave the range of fp32; it is infinite or NaN then.
- * max_rows: the most rows that a sequence has, as far as the host knows it; it chooses the kernel, results do
- * not depend on it. */
+ * Value scales above 2^125, which only infinities give, count as 2^125.  From values of about 2^110 on a row's sums
+ * may leave the range of fp32; it is infinite or NaN then.  Scores are fp32 sums of exact products, good to 2^-23 of
+ * their size; from 2^22 on a row may be zero, infinite or NaN.  Each probability is rounded to 11 bits (12 where a
+ * sequence has few rows), and the bits that small ones lose are 2^-8 of the sum of weights times values' scales at most.
+ * max_rows: the most rows that a sequence has, as far as the host knows it; it chooses the kernel, so results
+ * depend on it by these roundings. */
 int neon_kv4_attend(neon_kv4_handle* h, const neon_kv4_batch* batch, const void* cache, int rows, int dtype,
                     const void* q, int64_t q_stride, const void* sinks, int window, float scale, int max_rows,
                     void* out, void* workspace, uint64_t workspace_bytes, void* cuda_stream);

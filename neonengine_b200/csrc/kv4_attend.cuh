@@ -13,12 +13,16 @@
 //   scale is exact.  Queries are f16, every row scaled by a power of two so that its largest value lies in [2^14, 2^15):
 //   exact for bf16 and f16 down to 2^-28 of the largest.
 //   Values: a pair of positions of one column is one f16x2 operand, multiplied by the two positions' scales relative to
-//   the largest scale met so far (outputs are rescaled when it grows).  Where scales lie further apart than 2^7, or grow
-//   by more than 2^2, a probability that f16 rounds away could belong to a value that counts: such a step's values are
-//   added in f32, one position at a time (five times as long, and rare), so no spread of scales loses anything.
-//   Probabilities are rounded to f16 (2^-12), once; sums and statistics are f32, and the softmax sum is one more product, with
-//   a row of ones.  The running maximum is raised only when a probability relative to it exceeds 2^8, so that most steps
-//   need no exchange between lanes but one vote.
+//   the largest scale met so far (outputs are rescaled when it grows).  Where a step's scales lie more than 2^7 below it, its
+//   values are added in f32, one position at a time (five times as long, and rare).
+//   Probabilities are f16, relative to a level of their row: a group (the 64 or 32 positions weighed at once) whose largest exceeds 2^15
+//   raises it, to 2^8 below.  So a probability is rounded by 2^-12 of itself or by 2^-25, and the row's sum is 2^7 or more.  With value
+//   scales 2^apart apart at most, n positions lose n * 2^(apart - 32) of the sum of weights times scales: 2^-9, once n * 2^apart is 2^23
+//   (kCareful: 65536 positions of a warp's run at scales within 2^7).  From there on a group whose largest is below 1 lowers
+//   the level, to 2^5 below it: then what a group loses is 2^-12 of its own, wherever the row's largest stands and whatever its value is.
+//   Lowering ends where it takes the sum to 2^30; a group that needs more loses 2^-49 of the sum, and where scales lie further
+//   apart than 2^24 it is added in f32.  Levels are whole numbers, so that rescaling is exact.
+//   The softmax sum is one more product, with a row of ones.  Most steps need no exchange between lanes but one vote.
 // Steps travel by bulk copies (one per page and head: a record is contiguous) into a ring per warp.
 // What bounds it at G = 8: not the memory but issue slots and the conversions (two codes each, 64 lanes a clock and SM).  Measured with 64
 // query and 8 key/value heads of 64: 64 sequences of 200 to 32768 positions 123 us for 476 MB, 3.9 TB/s (streaming the records alone 87,
@@ -32,10 +36,15 @@ namespace neon {
 namespace kv4 {
 
 constexpr int kStep = 64;             // positions of a step
-constexpr float kNoMax = -1e30f;      // running maximum before the first score
+constexpr float kNoMax = -1e30f;      // level before the first score
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr uint32_t kRaise = 0x5c00;   // f16 2^8: what a probability relative to the running maximum may reach
-constexpr int kSpread = 7, kGrowth = 2;  // how far (log2) value scales may lie below the largest, and the largest may grow, for f16 operands
+// where (log2) the largest probability of a group may lie, as f16 pairs too, and where it is put when it does not
+constexpr float kHigh = 15.f, kLow = 0.f, kRaiseTo = 8.f, kLowerTo = 5.f;
+constexpr uint32_t kHighest = 0x78007800u, kLowest = 0x3c003c00u;
+constexpr int kSpread = 7;         // how far (log2) a step's value scales may lie below the largest for f16 operands
+constexpr int kCareful = 1 << 23;  // positions times how far the run's scales lie apart before small probabilities are looked after
+constexpr int kMostSum = 30;       // (log2) how far lowering its level may take a row's sum
+constexpr int kWide = 24;          // (log2) how far apart the run's scales may lie for what a group loses then not to count
 
 struct AttendParams {
     Batch b;
@@ -141,11 +150,17 @@ __device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
     asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
     return d;
 }
-__device__ __forceinline__ uint32_t max_f16x2(uint32_t a, uint32_t b) {
+__device__ __forceinline__ uint32_t max_f16x2(uint32_t a, uint32_t b) {  // passes over NaN
     uint32_t d;
     asm("max.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
     return d;
 }
+__device__ __forceinline__ uint32_t min_f16x2(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("min.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
+__device__ __forceinline__ __half2 as_half2(uint32_t v) { return *reinterpret_cast<__half2*>(&v); }
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -153,6 +168,12 @@ __device__ __forceinline__ float ex2(float x) {
 }
 // 2^e for -126 <= e <= 127, 0 below, infinity above
 __device__ __forceinline__ float pow2i(int e) { return __uint_as_float((uint32_t)min(max(e + 127, 0), 255) << 23); }
+
+// floor(log2 x) of a positive x; 0 of infinities and NaN
+__device__ __forceinline__ int log2_of(float x) {
+    const int e = (int)(__float_as_uint(x) >> 23) - 127;
+    return e < 128 ? e : 0;
+}
 
 __device__ __forceinline__ bool wait_bounded(uint64_t* bar, int parity) {
     if (sm100::mbar_test(bar, parity)) return true;
@@ -347,7 +368,8 @@ __global__ void __launch_bounds__(kAttendWarps * 32, (D == 64 && NT == 1) ? 2 : 
                 l[j][0] = l[j][1] = l[j][2] = l[j][3] = 0.f;
                 m[j][0] = m[j][1] = kNoMax;
             }
-            int ve[NB];  // largest value scale so far (its byte), per block
+            int ve[NB];          // largest value scale so far (its byte), per block
+            int apart = kSpread;  // how far below it others were, at most
 #pragma unroll
             for (int b = 0; b < NB; ++b) ve[b] = 0;
             const int n = min(q.steps - step, left);
@@ -356,7 +378,9 @@ __global__ void __launch_bounds__(kAttendWarps * 32, (D == 64 && NT == 1) ? 2 : 
             const int see_begin = first / kStep, see_end = pos_hi < 0 ? 0 : pos_hi / kStep + 1;
             const int open_begin = p.window > 0 ? ((pos_hi - p.window) >> 6) + 1 : 0, open_end = (min(pos_lo, q.len - 1) + 1) >> 6;
 
-            for (int at_step = q.lo_step + step, end_step = at_step + n; at_step < end_step; ++at_step) {
+            const int first_step = q.lo_step + step;
+            int careful_from = first_step + (kCareful >> kSpread) / kStep;
+            for (int at_step = first_step, end_step = at_step + n; at_step < end_step; ++at_step) {
                 const int p0 = at_step * kStep;  // first position of the step
                 if (!wait_bounded(&full[stage], phase)) {
                     timeout = true;
@@ -402,6 +426,7 @@ __global__ void __launch_bounds__(kAttendWarps * 32, (D == 64 && NT == 1) ? 2 : 
                     }
                     bool plain = true;  // f16 operands do
                     if (__any_sync(0xffffffffu, below > (uint32_t)kSpread)) {  // (kSpread has all its bits set)
+                        int grown = 0, under = 0;
 #pragma unroll
                         for (int b = 0; b < NB; ++b) {
                             for (int i = 0; i < 2; ++i) vb[b][i] = vb[b][i] > kTopScale && vb[b][i] < 255 ? kTopScale : vb[b][i];
@@ -428,7 +453,7 @@ __global__ void __launch_bounds__(kAttendWarps * 32, (D == 64 && NT == 1) ? 2 : 
                             }
                             const int low = __reduce_min_sync(0xffffffffu, min(vb[b][0] < 0 ? 999 : vb[b][0], vb[b][1] < 0 ? 999 : vb[b][1]));
                             if (top > ve[b]) {
-                                plain = plain && (ve[b] == 0 || top - ve[b] <= kGrowth);
+                                if (ve[b] > 0) grown = max(grown, top - ve[b]);
                                 const float f = pow2i(ve[b] - top);
                                 ve[b] = top;
 #pragma unroll
@@ -439,8 +464,11 @@ __global__ void __launch_bounds__(kAttendWarps * 32, (D == 64 && NT == 1) ? 2 : 
                                             o[j][i][0] *= f; o[j][i][1] *= f; o[j][i][2] *= f; o[j][i][3] *= f;
                                         }
                             }
-                            plain = plain && ve[b] - low <= kSpread;
+                            under = max(under, ve[b] - low);
                         }
+                        plain = under <= kSpread;
+                        apart = max(apart + grown, under);
+                        careful_from = first_step + (kCareful >> min(apart, 31)) / kStep;
                     }
                     // scales relative to the largest: 1 .. 2^-7 (anything finite where no row looks)
 #pragma unroll
@@ -507,12 +535,29 @@ __global__ void __launch_bounds__(kAttendWarps * 32, (D == 64 && NT == 1) ? 2 : 
 #pragma unroll
                                     for (int h = 0; h < 2; ++h) {
                                         pf[j][i][h] = pack2(ex2(argument(j, i, 2 * h)), ex2(argument(j, i, 2 * h + 1)), __half());
-                                        top = max_f16x2(top, pf[j][i][h]);  // passes over NaN
+                                        top = max_f16x2(top, pf[j][i][h]);
                                     }
                         };
                         weigh();
-                        // probabilities are not negative: their bits are in order
-                        if (__any_sync(0xffffffffu, max(top & 0xffffu, top >> 16) > kRaise)) {
+                        bool exact = !plain;  // values in f32
+                        bool move = __any_sync(0xffffffffu, !__hble2(as_half2(top), as_half2(kHighest)));
+                        const bool careful = at_step >= careful_from;
+                        if (careful) {  // is the largest of each column large enough, too?
+                            uint32_t least = kHighest;
+#pragma unroll
+                            for (int j = 0; j < NT; ++j) {
+                                uint32_t most = 0;  // of each of two columns
+#pragma unroll
+                                for (int i = 0; i < TI; ++i) most = max_f16x2(most, max_f16x2(pf[j][i][0], pf[j][i][1]));
+#pragma unroll
+                                for (int off = 4; off < 32; off <<= 1) most = max_f16x2(most, __shfl_xor_sync(0xffffffffu, most, off));
+                                least = min_f16x2(least, most);
+                            }
+                            move = move || __any_sync(0xffffffffu, !__hbge2(as_half2(least), as_half2(kLowest)));
+                        }
+                        if (move) {
+                            bool moved = false, lost = false;
+                            float f[NT][2];
 #pragma unroll
                             for (int j = 0; j < NT; ++j)
 #pragma unroll
@@ -523,16 +568,31 @@ __global__ void __launch_bounds__(kAttendWarps * 32, (D == 64 && NT == 1) ? 2 : 
                                     for (int i = 0; i < TI; ++i) x = fmaxf(x, fmaxf(sc[j][i][c] * factor, sc[j][i][c + 2] * factor));
 #pragma unroll
                                     for (int off = 4; off < 32; off <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, off));
-                                    const float now = fmaxf(m[j][c], x), f = ex2(m[j][c] - now);
+                                    const float old = m[j][c];
+                                    float now = x > old + kHigh ? rintf(x) - kRaiseTo : old;
+                                    if (careful && x < old + kLow && x > -INFINITY) {
+                                        now = fmaxf(rintf(x) - kLowerTo, old - (float)max(kMostSum - max(log2_of(l[j][c]), 0), 0));
+                                        lost = lost || x < now + kLow;
+                                    }
+                                    moved = moved || now != old;
+                                    f[j][c] = pow2i((int)(old - now));
                                     m[j][c] = now;
-                                    l[j][c] *= f;
-#pragma unroll
-                                    for (int i = 0; i < D / 16; ++i) { o[j][i][c] *= f; o[j][i][c + 2] *= f; }
                                 }
-                            weigh();
+                            if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+                                for (int j = 0; j < NT; ++j)
+#pragma unroll
+                                    for (int c = 0; c < 2; ++c) {
+                                        l[j][c] *= f[j][c];
+#pragma unroll
+                                        for (int i = 0; i < D / 16; ++i) { o[j][i][c] *= f[j][c]; o[j][i][c + 2] *= f[j][c]; }
+                                    }
+                                weigh();
+                            }
+                            exact = exact || (apart > kWide && __any_sync(0xffffffffu, lost));
                         }
                         // ---- values ------------------------------------------------------------------------------------------
-                        if (plain) {
+                        if (!exact) {
 #pragma unroll
                             for (int i = 0; i < TI; ++i) {
                                 const int tile = 16 * (i0 + i);
