@@ -358,7 +358,7 @@ __global__ void __launch_bounds__(kAttendWarps * 32, (D == 64 && NT == 1) ? 2 : 
             // what column c sees: positions above sees_lo(c), up to sees_hi(c)
             auto sees_hi = [&](int c) { return c < rows ? min(q.pos0 + p.token(r0 + c), q.len - 1) : -1; };
             auto sees_lo = [&](int c) { return p.window > 0 ? q.pos0 + p.token(r0 + c) - p.window : -1; };
-            const int pos_lo = q.pos0 + p.token(r0), pos_hi = min(q.pos0 + p.token(r0 + rows - 1), q.len - 1);
+            const int pos_lo = q.pos0 + p.token(r0), pos_last = q.pos0 + p.token(r0 + rows - 1), pos_hi = min(pos_last, q.len - 1);
             const int first = p.window > 0 ? max(pos_lo - p.window + 1, 0) : 0;
             float o[NT][D / 16][4], l[NT][4], m[NT][2];
 #pragma unroll
@@ -376,7 +376,7 @@ __global__ void __launch_bounds__(kAttendWarps * 32, (D == 64 && NT == 1) ? 2 : 
             const bool starts = step == 0, ends = step + n == q.steps;
             // steps that any row sees a position of; steps of which every row sees every position
             const int see_begin = first / kStep, see_end = pos_hi < 0 ? 0 : pos_hi / kStep + 1;
-            const int open_begin = p.window > 0 ? ((pos_hi - p.window) >> 6) + 1 : 0, open_end = (min(pos_lo, q.len - 1) + 1) >> 6;
+            const int open_begin = p.window > 0 ? ((pos_last - p.window) >> 6) + 1 : 0, open_end = (min(pos_lo, q.len - 1) + 1) >> 6;
 
             const int first_step = q.lo_step + step;
             int careful_from = first_step + (kCareful >> kSpread) / kStep;
