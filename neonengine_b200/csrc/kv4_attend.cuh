@@ -62,6 +62,8 @@ struct AttendParams {
     uint32_t G_inverse;  // ceil(2^32 / G)
     // r / G for r < 2^26, exact as G <= 32
     __device__ __forceinline__ int token(int r) const { return G == 1 ? r : (int)__umulhi((uint32_t)r, G_inverse); }
+    // first position that a row at `pos` may see (pos may be below 0, the window any number)
+    __device__ __forceinline__ int first_seen(int pos) const { return window > 0 && pos >= window ? pos - window + 1 : 0; }
 };
 
 constexpr int kAttendWarps = 8;
@@ -82,7 +84,7 @@ __device__ __forceinline__ SeqPlan plan_of(const AttendParams& p, int s) {
     const int full = p.b.seq_lens[s];
     r.len = max(min(full, p.b.width * p.s.P), 0);
     r.pos0 = full - r.n;
-    const int lo = p.window > 0 ? max(r.pos0 - p.window + 1, 0) : 0;
+    const int lo = p.first_seen(r.pos0);
     r.lo_step = lo / kStep;
     r.blocks = r.n > 0 ? (r.n * p.G + p.R - 1) >> (31 - __clz(p.R)) : 0;  // R is a power of two
     r.steps = r.n > 0 && r.len > lo ? (r.len + kStep - 1) / kStep - r.lo_step : 0;
@@ -357,9 +359,9 @@ __global__ void __launch_bounds__(kAttendWarps * 32, (D == 64 && NT == 1) ? 2 : 
             }
             // what column c sees: positions above sees_lo(c), up to sees_hi(c)
             auto sees_hi = [&](int c) { return c < rows ? min(q.pos0 + p.token(r0 + c), q.len - 1) : -1; };
-            auto sees_lo = [&](int c) { return p.window > 0 ? q.pos0 + p.token(r0 + c) - p.window : -1; };
+            auto sees_lo = [&](int c) { return p.first_seen(q.pos0 + p.token(r0 + c)) - 1; };
             const int pos_lo = q.pos0 + p.token(r0), pos_last = q.pos0 + p.token(r0 + rows - 1), pos_hi = min(pos_last, q.len - 1);
-            const int first = p.window > 0 ? max(pos_lo - p.window + 1, 0) : 0;
+            const int first = p.first_seen(pos_lo);
             float o[NT][D / 16][4], l[NT][4], m[NT][2];
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
@@ -376,7 +378,7 @@ __global__ void __launch_bounds__(kAttendWarps * 32, (D == 64 && NT == 1) ? 2 : 
             const bool starts = step == 0, ends = step + n == q.steps;
             // steps that any row sees a position of; steps of which every row sees every position
             const int see_begin = first / kStep, see_end = pos_hi < 0 ? 0 : pos_hi / kStep + 1;
-            const int open_begin = p.window > 0 ? ((pos_last - p.window) >> 6) + 1 : 0, open_end = (min(pos_lo, q.len - 1) + 1) >> 6;
+            const int open_begin = (p.first_seen(pos_last) + kStep - 1) / kStep, open_end = (min(pos_lo, q.len - 1) + 1) >> 6;
 
             const int first_step = q.lo_step + step;
             int careful_from = first_step + (kCareful >> kSpread) / kStep;

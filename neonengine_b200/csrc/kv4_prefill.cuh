@@ -195,7 +195,7 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1) prefill_kernel(const Attend
     const SeqPlan q = plan_of(one, seq);
     const int r0 = s.item[1] * kPreRows, rows = min(kPreRows, q.n * p.G - r0);
     const int pos_lo = q.pos0 + p.token(r0), pos_hi = min(q.pos0 + p.token(r0 + rows - 1), q.len - 1);
-    const int first = p.window > 0 ? max(pos_lo - p.window + 1, 0) : 0;
+    const int first = p.first_seen(pos_lo);
     const int step0 = first / kStep, n = pos_hi < first ? 0 : pos_hi / kStep + 1 - step0;
     // ---- queries, as bf16 terms -------------------------------------------------------------------------------------------
     const int tile = warp / 4;  // of a softmax warp
@@ -234,7 +234,7 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1) prefill_kernel(const Attend
 
     if (n > 0 && warp < kPreSoftmaxWarps) {
         // ---- softmax: this thread's row ------------------------------------------------------------------------------------
-        const int hi = tid < rows ? min(q.pos0 + token, q.len - 1) : -1, lo = p.window > 0 ? q.pos0 + token - p.window : -1;
+        const int hi = tid < rows ? min(q.pos0 + token, q.len - 1) : -1, lo = p.first_seen(q.pos0 + token) - 1;
         const float positive = fabsf(p.scale) * kLog2e, qs = positive == 0.f ? 1e-30f : positive;
         const uint32_t lanes = tmem + ((uint32_t)(warp & 3) << 21);  // this warp's lanes: 32 * (warp % 4) in the upper half
         float m = kNoMax, l[4] = {0.f, 0.f, 0.f, 0.f};

@@ -46,3 +46,20 @@ def test_sequences_longer_than_their_table(form, window):
         want, tol = expect(kv, cache, table[b], q[mine], n, length, window)
         assert ((out[mine].double() - want).abs() <= tol).all(), (b, length)
     kv.close()
+
+
+@pytest.mark.parametrize("form", [(16, 2, 64, 64), (16, 2, 128, 32)])
+@pytest.mark.parametrize("rows", [20, 90])
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 8, 2 ** 30])
+def test_largest_windows(form, rows, window):
+    """More rows than positions (the first see none) under a window as large as a number can be: as without one."""
+    lens = [11, 300]
+    kv, table, cache, q, cu, batch = world(*form, lens, [rows, rows], 300 // form[3] + 1, 3)
+    for max_rows in (1, rows, 100):
+        out, plain = (kv.attend(batch, cache, q, window=w, max_rows=max_rows) for w in (window, 0))
+        assert torch.equal(out, plain)
+        for b, length in enumerate(lens):
+            want, tol = expect(kv, cache, table[b], q[b * rows:(b + 1) * rows], rows, length, 0)
+            assert ((out[b * rows:(b + 1) * rows].double() - want).abs() <= tol).all()
+    assert kv.status() == 0
+    kv.close()
