@@ -125,10 +125,12 @@ class Kv4Cache:
 
     def read(self, batch: Kv4Batch, cache, rows: int | None = None, dtype=torch.bfloat16, out=None, stream=None):
         """(keys, values) [rows, n_kv_heads, head_dim] that the cache holds at the positions of the batch's rows, bf16 or
-        fp32; ``out``: a pair of tensors to write to."""
+        fp32; ``out``: a pair of tensors to write to.  A batch with row offsets needs ``rows`` or ``out``, as the host does not know
+        how many rows it has."""
         if stream is not None:
             return self._on(stream, self.read, batch, cache, rows, dtype, out)
         if out is None:
+            _need(rows is not None or batch.one_each, "rows: the number of rows of a batch with row offsets")
             rows = batch.batch if rows is None else rows
             out = [torch.zeros((rows, self.n_kv_heads, self.head_dim), dtype=dtype, device=self.device) for _ in range(2)]
         k, v = out
