@@ -124,7 +124,8 @@ int neon_decoder_step_host(neon_decoder_handle* h, const int32_t* tokens, const 
 int neon_decoder_read(neon_decoder_handle* h, const char* name, void* dst, uint64_t bytes);
 
 /* Options: "use_graphs" (default 1), "pdl" (programmatic dependent launch, a bit per
- * kernel kind: 1 GEMV, 2 RMSNorm, 4 rotary/cache, 8 attention, 16 merge, 32 others; default 29), "moe.<option>" (passed to every layer, see neon_moe.h), "kv_bits"
+ * kernel kind: 1 GEMV, 2 RMSNorm, 4 rotary/cache, 8 attention, 16 merge, 32 others, 64 sampling; default 93; the MoE layers have
+ * "moe.pdl" of their own), "moe.<option>" (passed to every layer, see neon_moe.h), "kv_bits"
  * (16, or 4: see above; switching empties the cache and waits for the device; a caller's own graph of earlier
  * steps may not be replayed after it), "stop_after_layer" (debug: run only the first n layers
  * and skip the head; 0 = all). */

@@ -70,7 +70,7 @@ struct neon_decoder_handle {
     float mscale = 1.f;
     int64_t launches = 0;
     int use_graphs = 1, stop_after = 0;
-    int pdl = 29;  // programmatic dependent launch per kernel kind (PdlBit); RMSNorm measured slower with it
+    int pdl = 93;  // programmatic dependent launch per kernel kind (PdlBit); RMSNorm measured slower with it
     cudaStream_t own_stream = nullptr, last_stream = nullptr;
     // one cached graph
     struct {
@@ -167,7 +167,7 @@ void launch_pdl(neon_decoder_handle* h, bool pdl, void (*kernel)(KArgs...), dim3
     h->launches++;
 }
 
-enum PdlBit { kPdlGemv = 1, kPdlNorm = 2, kPdlRope = 4, kPdlAttn = 8, kPdlMerge = 16, kPdlOther = 32 };
+enum PdlBit { kPdlGemv = 1, kPdlNorm = 2, kPdlRope = 4, kPdlAttn = 8, kPdlMerge = 16, kPdlOther = 32, kPdlSampler = 64 };
 
 template <typename... KArgs, typename... Args>
 void launch(neon_decoder_handle* h, int bit, void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st,
@@ -244,9 +244,10 @@ void launch_attention4(neon_decoder_handle* h, const LayerW& L, int layer, int B
     p.inv_freq = h->inv_freq; p.mscale = h->mscale;
     p.q_out = h->kv4.q;
     p.cache = L.pages;
-    h->launches += kv4::launch_append(p, NEON_KV4_F32, NEON_KV4_BF16, st);
+    h->launches += kv4::launch_append(p, NEON_KV4_F32, NEON_KV4_BF16, st, (h->pdl & kPdlRope) != 0);
     h->launches += kv4::launch_attend(p.s, batch, L.pages, NEON_KV4_BF16, h->kv4.q, QD, L.sinks, c.window > 0 && layer % 2 == 0 ? c.window : 0,
-                                      1.f / std::sqrt((float)c.head_dim), 1, h->attn, h->kv4.scratch, st);
+                                      1.f / std::sqrt((float)c.head_dim), 1, h->attn, h->kv4.scratch, st, (h->pdl & kPdlAttn) != 0,
+                                      (h->pdl & kPdlMerge) != 0);
 }
 
 int step_eager(neon_decoder_handle* h, const int32_t* tokens, const int32_t* positions, int B, float* logits, int32_t* next,
@@ -295,7 +296,7 @@ int step_eager(neon_decoder_handle* h, const int32_t* tokens, const int32_t* pos
     const auto& s = h->sampling;
     if (next && s.uniform)
         h->launches += sampler::launch(lg, NEON_SAMPLER_F32, c.vocab, c.vocab, B, s.uniform, s.temperature, s.top_k, s.top_p, s.min_p, next,
-                                       nullptr, nullptr, s.scratch, st);
+                                       nullptr, nullptr, s.scratch, st, (h->pdl & kPdlSampler) != 0);
     else if (next) launch(h, kPdlOther, argmax_kernel, dim3(B), dim3(1024), 0, st, (const float*)lg, c.vocab, next);
     DCU(h, cudaGetLastError());
     return NEON_MOE_OK;

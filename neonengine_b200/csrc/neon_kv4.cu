@@ -106,7 +106,7 @@ int attend_grid(const Shape& s, const Batch& b, int nt) {
 // The kernel may be set up while what runs before it on the stream drains (append 6.4 -> 6.3 us, attention of one token 10.0 -> 9.8, 8
 // layers of the decoder's step 1097 -> 1090); it waits for that before it reads or writes memory.
 template <class F>
-void with_pdl(void (*kernel)(F), unsigned grid, int threads, size_t smem, cudaStream_t st, const F& p) {
+void with_pdl(bool pdl, void (*kernel)(F), unsigned grid, int threads, size_t smem, cudaStream_t st, const F& p) {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(grid);
     cfg.blockDim = dim3(threads);
@@ -116,20 +116,20 @@ void with_pdl(void (*kernel)(F), unsigned grid, int threads, size_t smem, cudaSt
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = pdl;
     cudaLaunchKernelEx(&cfg, kernel, p);
 }
 
 template <int DIM, int PAGE, int NT>
-cudaError_t attend_variant(const AttendParams* run, cudaStream_t st) {
+cudaError_t attend_variant(const AttendParams* run, cudaStream_t st, bool pdl, bool pdl_merge) {
     using W = WarpSmem<DIM>;
     if (!run) return cudaFuncSetAttribute(attend_kernel<DIM, PAGE, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, 226 * 1024);
     AttendParams p = *run;
     const int plan = plan_bytes(p.b.n), budget = kSharedPerSm / ctas_per_sm(p.s, NT) - 2048 - plan;
     p.stages = std::min(W::kMaxStages, (budget / kAttendWarps - W::bytes(0)) / W::kRing);
-    with_pdl(attend_kernel<DIM, PAGE, NT>, (unsigned)p.grid, kAttendWarps * 32, plan + kAttendWarps * W::bytes(p.stages), st, p);
+    with_pdl(pdl, attend_kernel<DIM, PAGE, NT>, (unsigned)p.grid, kAttendWarps * 32, plan + kAttendWarps * W::bytes(p.stages), st, p);
     const long long tasks = (long long)p.b.rows * p.s.nq;
-    with_pdl(merge_kernel<DIM>, (unsigned)((tasks + 7) / 8), 256, plan, st, p);
+    with_pdl(pdl_merge, merge_kernel<DIM>, (unsigned)((tasks + 7) / 8), 256, plan, st, p);
     return cudaSuccess;
 }
 // Chunks of prompts: 256 rows of a key/value head at a time on tcgen05.  Heads of 64 only: at 128 columns queries, operands
@@ -170,7 +170,7 @@ cudaError_t configure_attend() {
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess || done[dev & 63]) return e;
-    e = each_variant([](int, int, int, auto variant) { return variant(nullptr, nullptr); });
+    e = each_variant([](int, int, int, auto variant) { return variant(nullptr, nullptr, false, false); });
     if (e == cudaSuccess) e = configure_prefill();
     if (e == cudaSuccess) done[dev & 63] = true;
     return e;
@@ -183,7 +183,7 @@ uint64_t attend_workspace(const Shape& s, const Batch& b, int max_rows) {
 }
 
 int launch_attend(const Shape& s, const Batch& b, const uint8_t* cache, int dtype, const void* q, long long q_stride, const uint16_t* sinks,
-                  int window, float scale, int max_rows, void* out, float* workspace, cudaStream_t st) {
+                  int window, float scale, int max_rows, void* out, float* workspace, cudaStream_t st, bool pdl, bool pdl_merge) {
     AttendParams p{};
     p.b = b; p.s = s; p.cache = cache; p.q = q; p.q_stride = q_stride; p.sinks = sinks;
     p.window = window; p.G = s.nq / s.nkv; p.half = dtype == NEON_KV4_F16; p.scale = scale; p.out = out; p.part = workspace;
@@ -196,22 +196,22 @@ int launch_attend(const Shape& s, const Batch& b, const uint8_t* cache, int dtyp
         return 1;
     }
     each_variant([&](int dim, int page, int groups, auto variant) {
-        return dim == s.D && page == s.P && groups == nt ? variant(&p, st) : cudaSuccess;
+        return dim == s.D && page == s.P && groups == nt ? variant(&p, st, pdl, pdl_merge) : cudaSuccess;
     });
     return 2;
 }
 
-int launch_append(const AppendParams& given, int dtype, int out_dtype, cudaStream_t st) {
+int launch_append(const AppendParams& given, int dtype, int out_dtype, cudaStream_t st, bool pdl) {
     AppendParams p = given;
     // a warp per row, unless there are so few rows that its ten or so rounds would be what takes the time: 8 rows of 80 heads 3.3 us in
     // parts, 6.0 by whole rows; 1024 rows 6.4 with this rule, 7.3 by whole rows, 12.0 in ten parts
     const int heads = (p.q ? p.s.nq : 0) + 2 * p.s.nkv, rounds = (heads * p.s.D / 16 + 31) / 32;
     p.split = std::min(rounds, std::max(1, kSms * 16 / p.b.rows));
     const unsigned grid = (unsigned)(((long long)p.b.rows * p.split + kAppendWarps - 1) / kAppendWarps);
-#define RUN(DT, DIM)                                                                                              \
-    if (dtype == DT && p.s.D == DIM) {                                                                            \
-        if (out_dtype == NEON_KV4_F16) with_pdl(append_kernel<DT, __half, DIM>, grid, kAppendWarps * 32, 0, st, p); \
-        else with_pdl(append_kernel<DT, __nv_bfloat16, DIM>, grid, kAppendWarps * 32, 0, st, p);                   \
+#define RUN(DT, DIM)                                                                                                     \
+    if (dtype == DT && p.s.D == DIM) {                                                                                   \
+        if (out_dtype == NEON_KV4_F16) with_pdl(pdl, append_kernel<DT, __half, DIM>, grid, kAppendWarps * 32, 0, st, p); \
+        else with_pdl(pdl, append_kernel<DT, __nv_bfloat16, DIM>, grid, kAppendWarps * 32, 0, st, p);                    \
     }
     RUN(NEON_KV4_F32, 64) RUN(NEON_KV4_BF16, 64) RUN(NEON_KV4_F16, 64) RUN(NEON_KV4_F32, 128) RUN(NEON_KV4_BF16, 128) RUN(NEON_KV4_F16, 128)
 #undef RUN
@@ -312,8 +312,8 @@ int neon_kv4_read(neon_kv4_handle* h, const neon_kv4_batch* batch, const void* c
     const ReadParams p{device_batch(h, batch, rows), h->shape, static_cast<const uint8_t*>(cache), k_out, v_out, rows <= 1024 ? 4 : 1};
     cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);
     const unsigned grid = ((unsigned)rows * p.split + 3) / 4;
-    if (dtype == NEON_KV4_F32) with_pdl(read_kernel<float>, grid, 128, 0, st, p);
-    else with_pdl(read_kernel<__nv_bfloat16>, grid, 128, 0, st, p);
+    if (dtype == NEON_KV4_F32) with_pdl(true, read_kernel<float>, grid, 128, 0, st, p);
+    else with_pdl(true, read_kernel<__nv_bfloat16>, grid, 128, 0, st, p);
     return launched(h, 1);
 }
 

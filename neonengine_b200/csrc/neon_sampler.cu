@@ -72,7 +72,7 @@ uint64_t workspace(int vocab, int batch) {
 
 int launch(const void* logits, int dtype, long long row_stride, int vocab, int batch, const float* uniform, const float* temperature,
            const int32_t* top_k, const float* top_p, const float* min_p, int32_t* tokens, float* probs, int32_t* kept, void* workspace,
-           cudaStream_t st) {
+           cudaStream_t st, bool pdl) {
     Params p{};
     p.logits = logits; p.dtype = dtype; p.vocab = vocab; p.batch = batch; p.stride = row_stride;
     p.uniform = uniform; p.temperature = temperature; p.top_k = top_k; p.top_p = top_p; p.min_p = min_p;
@@ -100,11 +100,11 @@ int launch(const void* logits, int dtype, long long row_stride, int vocab, int b
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.stream = st;
     cfg.attrs = attr;
-    cfg.numAttrs = n <= 8 * kScanWarps * grid;
+    cfg.numAttrs = pdl && n <= 8 * kScanWarps * grid;
     cfg.gridDim = dim3(grid);
     cfg.blockDim = dim3(kScanWarps * 32);
     cudaLaunchKernelEx(&cfg, scan, static_cast<const Params>(p));
-    cfg.numAttrs = 1;
+    cfg.numAttrs = pdl;
     cfg.blockDim = dim3(kPickThreads);
     cfg.gridDim = dim3(batch);
     cfg.dynamicSmemBytes = sizeof(PickSmem);

@@ -1,0 +1,42 @@
+"""Options of the decoder with a 4-bit cache and sampling."""
+import pytest
+
+from test_decoder_kv4_gpu import ints, make, small_shape
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+DEV = "cuda:0"
+
+
+def programmatic_edges(s):
+    """How many of a captured step's edges let a kernel start before its predecessor is over."""
+    from cuda.bindings import runtime
+    tokens, pos, nxt = ints(3, 4), ints(9, 70), torch.zeros(2, dtype=torch.int32, device=DEV)
+    s.step(tokens, pos, next_tokens=nxt)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph(keep_graph=True)
+    with torch.cuda.graph(graph):
+        s.step(tokens, pos, next_tokens=nxt)
+    raw = runtime.cudaGraph_t(graph.raw_cuda_graph())
+    err, _, _, _, n = runtime.cudaGraphGetEdges_v2(raw)
+    assert err == 0
+    err, _, _, data, n = runtime.cudaGraphGetEdges_v2(raw, n)
+    assert err == 0 and n > 0
+    return sum(int(d.type) == int(runtime.cudaGraphDependencyType.cudaGraphDependencyTypeProgrammatic) for d in data[:n])
+
+
+@pytest.mark.parametrize("kv_bits", [4, 16])
+def test_pdl_option_covers_every_kernel(kv_bits):
+    """"pdl" has a bit per kind of kernel, the 4-bit cache's and the sampler's among them: 0 leaves what the MoE layers do by themselves."""
+    shape = small_shape(vocab=20000)
+    s = make(shape, 2, 128, seed=3, kv_bits=16)
+    s.set_option("pdl", 0)
+    moe = programmatic_edges(s)
+    s.set_option("kv_bits", kv_bits)
+    s.set_sampling(torch.rand(2, device=DEV), top_p=torch.full((2,), 0.9, device=DEV))
+    # rotation and cache 4, attention 8, merging 16: a kernel a layer; sampler 64: three kernels where rows are cut
+    for bits, kernels in ((0, 0), (4, shape.n_layers), (8, shape.n_layers), (16, shape.n_layers), (64, 3)):
+        s.set_option("pdl", bits)
+        assert programmatic_edges(s) == moe + kernels, bits
+    s.close()
