@@ -106,7 +106,8 @@ int neon_decoder_step(neon_decoder_handle* h, const int32_t* tokens, const int32
 
 /* Next tokens are sampled from now on (neon_sampler.h) instead of being the largest logits'.  Device arrays of at least max_batch
  * elements that every step reads as it runs, so they may be refilled between steps: uniform fp32, numbers in [0, 1);
- * temperature, top_p, min_p fp32, top_k int32, each NULL for none.  uniform NULL (and all others): the largest again. */
+ * temperature, top_p, min_p fp32, top_k int32, each NULL for none.  uniform NULL (and all others): the largest again.  The arrays
+ * have to live until the steps enqueued with them are over, and graphs that the caller captured of such steps are gone. */
 int neon_decoder_set_sampling(neon_decoder_handle* h, const float* uniform, const float* temperature,
                               const int32_t* top_k, const float* top_p, const float* min_p);
 

@@ -42,6 +42,7 @@ class DecoderSystem:
         if rc != 0:
             raise RuntimeError(f"neon_decoder_create failed ({rc}): {self._lib.neon_decoder_last_error(None).decode()}")
         self._h = handle
+        self._sampling = ()  # what steps read
 
     def _check(self, rc: int, what: str) -> None:
         if rc != 0:
@@ -76,15 +77,18 @@ class DecoderSystem:
     # -- execution -----------------------------------------------------------------------
     def set_sampling(self, uniform=None, temperature=None, top_k=None, top_p=None, min_p=None) -> None:
         """Next tokens are sampled from now on: device tensors of at least ``max_batch`` elements (fp32, ``top_k`` int32) that every
-        step reads as it runs and the caller may refill between steps.  Without arguments: the largest logit again."""
+        step reads as it runs and the caller may refill between steps.  Without arguments: the largest logit again.  Waits for the
+        device where it lets go of tensors given before; a caller's own graphs of steps need theirs alive."""
         import torch
         given = [uniform, temperature, top_k, top_p, min_p]
         for t, dtype in zip(given, (torch.float32, torch.float32, torch.int32, torch.float32, torch.float32)):
             if t is not None and (t.dtype is not dtype or t.numel() < self.max_batch or not t.is_contiguous() or t.get_device() != self.device):
                 raise ValueError(f"contiguous {dtype} tensors of at least {self.max_batch} elements on device {self.device}")
+        if any(old is not None and all(old is not t for t in given) for old in self._sampling):
+            torch.cuda.synchronize(self.device)  # steps under way, on whatever stream, still read them
         self._check(self._lib.neon_decoder_set_sampling(self._h, *[None if t is None else t.data_ptr() for t in given]),
                     "neon_decoder_set_sampling")
-        self._sampling = given  # alive as long as steps may read them
+        self._sampling = given
 
     def step(self, tokens, positions, logits=None, next_tokens=None, stream=None):
         """One decode step over device tensors: ``tokens``/``positions`` torch int32 [B];

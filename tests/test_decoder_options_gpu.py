@@ -40,3 +40,30 @@ def test_pdl_option_covers_every_kernel(kv_bits):
         s.set_option("pdl", bits)
         assert programmatic_edges(s) == moe + kernels, bits
     s.close()
+
+
+@pytest.mark.parametrize("then", ["other", "none"])
+def test_sampling_settings_outlive_steps_under_way(then):
+    """A step on another stream has not run when new settings are given: what it still reads is not handed out again before."""
+    shape, vocab = small_shape(vocab=20000), 20000
+    s = make(shape, 2, 64, seed=6)
+    side, logits, nxt = torch.cuda.Stream(), torch.empty((2, vocab), device=DEV), torch.zeros(2, dtype=torch.int32, device=DEV)
+    tokens, pos = ints(3, 4), ints(0, 1)
+    new = [torch.full((2,), 0.5, device=DEV), torch.full((2,), 0.1, device=DEV)]
+    given = [torch.full((2,), 0.25, device=DEV), torch.full((2,), 50.0, device=DEV)]
+    places = [t.data_ptr() for t in given]
+    s.set_sampling(*given)
+    s.step(tokens, pos, logits=logits, next_tokens=nxt)
+    want = nxt.clone()
+    torch.cuda.synchronize()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(40000000)
+    s.step(tokens, pos, logits=logits, next_tokens=nxt, stream=side)
+    del given
+    s.set_sampling(*(new if then == "other" else ()))
+    again = [torch.full((2,), x, device=DEV) for x in (0.9, 0.01, 0.9, 0.01)]  # the memory that is free now
+    assert set(places) & {t.data_ptr() for t in again}
+    torch.cuda.synchronize()
+    assert torch.equal(nxt, want)
+    s.close()
