@@ -91,7 +91,7 @@ int neon_decoder_set_moe(neon_decoder_handle* h, int layer, const void* router_w
                          int on_device);
 
 /* Fills cache positions [0, n_pos) of one layer for sequences [0, batch): k, v bf16
- * [batch, n_pos, n_kv_heads, 64] (keys already rotated). */
+ * [batch, n_pos, n_kv_heads, 64] (keys already rotated; in device memory on 16-byte boundaries). */
 int neon_decoder_load_kv(neon_decoder_handle* h, int layer, const void* k, const void* v, int batch,
                          int n_pos, int on_device);
 

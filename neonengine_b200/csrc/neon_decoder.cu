@@ -566,6 +566,8 @@ int neon_decoder_load_kv(neon_decoder_handle* h, int layer, const void* k, const
     if (batch < 0 || batch > c.max_batch || n_pos < 0 || n_pos > c.max_ctx)
         return dfail(h, NEON_MOE_EINVAL, "batch %d / positions %d outside the cache", batch, n_pos);
     if (!k || !v) return dfail(h, NEON_MOE_EINVAL, "null cache tensor");
+    if (on_device && (reinterpret_cast<uintptr_t>(k) % 16 || reinterpret_cast<uintptr_t>(v) % (h->kv4.on() ? 16 : 2)))
+        return dfail(h, NEON_MOE_EINVAL, "device keys (with a 4-bit cache values, too) have to start on a 16-byte boundary");
     DCU(h, cudaSetDevice(c.device));
     LayerW& L = h->layers[layer];
     if (h->kv4.on()) return load_kv4(h, L, k, v, batch, n_pos, on_device);

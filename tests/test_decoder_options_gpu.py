@@ -67,3 +67,23 @@ def test_sampling_settings_outlive_steps_under_way(then):
     torch.cuda.synchronize()
     assert torch.equal(nxt, want)
     s.close()
+
+
+@pytest.mark.parametrize("kv_bits", [4, 16])
+def test_load_kv_refuses_unaligned_tensors(kv_bits):
+    """Device tensors are read 16 bytes at a time (16-bit caches' values are not)."""
+    shape = small_shape()
+    s = make(shape, 2, 64, seed=6, kv_bits=kv_bits)
+    flat = torch.randn(2 * 40 * 2 * 64 + 8, device=DEV).to(torch.bfloat16)
+    whole, shifted = flat[:-8].view(2, 40, 2, 64), flat[1:-7].view(2, 40, 2, 64)
+    with pytest.raises(RuntimeError, match="16-byte"):
+        s.load_kv(0, shifted, whole)
+    if kv_bits == 4:
+        with pytest.raises(RuntimeError, match="16-byte"):
+            s.load_kv(0, whole, shifted)
+    else:
+        s.load_kv(0, whole, shifted)
+    s.load_kv(0, whole, whole)
+    s.step(ints(3, 4), ints(39, 40))
+    assert torch.from_numpy(s.read("logits")).isfinite().all()
+    s.close()
