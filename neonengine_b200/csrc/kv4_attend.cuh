@@ -46,6 +46,8 @@ constexpr int kCareful = 1 << 23;  // positions times how far the run's scales l
 constexpr int kMostSum = 30;       // (log2) how far lowering its level may take a row's sum
 constexpr int kWide = 24;          // (log2) how far apart the run's scales may lie for what a group loses then not to count
 
+constexpr int kMaxHeadRows = 1 << 26;  // rows times query heads a key/value head of a call
+
 struct AttendParams {
     Batch b;
     Shape s;
@@ -60,7 +62,7 @@ struct AttendParams {
     int grid, stages;
     int R;        // rows (tokens times G) of an item: 8 * NT
     uint32_t G_inverse;  // ceil(2^32 / G)
-    // r / G for r < 2^26, exact as G <= 32
+    // r / G for r < kMaxHeadRows: exact, as r * (G_inverse * G - 2^32) < 2^32
     __device__ __forceinline__ int token(int r) const { return G == 1 ? r : (int)__umulhi((uint32_t)r, G_inverse); }
     // first position that a row at `pos` may see (pos may be below 0, the window any number)
     __device__ __forceinline__ int first_seen(int pos) const { return window > 0 && pos >= window ? pos - window + 1 : 0; }

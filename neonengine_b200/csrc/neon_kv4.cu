@@ -334,6 +334,8 @@ int neon_kv4_attend(neon_kv4_handle* h, const neon_kv4_batch* batch, const void*
     if (!std::isfinite(scale)) return fail(h, NEON_MOE_EINVAL, "scale is not finite");
     const Shape& s = h->shape;
     if (q_stride < s.nq * s.D) return fail(h, NEON_MOE_EINVAL, "a row stride is smaller than the row");
+    if ((int64_t)rows * (s.nq / s.nkv) > kMaxHeadRows)
+        return fail(h, NEON_MOE_EINVAL, "%d rows of %d query heads a key/value head are more than %d", rows, s.nq / s.nkv, kMaxHeadRows);
     if (!aligned(q, q_stride, dtype) || reinterpret_cast<uintptr_t>(out) % 16 || reinterpret_cast<uintptr_t>(workspace) % 16)
         return fail(h, NEON_MOE_EINVAL, "q rows, out and workspace have to start on 16-byte boundaries");
     const Batch b = device_batch(h, batch, rows);

@@ -24,3 +24,18 @@ def test_read_of_ragged_rows_wants_their_number():
     one, _ = kv.read(each, cache)
     assert one.shape == (2, 2, 64) and torch.equal(one, k[[2, 6]])
     kv.close()
+
+
+def test_attention_refuses_more_rows_than_it_can_number():
+    """Rows times query heads a key/value head: 2^26 at most.  (The buffers are never looked at.)"""
+    from neonengine_b200.kv4_cache import Kv4Cache
+    kv = Kv4Cache(32, 1, 64, 32)
+    small = torch.zeros(4096, device=DEV, dtype=torch.uint8)
+    cu = torch.tensor([0, 2 ** 21 + 1], dtype=torch.int32, device=DEV)
+    batch = kv.batch(torch.tensor([40], dtype=torch.int32, device=DEV), torch.zeros((1, 2), dtype=torch.int32, device=DEV), cu)
+    batch._c.n_pages = 1
+    one = ctypes.c_void_p(small.data_ptr())
+    rc = kv._lib.neon_kv4_attend(kv._h, batch._ref, one, 2 ** 21 + 1, 1, one, 2048, None, 0, 1.0, 2 ** 21 + 1, one, one, 1 << 40, None)
+    assert rc == 1 and b"query heads" in kv._lib.neon_kv4_last_error(kv._h)
+    assert kv.launch_count == 0 and kv.status() == 0
+    kv.close()
