@@ -108,7 +108,8 @@ uint64_t neon_kv4_attend_workspace(neon_kv4_handle* h, const neon_kv4_batch* bat
  * p <= the row's own (and > own - window where window > 0); query head j reads key/value head
  * j / (n_q_heads / n_kv_heads).  q (rows q_stride elements apart) and out ([rows, n_q_heads, D] contiguous):
  * dtype BF16 or F16.  sinks: bf16 [n_q_heads] or NULL.  Rows that see no position get zeros.  rows * n_q_heads / n_kv_heads
- * is 2^26 at most.
+ * is 2^26 at most; a call is refused, too, whose table could hold more than 2^35 steps: 64 positions for 8 to 32 of those
+ * products and a key/value head.
  * Value scales above 2^125, which only infinities give, count as 2^125.  From values of about 2^110 on a row's sums
  * may leave the range of fp32; it is infinite or NaN then.  Scores are fp32 sums of exact products, good to 2^-23 of
  * their size; from 2^22 on a row may be zero, infinite or NaN.  Each probability is rounded to 11 bits (12 where a

@@ -46,7 +46,8 @@ constexpr int kCareful = 1 << 23;  // positions times how far the run's scales l
 constexpr int kMostSum = 30;       // (log2) how far lowering its level may take a row's sum
 constexpr int kWide = 24;          // (log2) how far apart the run's scales may lie for what a group loses then not to count
 
-constexpr int kMaxHeadRows = 1 << 26;  // rows times query heads a key/value head of a call
+constexpr int kMaxHeadRows = 1 << 26;        // rows times query heads a key/value head of a call
+constexpr long long kMaxCtaUnits = 1 << 28;  // steps of a CTA: eight times as many are below 2^32 (and would take half a minute)
 
 struct AttendParams {
     Batch b;

@@ -20,6 +20,8 @@ cudaError_t configure_attend();
 // kernel be set up while what runs before it drains.
 int launch_append(const AppendParams& p, int dtype, int out_dtype, cudaStream_t st, bool pdl = true);
 uint64_t attend_workspace(const Shape& s, const Batch& b, int max_rows);
+// whether the steps of a call can be numbered, whatever its lengths are within the table
+bool attend_counts(const Shape& s, const Batch& b, int max_rows, int window);
 int launch_attend(const Shape& s, const Batch& b, const uint8_t* cache, int dtype, const void* q, long long q_stride, const uint16_t* sinks,
                   int window, float scale, int max_rows, void* out, float* workspace, cudaStream_t st, bool pdl = true, bool pdl_merge = true);
 }  // namespace kv4

@@ -96,10 +96,13 @@ int column_groups(const Shape& s, int max_rows) {
 }
 // one instead of two, with eight rows of 64: 54 us instead of 46
 int ctas_per_sm(const Shape& s, int nt) { return s.D == 64 && nt == 1 ? 2 : 1; }
-int attend_grid(const Shape& s, const Batch& b, int nt) {
+// steps that there can be in all, as the table's width bounds the lengths
+long long most_units(const Shape& s, const Batch& b, int nt) {
     const long long steps = ((long long)b.width * s.P + kStep - 1) / kStep;
-    const long long blocks = (long long)b.rows * (s.nq / s.nkv) / (8 * nt) + b.n;
-    const long long most = (steps * blocks * s.nkv + kAttendWarps - 1) / kAttendWarps;  // CTAs that there can be steps for
+    return steps * ((long long)b.rows * (s.nq / s.nkv) / (8 * nt) + b.n) * s.nkv;
+}
+int attend_grid(const Shape& s, const Batch& b, int nt) {
+    const long long most = (most_units(s, b, nt) + kAttendWarps - 1) / kAttendWarps;  // CTAs that there can be steps for
     return (int)std::min<long long>(kSms * ctas_per_sm(s, nt), std::max<long long>(most, 1));
 }
 
@@ -174,6 +177,11 @@ cudaError_t configure_attend() {
     if (e == cudaSuccess) e = configure_prefill();
     if (e == cudaSuccess) done[dev & 63] = true;
     return e;
+}
+
+bool attend_counts(const Shape& s, const Batch& b, int max_rows, int window) {
+    const int nt = column_groups(s, max_rows);
+    return prefills(s, b, max_rows, window) || most_units(s, b, nt) / attend_grid(s, b, nt) < kMaxCtaUnits;
 }
 
 uint64_t attend_workspace(const Shape& s, const Batch& b, int max_rows) {
@@ -336,6 +344,8 @@ int neon_kv4_attend(neon_kv4_handle* h, const neon_kv4_batch* batch, const void*
     if (q_stride < s.nq * s.D) return fail(h, NEON_MOE_EINVAL, "a row stride is smaller than the row");
     if ((int64_t)rows * (s.nq / s.nkv) > kMaxHeadRows)
         return fail(h, NEON_MOE_EINVAL, "%d rows of %d query heads a key/value head are more than %d", rows, s.nq / s.nkv, kMaxHeadRows);
+    if (!attend_counts(s, device_batch(h, batch, rows), max_rows, window))
+        return fail(h, NEON_MOE_EINVAL, "%d rows over page tables of %d columns", rows, batch->table_width);
     if (!aligned(q, q_stride, dtype) || reinterpret_cast<uintptr_t>(out) % 16 || reinterpret_cast<uintptr_t>(workspace) % 16)
         return fail(h, NEON_MOE_EINVAL, "q rows, out and workspace have to start on 16-byte boundaries");
     const Batch b = device_batch(h, batch, rows);

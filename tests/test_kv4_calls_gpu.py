@@ -39,3 +39,19 @@ def test_attention_refuses_more_rows_than_it_can_number():
     assert rc == 1 and b"query heads" in kv._lib.neon_kv4_last_error(kv._h)
     assert kv.launch_count == 0 and kv.status() == 0
     kv.close()
+
+
+def test_attention_refuses_more_steps_than_it_can_number():
+    """Steps of 64 positions times blocks of rows, as the table's width bounds them.  (The buffers are never looked at.)"""
+    from neonengine_b200.kv4_cache import Kv4Cache
+    kv = Kv4Cache(128, 128, 64, 64)
+    small = torch.zeros(4096, device=DEV, dtype=torch.uint8)
+    rows = 2 ** 20
+    batch = kv.batch(torch.tensor([40], dtype=torch.int32, device=DEV), torch.zeros((1, 1), dtype=torch.int32, device=DEV),
+                     torch.tensor([0, rows], dtype=torch.int32, device=DEV))
+    batch._c.n_pages, batch._c.table_width, batch._c.table_stride = 1, 2 ** 24, 2 ** 24
+    one = ctypes.c_void_p(small.data_ptr())
+    rc = kv._lib.neon_kv4_attend(kv._h, batch._ref, one, rows, 1, one, 8192, None, 0, 1.0, 1, one, one, 1 << 62, None)
+    assert rc == 1 and b"page tables" in kv._lib.neon_kv4_last_error(kv._h)
+    assert kv.launch_count == 0 and kv.status() == 0
+    kv.close()
