@@ -232,6 +232,8 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1) prefill_kernel(const Attend
         return (bool)__all_sync(0xffffffffu, parked_wait(bar, parity & 1, &s.abort, p.b.status));
     };
 
+    bool issue = false;  // this thread has issued products
+    int fetched = 0;     // steps that were sent for
     if (n > 0 && warp < kPreSoftmaxWarps) {
         // ---- softmax: this thread's row ------------------------------------------------------------------------------------
         const int hi = tid < rows ? min(q.pos0 + token, q.len - 1) : -1, lo = p.first_seen(q.pos0 + token) - 1;
@@ -410,7 +412,7 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1) prefill_kernel(const Attend
         }
     } else if (n > 0 && warp == kPreCopyWarp) {
         // ---- copies ----------------------------------------------------------------------------------------------------------
-        int id_base = -64, ids = -1, fetched = 0;
+        int id_base = -64, ids = -1;
         for (int j = 0; j < n; ++j, ++fetched) {
             const int page = (step0 + j) * kPages, stage = j % kPreRaw;
             if ((uint32_t)(page - id_base) >= 32u) {
@@ -439,8 +441,6 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1) prefill_kernel(const Attend
             if (lane < kPages && id >= 0)
                 sm100::bulk_load(s.raw[stage] + lane * kRec, p.cache + ((long long)id * p.s.nkv + kvh) * kRec, kRec, &s.raw_full[stage]);
         }
-        if (*(volatile int*)&s.abort)  // no copy may land after the CTA is gone
-            for (int j = max(0, fetched - kPreRaw); j < fetched; ++j) wait_bounded(&s.raw_full[j % kPreRaw], (j / kPreRaw) & 1);
     } else if (n > 0 && warp == kPreScoreWarp) {
         // ---- scores ----------------------------------------------------------------------------------------------------------
         // f32 += bf16 * bf16; 128 rows, both operands K-major.  Descriptors differ by their start addresses (in 16 bytes) alone:
@@ -448,7 +448,7 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1) prefill_kernel(const Attend
         const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((kStep / 8) << 17) | ((128u >> 4) << 24);
         const uint64_t dq = sm100::make_sw128_desc(sm100::smem_u32(s.q[0])), dk = sm100::make_sw128_desc(sm100::smem_u32(s.k[0]));
         constexpr uint32_t kTerm = kPreRows * 128 / 16, kTile = 128 * 128 / 16, kStageK = kStep * 128 / 16;
-        const bool issue = sm100::elect_one();
+        issue = sm100::elect_one();
         bool ok = true;
         for (int j = 0; j < n && ok; ++j) {
             ok = wait(&s.kv_full[j % kPreStages], j / kPreStages);
@@ -469,17 +469,12 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1) prefill_kernel(const Attend
                 __syncwarp();
             }
         }
-        if (!ok) {  // what was issued has to end before tensor memory is given back
-            if (issue) sm100::tc_commit(&s.drained[0]);
-            __syncwarp();
-            wait_bounded(&s.drained[0], 0);
-        }
     } else if (n > 0 && warp == kPreOutputWarp) {
         // ---- outputs: f32 += tf32 * tf32 -----------------------------------------------------------------------------------------
         const uint32_t idesc = (1u << 4) | (2u << 7) | (2u << 10) | ((kPreN / 8) << 17) | ((128u >> 4) << 24);
         const uint64_t dv = sm100::make_sw128_desc(sm100::smem_u32(s.v[0][0]));
         constexpr uint32_t kHalfV = kPreN * 128 / 16;
-        const bool issue = sm100::elect_one();
+        issue = sm100::elect_one();
         bool ok = true;
         for (int j = 0; j < n && ok; ++j) {
             const int stage = j % kPreStages;
@@ -499,11 +494,6 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1) prefill_kernel(const Attend
                 __syncwarp();
             }
         }
-        if (!ok) {
-            if (issue) sm100::tc_commit(&s.drained[1]);
-            __syncwarp();
-            wait_bounded(&s.drained[1], 0);
-        }
     }
     if (n == 0 && tid < rows)
         for (int c = 0; c < D; c += 8) {
@@ -512,6 +502,17 @@ __global__ void __launch_bounds__(kPreWarps * 32, 1) prefill_kernel(const Attend
         }
     sm100::tc_fence_before();
     __syncthreads();
+    if (s.abort) {  // the same for the whole CTA: nobody waits any more.  What is under way has to end before shared and tensor memory go
+        if (warp == kPreScoreWarp || warp == kPreOutputWarp) {
+            uint64_t* done = &s.drained[warp == kPreOutputWarp];
+            if (issue) sm100::tc_commit(done);
+            __syncwarp();
+            if (n > 0) wait_bounded(done, 0);
+        } else if (warp == kPreCopyWarp) {
+            for (int j = max(0, fetched - kPreRaw); j < fetched; ++j) wait_bounded(&s.raw_full[j % kPreRaw], (j / kPreRaw) & 1);
+        }
+        __syncthreads();
+    }
     if (warp == kPreScoreWarp) sm100::tmem_dealloc(tmem, 512);
 }
 
