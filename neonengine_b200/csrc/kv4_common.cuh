@@ -31,8 +31,6 @@ struct Batch {
         const int lo = min(max(cu_q[b], 0), rows), hi = min(max(cu_q[b + 1], lo), rows);
         return make_int2(lo, hi - lo);
     }
-    // positions of sequence b that its table can name
-    __device__ __forceinline__ int length(int b, int P) const { return min(seq_lens[b], width * P); }
 };
 
 __device__ __forceinline__ void report(int* status, int bits) { atomicOr(status, bits); }
