@@ -15,13 +15,13 @@
 //   Values: a pair of positions of one column is one f16x2 operand, multiplied by the two positions' scales relative to
 //   the largest scale met so far (outputs are rescaled when it grows).  Where a step's scales lie more than 2^7 below it, its
 //   values are added in f32, one position at a time (five times as long, and rare).
-//   Probabilities are f16, relative to a level of their row: a group (the 64 or 32 positions weighed at once) whose largest exceeds 2^15
-//   raises it, to 2^8 below.  So a probability is rounded by 2^-12 of itself or by 2^-25, and the row's sum is 2^7 or more.  With value
-//   scales 2^apart apart at most, n positions lose n * 2^(apart - 32) of the sum of weights times scales: 2^-9, once n * 2^apart is 2^23
+//   Probabilities are f16, relative to a level of their row: a group (the 64 or 32 positions weighed at once) whose largest would be
+//   infinite raises it, to 2^8 below.  So a probability is rounded by 2^-12 of itself or by 2^-25, and the row's sum is 2^8 or more.  With value
+//   scales 2^apart apart at most, n positions lose n * 2^(apart - 33) of the sum of weights times scales: 2^-10, once n * 2^apart is 2^23
 //   (kCareful: 65536 positions of a warp's run at scales within 2^7).  From there on a group whose largest is below 1 lowers
 //   the level, to 2^5 below it: then what a group loses is 2^-12 of its own, wherever the row's largest stands and whatever its value is.
 //   Lowering ends where it takes the sum to 2^30; a group that needs more loses 2^-49 of the sum, and where scales lie further
-//   apart than 2^24 it is added in f32.  Levels are whole numbers, so that rescaling is exact.
+//   apart than 2^24 it is added in f32.  Rescaling is off by 2^-22.
 //   The softmax sum is one more product, with a row of ones.  Most steps need no exchange between lanes but one vote.
 // Steps travel by bulk copies (one per page and head: a record is contiguous) into a ring per warp.
 // What bounds it at G = 8: not the memory but issue slots and the conversions (two codes each, 64 lanes a clock and SM).  Measured with 64
@@ -39,8 +39,8 @@ constexpr int kStep = 64;             // positions of a step
 constexpr float kNoMax = -1e30f;      // level before the first score
 constexpr float kLog2e = 1.4426950408889634f;
 // where (log2) the largest probability of a group may lie, as f16 pairs too, and where it is put when it does not
-constexpr float kHigh = 15.f, kLow = 0.f, kRaiseTo = 8.f, kLowerTo = 5.f;
-constexpr uint32_t kHighest = 0x78007800u, kLowest = 0x3c003c00u;
+constexpr float kHigh = 15.5f, kLow = 0.f, kRaiseTo = 8.f, kLowerTo = 5.f;
+constexpr uint32_t kHighest = 0x7bff7bffu, kLowest = 0x3c003c00u;  // (the largest f16; those below it by half a step round to it)
 constexpr int kSpread = 7;         // how far (log2) a step's value scales may lie below the largest for f16 operands
 constexpr int kCareful = 1 << 23;  // positions times how far the run's scales lie apart before small probabilities are looked after
 constexpr int kMostSum = 30;       // (log2) how far lowering its level may take a row's sum
@@ -561,39 +561,38 @@ __global__ void __launch_bounds__(kAttendWarps * 32, (D == 64 && NT == 1) ? 2 : 
                             move = move || __any_sync(0xffffffffu, !__hbge2(as_half2(least), as_half2(kLowest)));
                         }
                         if (move) {
-                            bool moved = false, lost = false;
-                            float f[NT][2];
+                            bool lost = false;
+                            float x[NT][2];  // the largest scores, in units of log 2
 #pragma unroll
                             for (int j = 0; j < NT; ++j)
 #pragma unroll
                                 for (int c = 0; c < 2; ++c) {
-                                    float x = -INFINITY, factor = qs[j][c];
+                                    float factor = qs[j][c];
+                                    x[j][c] = -INFINITY;
                                     asm volatile("" : "+f"(factor));  // keeps these products out of the steps that need none
 #pragma unroll
-                                    for (int i = 0; i < TI; ++i) x = fmaxf(x, fmaxf(sc[j][i][c] * factor, sc[j][i][c + 2] * factor));
+                                    for (int i = 0; i < TI; ++i) x[j][c] = fmaxf(x[j][c], fmaxf(sc[j][i][c] * factor, sc[j][i][c + 2] * factor));
 #pragma unroll
-                                    for (int off = 4; off < 32; off <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, off));
-                                    const float old = m[j][c];
-                                    float now = x > old + kHigh ? rintf(x) - kRaiseTo : old;
-                                    if (careful && x < old + kLow && x > -INFINITY) {
-                                        now = fmaxf(rintf(x) - kLowerTo, old - (float)max(kMostSum - max(log2_of(l[j][c]), 0), 0));
-                                        lost = lost || x < now + kLow;
-                                    }
-                                    moved = moved || now != old;
-                                    f[j][c] = pow2i((int)(old - now));
-                                    m[j][c] = now;
+                                    for (int off = 4; off < 32; off <<= 1) x[j][c] = fmaxf(x[j][c], __shfl_xor_sync(0xffffffffu, x[j][c], off));
                                 }
-                            if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
-                                for (int j = 0; j < NT; ++j)
+                            for (int j = 0; j < NT; ++j)
 #pragma unroll
-                                    for (int c = 0; c < 2; ++c) {
-                                        l[j][c] *= f[j][c];
-#pragma unroll
-                                        for (int i = 0; i < D / 16; ++i) { o[j][i][c] *= f[j][c]; o[j][i][c + 2] *= f[j][c]; }
+                                for (int c = 0; c < 2; ++c) {
+                                    float now = x[j][c] > m[j][c] + kHigh ? x[j][c] - kRaiseTo : m[j][c];
+                                    if (careful) {
+                                        const bool low = x[j][c] < now + kLow && x[j][c] > -INFINITY;
+                                        const float floor = now - (float)max(kMostSum - max(log2_of(l[j][c]), 0), 0);
+                                        now = low ? fmaxf(x[j][c] - kLowerTo, floor) : now;
+                                        lost = lost || (low && x[j][c] < now + kLow);
                                     }
-                                weigh();
-                            }
+                                    const float f = ex2(m[j][c] - now);
+                                    m[j][c] = now;
+                                    l[j][c] *= f;
+#pragma unroll
+                                    for (int i = 0; i < D / 16; ++i) { o[j][i][c] *= f; o[j][i][c + 2] *= f; }
+                                }
+                            weigh();
                             exact = exact || (apart > kWide && __any_sync(0xffffffffu, lost));
                         }
                         // ---- values ------------------------------------------------------------------------------------------
