@@ -100,7 +100,8 @@ int neon_decoder_load_kv(neon_decoder_handle* h, int layer, const void* k, const
  * slot and attention covers positions <= it); logits fp32 [batch, vocab] or NULL (internal
  * buffer); next_tokens int32 [batch] or NULL.  Token ids and positions outside their ranges are
  * clamped into range by the kernels (they live in device memory, so the host cannot check them).  The second call with the same arguments is
- * captured into a CUDA graph and replayed from then on (option use_graphs). */
+ * captured into a CUDA graph and replayed from then on (option use_graphs).  With "kv_bits" 4 a wait inside a kernel that ran out
+ * shows in "kv4_status" (neon_decoder_read); neon_decoder_step_host looks at it by itself. */
 int neon_decoder_step(neon_decoder_handle* h, const int32_t* tokens, const int32_t* positions, int batch,
                       float* logits, int32_t* next_tokens, void* cuda_stream);
 

@@ -74,7 +74,7 @@ typedef struct neon_kv4_batch {
 
 /* bits of neon_kv4_status */
 #define NEON_KV4_BAD_PAGE 1    /* a page id outside the cache was met                     */
-#define NEON_KV4_BAD_LENGTH 2  /* a sequence longer than its table, or cu_q not ascending */
+#define NEON_KV4_BAD_LENGTH 2  /* a sequence longer than its table, or (seen by attention) cu_q not ascending */
 #define NEON_KV4_TIMEOUT 4     /* a wait inside a kernel ran out                          */
 
 int neon_kv4_create(const neon_kv4_config* cfg, neon_kv4_handle** out);
@@ -115,7 +115,7 @@ uint64_t neon_kv4_attend_workspace(neon_kv4_handle* h, const neon_kv4_batch* bat
  * their size; from 2^22 on a row may be zero, infinite or NaN.  Each probability is rounded to 11 bits (12 where a
  * sequence has few rows), and the bits that small ones lose are 2^-8 of the sum of weights times values' scales at most.
  * max_rows: the most rows that a sequence has, as far as the host knows it; it chooses the kernel, so results
- * depend on it by these roundings. */
+ * depend on it by these roundings, and speed does: 64 sequences of one row and 4000 positions 48 us told 1, 104 told 64. */
 int neon_kv4_attend(neon_kv4_handle* h, const neon_kv4_batch* batch, const void* cache, int rows, int dtype,
                     const void* q, int64_t q_stride, const void* sinks, int window, float scale, int max_rows,
                     void* out, void* workspace, uint64_t workspace_bytes, void* cuda_stream);

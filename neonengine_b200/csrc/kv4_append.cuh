@@ -229,8 +229,9 @@ struct ReadParams {
     int split;  // warps per row
 };
 
-// A warp (or `split` of them) per row; a lane turns eight codes into values, 32 pieces of the row's heads at a time.  Memory bound: 13320
-// rows of 8 + 8 heads of 64 to bf16 take 15 us (2.6 KB a row, 2.3 TB/s); a few rows 2 us.
+// A warp (or `split` of them) per row; a lane turns eight codes into values, 32 pieces of the row's heads at a time.  13320 rows of 8 + 8
+// heads of 64 to bf16 take 11 us behind the append (2.6 KB a row), 17 from HBM: not the memory bounds it but some 1.8 instructions a
+// clock and SM, divisions by the head's and page's size and four bytes of codes a lane among them.  A few rows take 2 us.
 template <class OutT>
 __global__ void __launch_bounds__(128) read_kernel(const ReadParams p) {
     const int task = blockIdx.x * 4 + threadIdx.x / 32, row = task / p.split, lane = threadIdx.x & 31, D = p.s.D, per_head = D / 8, units = p.s.nkv * per_head;

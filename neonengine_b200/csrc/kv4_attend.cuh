@@ -25,9 +25,10 @@
 //   The softmax sum is one more product, with a row of ones.  Most steps need no exchange between lanes but one vote.
 // Steps travel by bulk copies (one per page and head: a record is contiguous) into a ring per warp.
 // What bounds it at G = 8: not the memory but issue slots and the conversions (two codes each, 64 lanes a clock and SM).  Measured with 64
-// query and 8 key/value heads of 64: 64 sequences of 200 to 32768 positions 123 us for 476 MB, 3.9 TB/s (streaming the records alone 87,
-// the arithmetic alone 106); 8 sequences of 4096 15.9 us and one of 1500 9.3, where what counts is the chain of plan, page ids, copies,
-// one or two steps, folding and the second launch.  24 sequences of 5 drafted tokens, 32 and 8 heads of 128, up to 6000 positions: 44 us.
+// query and 8 key/value heads of 64: 64 sequences of 200 to 32768 positions 125 us for 476 MB, 3.8 TB/s (2.0 instructions a clock and SM;
+// streaming the records alone 87 us); 8 sequences of 4096 16.2 us and one of 1500 9.3, where what counts is the chain of plan, page ids,
+// copies, one or two steps, folding and the second launch.  24 sequences of 5 drafted tokens, 32 and 8 heads of 128, up to 6000 positions:
+// 46 us, 1.0 instructions a clock and SM: latency, with eight warps at 255 registers.
 #pragma once
 #include "kv4_common.cuh"
 #include "sm100_ptx.cuh"

@@ -87,14 +87,14 @@ constexpr int kSms = 148, kSharedPerSm = 227 * 1024;
 
 // Columns of an item's products, in groups of eight.  More of them read, convert and scale the cache less often; fewer need fewer
 // registers, so that two CTAs fit a multiprocessor.  64 sequences of 4000 positions, 8 key/value heads, us by groups of columns:
-//   heads of 64    8 rows an item: 46 (1), 101 (4)    16 rows: 80 (1), 86 (2), 107 (4)    32 rows: 143 (1), 146 (2), 111 (4)
-//   heads of 128   8 rows: 77 (1), 102 (2)            16 rows: 142 (1), 106 (2)
+//   heads of 64    8 rows an item: 48 (1), 104 (4)    16 rows: 82 (1), 108 (4)    32 rows: 146 (1), 113 (4)
+//   heads of 128   8 rows: 79 (1), 104 (2)            16 rows: 143 (1), 109 (2)
 int column_groups(const Shape& s, int max_rows) {
     const long long rows = (long long)std::max(max_rows, 1) * (s.nq / s.nkv);
     if (s.D == 128) return rows <= 8 ? 1 : 2;
     return rows <= 16 ? 1 : 4;
 }
-// one instead of two, with eight rows of 64: 54 us instead of 46
+// one instead of two, with eight rows of 64: 56 us instead of 48, with sixteen 102 instead of 82
 int ctas_per_sm(const Shape& s, int nt) { return s.D == 64 && nt == 1 ? 2 : 1; }
 // steps that there can be in all, as the table's width bounds the lengths
 long long most_units(const Shape& s, const Batch& b, int nt) {
@@ -135,16 +135,20 @@ cudaError_t attend_variant(const AttendParams* run, cudaStream_t st, bool pdl, b
     with_pdl(pdl_merge, merge_kernel<DIM>, (unsigned)((tasks + 7) / 8), 256, plan, st, p);
     return cudaSuccess;
 }
-// Chunks of prompts: 256 rows of a key/value head at a time on tcgen05.  Heads of 64 only: at 128 columns queries, operands
-// and outputs would not fit a CTA.  An item walks its positions alone, 1.2 to 1.5 us a step of 64, whether or not there is work for
+// Chunks of prompts: 256 rows of a key/value head at a time on tcgen05.  Heads of 64 only: the kernel's three operand stages and
+// second query term would not fit a CTA at 128 columns (one with two stages, for bf16 queries, would), and those go to the other
+// kernel, 1910 us for two chunks of 2048 rows over up to 8192 positions, 32 and 8 heads.  An item walks its positions alone, 1.2 to 1.5 us a step of 64, whether or not there is work for
 // the other multiprocessors; the other kernel splits steps evenly over all of them, 2.9 ns a step of 32 rows.  So the first is faster
-// from about 480 blocks of 32 rows for every wave of items on.  At 8 key/value heads and 4096 positions (other kernel, this one):
-//   8 sequences of 128 rows (256 blocks, 1 wave)     65,  93 us       of 256 rows (512 blocks)            112,  80 us
-//   32 sequences of 64 rows (512 blocks, 2 waves)   112, 216 us       of 128 rows (1024 blocks, 2 waves)  206, 184 us
-//   one sequence of 512 rows (128 blocks, 1 wave)    39,  80 us
-// Where a window leaves a few steps only, the other kernel's split and its second launch cost more than they bring: window 128,
-// 32 sequences of 64 rows 33, 24 us; 8 sequences of 512 rows 41, 13 us; 64 sequences of 16 rows 24, 46 us (few rows: the products'
-// tiles are nearly empty).
+// from about 480 blocks of 32 rows for every wave of items on.  At 8 query and key/value heads and 4096 positions (other kernel, this one):
+//   8 sequences of 128 rows (256 blocks, 1 wave)     65,  94 us       of 256 rows (512 blocks)            111,  82 us
+//   32 sequences of 64 rows (512 blocks, 2 waves)   112, 216 us       of 128 rows (1024 blocks, 2 waves)  206, 187 us
+//   one sequence of 512 rows (128 blocks, 1 wave)    38,  79 us
+// Where a window leaves a few steps only, the other kernel's split and its second launch cost more than they bring.  Windows of 64, 128,
+// 256, 448, 512, 1024, us:
+//   32 sequences of 64 rows       23, 24   36, 26   43, 32   50, 40   46, 43   63, 69
+//   8 sequences of 128 rows       21, 15   18, 17   30, 20   28, 23   33, 25   36, 36
+//   one sequence of 512 rows      18, 19   22, 21   22, 23   24, 27   24, 28   29, 37
+// Below 64 rows the products' tiles are nearly empty: 64 sequences of 16 rows, window 128, 22, 46 us.
 constexpr int kPrefillRows = 64, kPrefillSpan = 512, kPrefillBlocks = 480;
 bool prefills(const Shape& s, const Batch& b, int max_rows, int window) {
     const int G = s.nq / s.nkv;

@@ -87,7 +87,8 @@ int launch(const void* logits, int dtype, long long row_stride, int vocab, int b
     p.heads = reinterpret_cast<ChunkHead*>(p.entries + n * kSlots);
     p.left = reinterpret_cast<int*>(p.heads + n);
     // A warp lists some 1.4 times as many elements as lanes' maxima pass its bound.  Longer lists let pick settle more rows, but all
-    // warps' together have to fit its list.
+    // warps' together have to fit its list.  64 rows with all filters, us by lanes' maxima (16, 8): 98 chunks 35, 71; 147 39, 37; 197 43, 40;
+    // 256 47, 44; 293 438, 51.  From 147 to 220 both settle such rows, and 16 reaches deeper.
     p.rank = p.chunks <= 220 ? 16 : 8;
     const unsigned grid = (unsigned)std::min<size_t>((n + kScanWarps - 1) / kScanWarps, 2 * kSms);
     void (*scan)(Params) = dtype == NEON_SAMPLER_F32 ? scan_kernel<0> : dtype == NEON_SAMPLER_BF16 ? scan_kernel<1> : scan_kernel<2>;

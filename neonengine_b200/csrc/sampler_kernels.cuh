@@ -14,9 +14,10 @@
 // Weights are integers of 2^-43 of the largest, so that sums depend on no order; a histogram keeps them as three words
 // of 15 bits each per element, which shared memory can add atomically.
 //
-// What bounds them, with 201088 fp32 logits a row.  scan: issue slots and the f64 units, for weights (256 rows 74 us with pick, 2.8 TB/s; without
-// sums it would be 38).  pick: a chain of barriers and of searches in shared memory, one CTA a row (1 row 17 us; 256 rows without
-// filters 8).  whole: the same and a histogram with two or three shared memory atomics an element; a few rows take 55 us, however few.
+// What bounds them, with 201088 fp32 logits a row.  scan: issue slots and the f64 units, for weights (256 rows 74 us with pick, 2.8 TB/s, 2.3
+// instructions a clock and SM; without sums it would be 38; 16-bit logits take as long, 79).  pick: a chain of barriers and of
+// searches in shared memory, one CTA a row (1 row 17 us; 256 rows without filters 8).  whole: the same and a histogram with two or three
+// shared memory atomics an element; a few rows take 55 us, however few.
 #pragma once
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>

@@ -148,7 +148,8 @@ class Kv4Cache:
                out=None, stream=None):
         """Attention of ``q`` [rows, n_q_heads, head_dim] (bf16 or fp16, rotated) over the cache; ``sinks``: bf16 [n_q_heads] logits of the
         softmax denominator; ``window`` > 0: only the last so many positions; ``scale``: default head_dim ** -0.5; ``max_rows``: the
-        most rows of a sequence, if the host knows it (speed only)."""
+        most rows of a sequence, as far as the host knows it; it chooses the kernel.  Without it a batch with row offsets counts as one
+        sequence of all rows: a batch of 64 single tokens then takes twice as long as with ``max_rows=1``."""
         if stream is not None:
             return self._on(stream, self.attend, batch, cache, q, sinks, window, scale, max_rows, out)
         rows, dtype = q.shape[0], q.dtype
