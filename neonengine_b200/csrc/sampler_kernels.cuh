@@ -822,7 +822,8 @@ __global__ void __launch_bounds__(kPickThreads) pick_kernel(const Params p, int 
         // the listed elements, side by side
         const uint32_t at = (uint32_t)prefix(mine.listed, s.scratch, n64);
         prefix(chunk_units(mine, weight), s.scratch, whole);
-        fits = n64 > 0 && n64 <= kList;
+        // (a bound above the largest: too many tokens share that for its stretch to list them, whatever other stretches list)
+        fits = n64 > 0 && n64 <= kList && !(bound > top);
         if (fits) {
             uint32_t* starts = &s.hist[0][0];  // where each chunk's entries go, and how many they are
             if (tid < p.chunks) {

@@ -97,3 +97,29 @@ def test_temperatures_whose_scale_leaves_f32(vocab, t):
     token, prob, kept = run(s, x, u, temperature=temperature, top_p=f32([0.4] * 6))  # reached by the second of them
     assert token == [zeros[int(v * 2)] for v in u] and kept == [2] * 6
     s.close()
+
+
+@pytest.mark.parametrize("t", [1.0, 0.3, 1e-30, 7.0])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+def test_largest_logits_that_no_list_holds(t, dtype):
+    """Thousands of equal largest logits fill stretches of their own; the only listed tokens weigh little or nothing."""
+    from neonengine_b200.sampler import Sampler
+    import sampler_reference as ref
+    vocab = 20011
+    x = torch.full((7, vocab), -60.0, device=DEV)
+    x[:, 100:150] = -55.0            # fifty that a stretch lists
+    x[:, 10240:14336] = 0.0          # 4096 that none can
+    x[:, 11000] = -0.0
+    x[3:, 3000:3020] = -1.0          # some more, of weight
+    x = x.to(dtype)
+    u = [0.0, 0.3, 0.77, 0.9, 1 - 2.0 ** -24, 0.55, 0.1234]
+    s, rows = Sampler(vocab), x.double().cpu().numpy()
+    for k, p, m in ((0, 0.3, 0.0), (0, 0.9, 0.0), (0, 0.001, 0.0), (0, 1.0, 1.0), (0, 1.0, 0.99), (0, 0.9, 1.0), (0, 0.3, 1e-6), (100, 1.0, 0.0), (5000, 0.3, 0.5)):
+        n = x.shape[0]
+        token, prob, kept = run(s, x, u, temperature=f32([t] * n), top_k=torch.full((n,), k, dtype=torch.int32, device=DEV),
+                                top_p=f32([p] * n), min_p=f32([m] * n))
+        for b in range(n):
+            want = ref.draw(rows[b], float(np.float32(u[b])), float(np.float32(t)), k, float(np.float32(p)), float(np.float32(m)))
+            assert (token[b], kept[b]) == (want[0], want[2]), (k, p, m, b, token[b], kept[b], want)
+            assert abs(prob[b] - want[1]) <= 2 ** -24 * want[1] * 1.01 + 1e-9
+    s.close()
